@@ -20,7 +20,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libalphasparse_b200.so")
 SYNTH_SRC = os.path.join(HERE, "synth", "synth.c")
 SYNTH_LIB = os.path.join(HERE, "synth", "libsynth.so")
-CUDA_SOURCES = ["core.cu", "spmv.cu", "spmv_band.cu", "spmv_bins.cu", "spmm.cu", "exchange.cu", "coo2csr.cu", "transfer.cu", "host_util.cu", "host_args.cu"]
+CUDA_SOURCES = ["core.cu", "spmv.cu", "spmv_band.cu", "spmv_bins.cu", "spmm.cu", "exchange.cu", "coo2csr.cu", "transfer.cu", "host_util.cu", "host_args.cu",
+                "embedding.cu", "route.cu", "experts.cu"]
 
 
 def _newer(target, deps):
@@ -41,7 +42,7 @@ def nvcc_path():
 
 def build_library(force=False, verbose_ptxas=False):
     srcs = [os.path.join(CSRC, s) for s in CUDA_SOURCES]
-    deps = srcs + [os.path.join(CSRC, h) for h in ("internal.h", "index_bounds.h")] + [
+    deps = srcs + [os.path.join(CSRC, h) for h in ("internal.h", "index_bounds.h", "rows.h")] + [
         os.path.join(ROOT, "include", "alphasparse", h)
         for h in os.listdir(os.path.join(ROOT, "include", "alphasparse"))
     ]

@@ -28,6 +28,10 @@ FORMAT_COO, FORMAT_CSR, FORMAT_CSC = 0, 1, 2
 FLOAT, DOUBLE, FLOAT_COMPLEX, DOUBLE_COMPLEX = 0, 1, 2, 3
 # alphasparse_cuda_alg_t
 ALG_AUTO, ALG_VECTOR, ALG_MERGE, ALG_ROWTILE = 0, 1, 2, 3
+# alphasparse_cuda_type_t / alphasparse_cuda_index_t / alphasparse_cuda_score_t
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+INDEX_I32, INDEX_I64 = 0, 1
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 
 
 class MatrixDescr(C.Structure):
@@ -115,6 +119,17 @@ def prototypes():
     p["alphasparse_cuda_exchange_destroy"] = (C.c_int, [_H])
     p["alphasparse_s_mv_exchange"] = (C.c_int, [C.c_float, _H, MatrixDescr, _H, C.c_float, _P])
     p["alphasparse_d_mv_exchange"] = (C.c_int, [C.c_double, _H, MatrixDescr, _H, C.c_double, _P])
+    _L, _F, _Z = C.c_int64, C.c_float, C.c_size_t
+    p["alphasparse_cuda_embedding"] = (C.c_int, [C.c_int, C.c_int, _L, _P, _L, _L, _L, _F, _P, _L, _P, _L])
+    p["alphasparse_cuda_embedding_grad_buffer_size"] = (C.c_int, [_L, _L, _L, C.POINTER(_Z)])
+    p["alphasparse_cuda_embedding_grad"] = (C.c_int, [C.c_int, C.c_int, C.c_int, _L, _P, _L, _L, _L, _F, _P, _L, _F, _P, _L, _P, _Z])
+    p["alphasparse_cuda_route"] = (C.c_int, [C.c_int, C.c_int, _L, _L, _P, _L, _P, _L, _L, _L, C.c_int, _F, _P, _L, _P, _L])
+    p["alphasparse_cuda_route_grad"] = (C.c_int, [C.c_int, C.c_int, _L, _L, _P, _L, _L, _P, _L, C.c_int, _F, _P, _L, _P, _L])
+    p["alphasparse_cuda_expert_plan_buffer_size"] = (C.c_int, [_L, _L, _L, C.POINTER(_Z)])
+    p["alphasparse_cuda_expert_plan"] = (C.c_int, [_L, _L, _L, _P, _L, _P, _P, _L, _P, _Z])
+    p["alphasparse_cuda_expert_dispatch"] = (C.c_int, [C.c_int, _L, _L, _L, _P, _L, _P, _L, _L, _P, _L])
+    p["alphasparse_cuda_expert_combine"] = (C.c_int, [C.c_int, _L, _L, _L, _L, _P, _L, _P, _L, _P, _L, _F, _P, _L])
+    p["alphasparse_cuda_expert_combine_grad"] = (C.c_int, [C.c_int, _L, _L, _L, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L])
     p["alphasparse_cuda_kernel_status"] = (C.c_int, [_H, C.POINTER(C.c_int), C.c_int])
     p["alphasparse_cuda_profile_kernel"] = (C.c_int, [_H, C.c_int])
     p["alphasparse_cuda_kernel_ms"] = (C.c_int, [_H, C.POINTER(C.c_float)])

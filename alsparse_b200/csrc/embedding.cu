@@ -1,0 +1,436 @@
+// Embedding lookup and the gradient of its table: Y = scale S E and dE = alpha S^T dY + beta dE, S the one-hot matrix of
+// the tokens.  S is never stored: the lookup reads the tokens, the gradient sorts their positions by token (the transpose
+// of S in CSR form, made for one product) and sums the rows of dY run by run.  No counterpart in the reference.
+#include <stdio.h>
+
+#include <algorithm>
+
+#include "rows.h"
+
+namespace asb {
+
+// ---- checks shared by the operators on rows ----------------------------------------------------
+
+// true when `p` is memory the kernels of device `dev` can use: allocated on that device, or managed
+static bool memory_of(const void *p, int dev) {
+    cudaPointerAttributes at;
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return false;
+    }
+    if (at.type == cudaMemoryTypeManaged) return true;
+    return at.type == cudaMemoryTypeDevice && at.device == dev;
+}
+
+alphasparse_status_t check_operands(const char *call, std::initializer_list<Operand> operands) {
+    char msg[200];
+    for (const Operand &o : operands) {
+        if (o.empty()) continue;
+        if (!o.p) return ALPHA_SPARSE_STATUS_NOT_INITIALIZED;
+        if (o.ld > kMostStride || (o.rows > 1 && o.ld < o.width) || o.begin() % o.elem) {
+            snprintf(msg, sizeof(msg), "%s: a leading dimension below the width or above 2^31 - 1, or an address that is no multiple of the element's size", call);
+            record_error(msg);
+            return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+        }
+    }
+    for (const Operand *a = operands.begin(); a != operands.end(); a++)
+        for (const Operand *b = operands.begin(); b != a; b++)
+            if ((a->written || b->written) && !a->empty() && !b->empty() && a->begin() < b->end() && b->begin() < a->end()) {
+                snprintf(msg, sizeof(msg), "%s: an output lies in the place of another operand", call);
+                record_error(msg);
+                return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+            }
+    int dev = -1;
+    ASB_CUDA_OR(cudaGetDevice(&dev), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    for (const Operand &o : operands)
+        if (!o.empty() && !memory_of(o.p, dev)) {
+            snprintf(msg, sizeof(msg), "%s takes pointers to memory of the current device only", call);
+            record_error(msg);
+            return ALPHA_SPARSE_STATUS_INVALID_POINTER;
+        }
+    return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+
+// ---- lookup --------------------------------------------------------------------------------------
+
+template <typename T, typename I, int N, int U>
+__global__ void __launch_bounds__(kRowThreads)
+    embedding_kernel(int rows, const I *__restrict__ token, int64_t inctoken, int64_t vocab, int nv, float scale,
+                     const T *__restrict__ table, int64_t ldt, T *__restrict__ y, int64_t ldy, int log) {
+    const int64_t r = (int64_t)blockIdx.x * (kRowThreads >> log) + (threadIdx.x >> log);
+    if (r >= rows) return;
+    const int64_t t = (int64_t)token[r * inctoken];
+    const bool inside = t >= 0 && t < vocab;
+    const T *src = table + (inside ? t : 0) * ldt;
+    T *dst = y + r * ldy;
+    const int v0 = (int)(blockIdx.y * (U << log) + (threadIdx.x & ((1 << log) - 1)));
+    Pack<T, N> p[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int v = v0 + (u << log);
+        p[u] = inside && v < nv ? load_pack<T, N>(src + (int64_t)v * N) : zero_pack<T, N>();
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int v = v0 + (u << log);
+        if (inside && scale != 1.f) {
+#pragma unroll
+            for (int i = 0; i < N; i++) p[u].v[i] = from_float<T>(to_float(p[u].v[i]) * scale);
+        }
+        if (v < nv) store_pack<T, N>(dst + (int64_t)v * N, p[u]);
+    }
+}
+
+// ---- gradient ------------------------------------------------------------------------------------
+
+constexpr int kGradRows = 512;     // table rows whose tokens one block of the sort collects
+constexpr int kGradSortWarps = 32;
+constexpr int kGradPiece = 32;     // sorted positions one block of the sum walks
+constexpr int kGradThreads = 128;
+
+// Positions sorted by token, stable, in one launch.  A block owns kGradRows rows of the table and reads every token:
+// a warp takes one contiguous share of them, counts those of each of the block's rows, and after the prefix over warps
+// and rows reads its share again and writes the positions to where they belong.  Tokens below the block's rows are
+// counted on the way, so that no block waits for another.
+template <typename I>
+__global__ void __launch_bounds__(kGradSortWarps * 32)
+    tokens_by_row_kernel(int tokens, const I *__restrict__ token, int64_t inctoken, int vocab, int *__restrict__ ptr,
+                         int *__restrict__ pos, int *__restrict__ row) {
+    extern __shared__ int s_count[];  // [warp][row]
+    __shared__ int s_sum[kGradSortWarps], s_below[kGradSortWarps];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int base = blockIdx.x * kGradRows;
+    const int mine = min(kGradRows, vocab - base);
+    for (int i = threadIdx.x; i < kGradSortWarps * kGradRows; i += blockDim.x) s_count[i] = 0;
+    __syncthreads();
+    const int share = (int)(((int64_t)tokens + kGradSortWarps * 32 - 1) / (kGradSortWarps * 32)) * 32;
+    const int64_t begin = min((int64_t)tokens, (int64_t)w * share), end = min((int64_t)tokens, begin + share);
+    int *count = s_count + w * kGradRows;
+    int below = 0;
+    for (int64_t i0 = begin; i0 < end; i0 += 128) {
+        int64_t t[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int64_t i = i0 + u * 32 + lane;
+            t[u] = i < end ? (int64_t)token[i * inctoken] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (t[u] >= 0 && t[u] < base) below++;
+            else if (t[u] >= base && t[u] < base + mine) atomicAdd(&count[t[u] - base], 1);
+        }
+    }
+    below = __reduce_add_sync(0xffffffffu, below);
+    if (lane == 0) s_below[w] = below;
+    __syncthreads();
+    int start = 0;
+    for (int v = 0; v < kGradSortWarps; v++) start += s_below[v];
+    int total = 0;
+    if (threadIdx.x < kGradRows)
+        for (int v = 0; v < kGradSortWarps; v++) {
+            const int c = s_count[v * kGradRows + threadIdx.x];
+            s_count[v * kGradRows + threadIdx.x] = total;
+            total += c;
+        }
+    int inc = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int n = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += n;
+    }
+    if (lane == 31) s_sum[w] = inc;
+    __syncthreads();
+    for (int v = 0; v < w; v++) start += s_sum[v];
+    start += inc - total;
+    if ((int)threadIdx.x < kGradRows) {
+        for (int v = 0; v < kGradSortWarps; v++) s_count[v * kGradRows + threadIdx.x] += start;
+        if ((int)threadIdx.x < mine) ptr[base + threadIdx.x] = start;
+        if (base + (int)threadIdx.x == vocab - 1) ptr[vocab] = start + total;
+    }
+    __syncthreads();
+    for (int64_t i0 = begin; i0 < end; i0 += 128) {
+        int64_t t[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int64_t i = i0 + u * 32 + lane;
+            t[u] = i < end ? (int64_t)token[i * inctoken] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const bool in = t[u] >= base && t[u] < base + mine;
+            if (!__any_sync(0xffffffffu, in)) continue;
+            const int r = in ? (int)(t[u] - base) : -1;
+            const unsigned same = __match_any_sync(0xffffffffu, r);
+            const int lower = __popc(same & ((1u << lane) - 1u));
+            const int at = in ? count[r] + lower : 0;
+            __syncwarp();
+            if (in) {
+                pos[at] = (int)(i0 + u * 32 + lane);
+                row[at] = base + r;
+                if (lower == 0) count[r] += __popc(same);
+            }
+            __syncwarp();
+        }
+    }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void finish_row(T *p, const float (&acc)[N], float alpha, float beta) {
+    Pack<T, N> out;
+    if (beta != 0.f) out = *reinterpret_cast<const Pack<T, N> *>(p);
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        out.v[i] = from_float<T>(beta != 0.f ? fmaf(alpha, acc[i], beta * to_float(out.v[i])) : alpha * acc[i]);
+    store_pack<T, N>(p, out);
+}
+
+// Block (piece, column tile): walks kGradPiece sorted positions, eight rows of dY requested at a time, and adds up runs of
+// one token in 32 bits, in the order of the tokens.  A run that begins and ends in the piece is finished here; what
+// the piece holds of others goes to the partial sums (first slot: of the run that came in, second: of the one that goes on).
+// The blocks behind take the table's rows that no token names: zeros for beta = 0, beta times what is there else.
+template <typename T, typename TO, int N>
+__global__ void __launch_bounds__(kGradThreads)
+    embedding_grad_kernel(int pieces, int tiles, int nv, int vocab, const int *__restrict__ ptr, const int *__restrict__ pos,
+                          const int *__restrict__ row, const T *__restrict__ dy, int64_t lddy, float alpha, float beta,
+                          TO *__restrict__ dtable, int64_t ldt, float *__restrict__ partial, int64_t ldp) {
+    const int64_t sums = (int64_t)pieces * tiles;
+    if (blockIdx.x >= sums) {
+        const int first = (int)(blockIdx.x - sums) * 8;
+        const float zero[N] = {};
+        for (int r = first; r < min(vocab, first + 8); r++) {
+            if (ptr[r] != ptr[r + 1]) continue;
+            for (int v = threadIdx.x; v < nv; v += kGradThreads) finish_row<TO, N>(dtable + (int64_t)r * ldt + (int64_t)v * N, zero, 0.f, beta);
+        }
+        return;
+    }
+    __shared__ int s_pos[kGradPiece], s_row[kGradPiece + 2];
+    const int piece = blockIdx.x / tiles, tile = blockIdx.x - piece * tiles;
+    const int count = ptr[vocab], begin = piece * kGradPiece, n = min(kGradPiece, count - begin);
+    if (n <= 0) return;
+    const int lane = threadIdx.x;
+    if (lane < kGradPiece + 2) {
+        const int i = begin + lane - 1;
+        s_row[lane] = i >= 0 && i < count ? row[i] : -1;
+        if (lane < n) s_pos[lane] = pos[begin + lane];
+    }
+    __syncthreads();
+    const int v = tile * kGradThreads + lane;
+    if (v >= nv) return;
+    const T *src = dy + (int64_t)v * N;
+    float acc[N] = {};
+    bool came_in = s_row[0] == s_row[1];
+    constexpr int kAhead = 8;
+    for (int i0 = 0; i0 < n; i0 += kAhead) {
+        Pack<T, N> p[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++)
+            if (i0 + u < n) p[u] = load_pack<T, N>(src + s_pos[i0 + u] * lddy);
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            const int i = i0 + u;
+            if (i >= n) break;
+#pragma unroll
+            for (int k = 0; k < N; k++) acc[k] += to_float(p[u].v[k]);
+            const bool ends = s_row[i + 1] != s_row[i + 2];
+            if (!ends && i + 1 < n) continue;
+            if (ends && !came_in) {
+                finish_row<TO, N>(dtable + (int64_t)s_row[i + 1] * ldt + (int64_t)v * N, acc, alpha, beta);
+            } else {
+                float *to = partial + ((int64_t)piece * 2 + (came_in ? 0 : 1)) * ldp + (int64_t)v * N;
+#pragma unroll
+                for (int k = 0; k < N; k++) to[k] = acc[k];
+            }
+            came_in = false;
+#pragma unroll
+            for (int k = 0; k < N; k++) acc[k] = 0.f;
+        }
+    }
+}
+
+// Runs that cross pieces: the block of the piece in which such a run begins adds its partial sums, a share of the pieces
+// per warp, the warps' sums in their order.  The order is fixed, so the result does not change from call to call.
+constexpr int kJoinWarps = 8;
+template <typename TO>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+    embedding_grad_join_kernel(int width, int vocab, const int *__restrict__ ptr, const int *__restrict__ row, float alpha,
+                               float beta, TO *__restrict__ dtable, int64_t ldt, const float *__restrict__ partial, int64_t ldp) {
+    __shared__ float4 s_sum[kJoinWarps][32];
+    const int piece = blockIdx.x, last = (piece + 1) * kGradPiece - 1;
+    if (last + 1 >= ptr[vocab]) return;
+    const int r = row[last];
+    if (row[last + 1] != r || ptr[r] < piece * kGradPiece) return;
+    const int first = piece + 1, pieces = (ptr[r + 1] - 1) / kGradPiece - piece;  // pieces behind this one
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int share = (pieces + kJoinWarps - 1) / kJoinWarps, begin = min(pieces, w * share), end = min(pieces, begin + share);
+    for (int c0 = blockIdx.y * 128; c0 < width; c0 += gridDim.y * 128) {
+        const int c = c0 + lane * 4;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < width) {
+            if (w == 0) acc = *reinterpret_cast<const float4 *>(partial + ((int64_t)piece * 2 + 1) * ldp + c);
+#pragma unroll 4
+            for (int i = begin; i < end; i++) {
+                const float4 p = *reinterpret_cast<const float4 *>(partial + (int64_t)(first + i) * 2 * ldp + c);
+                acc.x += p.x, acc.y += p.y, acc.z += p.z, acc.w += p.w;
+            }
+        }
+        s_sum[w][lane] = acc;
+        __syncthreads();
+        if (threadIdx.x < 128 && c0 + (int)threadIdx.x < width) {
+            float sum[1] = {0.f};
+            for (int v = 0; v < min(kJoinWarps, pieces); v++) sum[0] += reinterpret_cast<const float *>(s_sum[v])[threadIdx.x];
+            finish_row<TO, 1>(dtable + (int64_t)r * ldt + c0 + threadIdx.x, sum, alpha, beta);
+        }
+        __syncthreads();
+    }
+}
+
+// The pieces of the workspace, each on a 256-byte boundary
+struct GradSpace {
+    size_t ptr, pos, row, partial, bytes;
+    int64_t pieces, ldp;
+    GradSpace(int64_t tokens, int64_t vocab, int64_t width) {
+        const auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+        pieces = (tokens + kGradPiece - 1) / kGradPiece;
+        ldp = (width + 3) & ~(int64_t)3;
+        ptr = 0;
+        pos = up(sizeof(int) * ((size_t)vocab + 1));
+        row = pos + up(sizeof(int) * (size_t)tokens);
+        partial = row + up(sizeof(int) * (size_t)tokens);
+        bytes = partial + up(sizeof(float) * 2 * (size_t)pieces * (size_t)ldp);
+    }
+};
+
+static bool grad_sizes_fit(int64_t tokens, int64_t vocab, int64_t width) {
+    return tokens >= 0 && tokens <= kMostRows && vocab >= 0 && vocab <= kMostRows && width >= 0 && width <= kMostWidth;
+}
+
+template <typename T, typename TO>
+static cudaError_t launch_grad_sums(const GradSpace &sp, char *buffer, int64_t tokens, int64_t vocab, int64_t width, float alpha,
+                                    const T *dy, int64_t lddy, float beta, TO *dtable, int64_t ldt, cudaStream_t st) {
+    int *ptr = reinterpret_cast<int *>(buffer + sp.ptr), *pos = reinterpret_cast<int *>(buffer + sp.pos),
+        *row = reinterpret_cast<int *>(buffer + sp.row);
+    float *partial = reinterpret_cast<float *>(buffer + sp.partial);
+    const int vb = vector_bytes(sizeof(T), {address(dy), (uint64_t)lddy * sizeof(T), (uint64_t)width * sizeof(T)});
+    const int vo = vector_bytes(sizeof(TO), {address(dtable), (uint64_t)ldt * sizeof(TO), (uint64_t)width * sizeof(TO)});
+    const auto go = [&](auto n) {
+        constexpr int N = decltype(n)::value;
+        const int nv = (int)(width / N), tiles = (nv + kGradThreads - 1) / kGradThreads;
+        const int64_t blocks = sp.pieces * tiles + (beta == 1.f ? 0 : (vocab + 7) / 8);
+        if (blocks <= 0) return cudaSuccess;
+        if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+        embedding_grad_kernel<T, TO, N><<<(unsigned)blocks, kGradThreads, 0, st>>>(
+            (int)sp.pieces, tiles, nv, (int)vocab, ptr, pos, row, dy, lddy, alpha, beta, dtable, ldt, partial, sp.ldp);
+        return cudaGetLastError();
+    };
+    cudaError_t e;
+    constexpr int full = 16 / sizeof(T);
+    // a pack of the input becomes one of as many elements of the output: both have to allow it
+    if (vb == 16 && vo == 16) e = go(std::integral_constant<int, full>{});
+    else if (sizeof(T) == 2 && vb >= 4 && vo >= 2 * (int)sizeof(TO)) e = go(std::integral_constant<int, 2>{});
+    else e = go(std::integral_constant<int, 1>{});
+    if (e != cudaSuccess) return e;
+    count_launch();
+    if (sp.pieces > 1) {
+        const unsigned tiles = (unsigned)std::min<int64_t>(8, (width + 127) / 128);
+        embedding_grad_join_kernel<TO><<<dim3((unsigned)sp.pieces - 1, tiles), kJoinWarps * 32, 0, st>>>(
+            (int)width, (int)vocab, ptr, row, alpha, beta, dtable, ldt, partial, sp.ldp);
+        count_launch();
+    }
+    return cudaGetLastError();
+}
+
+}  // namespace asb
+
+using namespace asb;
+
+extern "C" alphasparse_status_t alphasparse_cuda_embedding(alphasparse_cuda_index_t index_type, alphasparse_cuda_type_t type,
+                                                           int64_t tokens, const void *token, int64_t inctoken, int64_t vocab,
+                                                           int64_t width, float scale, const void *table, int64_t ldt, void *y,
+                                                           int64_t ldy) {
+    const size_t ib = index_bytes(index_type), eb = type_bytes(type);
+    if (!ib || !eb || !grad_sizes_fit(tokens, vocab, width) || inctoken < 1) return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    if (tokens == 0 || width == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
+    const alphasparse_status_t s = check_operands("alphasparse_cuda_embedding", {{token, tokens, 1, inctoken, ib, false},
+                                                                               {table, vocab, width, ldt, eb, false},
+                                                                               {y, tokens, width, ldy, eb, true}});
+    if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+    const int vb = vector_bytes(eb, {address(table), (uint64_t)ldt * eb, address(y), (uint64_t)ldy * eb, (uint64_t)width * eb});
+    const int64_t nv = width * (int64_t)eb / vb;
+    const RowShape shape = row_shape(tokens, nv);
+    cudaStream_t st = current_stream();
+    const auto run = [&](auto t) {
+        using T = decltype(t);
+        const auto with_index = [&](auto i) {
+            using I = decltype(i);
+            with_pack<T>(vb, [&](auto n) {
+                constexpr int N = decltype(n)::value;
+                const auto kernel = shape.unroll == 1 ? embedding_kernel<T, I, N, 1> : embedding_kernel<T, I, N, 4>;
+                kernel<<<shape.grid, kRowThreads, 0, st>>>((int)tokens, (const I *)token, inctoken, vocab, (int)nv, scale,
+                                                         (const T *)table, ldt, (T *)y, ldy, shape.log);
+            });
+        };
+        if (index_type == ALPHA_SPARSE_CUDA_INDEX_I32) with_index((int32_t)0);
+        else with_index((int64_t)0);
+    };
+    ASB_BY_TYPE(type, run)
+    count_launch();
+    ASB_CUDA_OR(cudaGetLastError(), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+
+extern "C" alphasparse_status_t alphasparse_cuda_embedding_grad_buffer_size(int64_t tokens, int64_t vocab, int64_t width,
+                                                                           size_t *bytes) {
+    if (!bytes) return ALPHA_SPARSE_STATUS_NOT_INITIALIZED;
+    if (!grad_sizes_fit(tokens, vocab, width)) return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    *bytes = GradSpace(tokens, vocab, width).bytes;
+    return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+
+extern "C" alphasparse_status_t alphasparse_cuda_embedding_grad(alphasparse_cuda_index_t index_type, alphasparse_cuda_type_t type,
+                                                                alphasparse_cuda_type_t table_type, int64_t tokens,
+                                                                const void *token, int64_t inctoken, int64_t vocab,
+                                                                int64_t width, float alpha, const void *dy, int64_t lddy,
+                                                                float beta, void *dtable, int64_t ldt, void *buffer,
+                                                                size_t buffer_bytes) {
+    const size_t ib = index_bytes(index_type), eb = type_bytes(type), ob = type_bytes(table_type);
+    if (!ib || !eb || !ob || !grad_sizes_fit(tokens, vocab, width) || inctoken < 1) return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    if (table_type != type && table_type != ALPHA_SPARSE_CUDA_TYPE_F32) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+    if (vocab == 0 || width == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
+    const GradSpace sp(tokens, vocab, width);
+    if (buffer && (buffer_bytes < sp.bytes || address(buffer) % 16)) {
+        record_error("alphasparse_cuda_embedding_grad: the workspace is smaller than alphasparse_cuda_embedding_grad_buffer_size says, or not on a 16-byte boundary");
+        return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    }
+    const alphasparse_status_t s = check_operands(
+        "alphasparse_cuda_embedding_grad", {{token, tokens, 1, inctoken, ib, false},
+                                            {dy, tokens, width, lddy, eb, false},
+                                            {dtable, vocab, width, ldt, ob, true},
+                                            {buffer, 1, (int64_t)sp.bytes, (int64_t)0, 1, true}});
+    if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+    cudaStream_t st = current_stream();
+    char *space = static_cast<char *>(buffer);
+    int *ptr = reinterpret_cast<int *>(space + sp.ptr), *pos = reinterpret_cast<int *>(space + sp.pos),
+        *row = reinterpret_cast<int *>(space + sp.row);
+    const unsigned blocks = (unsigned)((vocab + kGradRows - 1) / kGradRows);
+    const size_t smem = sizeof(int) * kGradSortWarps * kGradRows;
+    const auto sort = [&](auto i) {
+        using I = decltype(i);
+        cudaError_t e = cudaFuncSetAttribute(tokens_by_row_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+        tokens_by_row_kernel<I><<<blocks, kGradSortWarps * 32, smem, st>>>((int)tokens, (const I *)token, inctoken, (int)vocab, ptr, pos, row);
+        return cudaGetLastError();
+    };
+    ASB_CUDA_OR(index_type == ALPHA_SPARSE_CUDA_INDEX_I32 ? sort((int32_t)0) : sort((int64_t)0), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    count_launch();
+    cudaError_t e = cudaSuccess;
+    const auto run = [&](auto t) {
+        using T = decltype(t);
+        if (table_type == ALPHA_SPARSE_CUDA_TYPE_F32)
+            e = launch_grad_sums<T, float>(sp, space, tokens, vocab, width, alpha, (const T *)dy, lddy, beta, (float *)dtable, ldt, st);
+        else
+            e = launch_grad_sums<T, T>(sp, space, tokens, vocab, width, alpha, (const T *)dy, lddy, beta, (T *)dtable, ldt, st);
+    };
+    ASB_BY_TYPE(type, run)
+    ASB_CUDA_OR(e, ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    return ALPHA_SPARSE_STATUS_SUCCESS;
+}

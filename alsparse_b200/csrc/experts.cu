@@ -1,0 +1,430 @@
+// Rows of tokens to their experts and back: the matrix of k entries per token that routing made, as a permutation (plan),
+// applied to the tokens' rows (dispatch), and with its weights to the experts' rows (combine, and the gradients).
+// No counterpart in the reference.
+//
+// The (token, choice) pairs stand in the order of their experts, and of the tokens within an expert; slot[t, j] is the row
+// of pair (t, j), -1 for an empty choice.  All that follows goes by slot: a token's row is read once and written to its k
+// places, or its k rows are read and written once.  Bound by HBM.
+#include <algorithm>
+
+#include "rows.h"
+
+namespace asb {
+
+// ---- plan ----------------------------------------------------------------------------------------
+
+constexpr int kPlanThreads = 512, kPlanWarps = kPlanThreads / 32;
+constexpr int kPlanKeys = 4096;    // pairs a block takes at least
+constexpr int kPlanMostBlocks = 256;
+
+// Exclusive prefix over the threads of the block; s_sum: one int per warp
+__device__ __forceinline__ int plan_scan(int v, int *s_sum) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    int inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int n = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += n;
+    }
+    if (lane == 31) s_sum[w] = inc;
+    __syncthreads();
+    int before = 0;
+    for (int i = 0; i < w; i++) before += s_sum[i];
+    __syncthreads();
+    return before + inc - v;
+}
+
+// A block takes a contiguous share of the pairs and each of its warps a contiguous share of that, counts the pairs of each
+// expert per warp, and (PLACE) after the prefix over experts, blocks and warps reads them again and places them.  With more
+// than one block a first launch writes the blocks' counts for the second to read.
+template <bool PLACE>
+__global__ void __launch_bounds__(kPlanThreads)
+    plan_kernel(int64_t pairs, int64_t share, int experts, int k, const int *__restrict__ index, int64_t ldi,
+                int *__restrict__ counts, int *__restrict__ offsets, int *__restrict__ slot, int64_t lds) {
+    extern __shared__ int s_count[];  // [warp][expert]
+    __shared__ int s_sum[kPlanWarps];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    for (int i = threadIdx.x; i < kPlanWarps * experts; i += kPlanThreads) s_count[i] = 0;
+    __syncthreads();
+    const int64_t first = blockIdx.x * share, last = min(pairs, first + share);
+    const int64_t part = (share / kPlanWarps + 31) / 32 * 32;
+    const int64_t begin = min(last, first + w * part), end = w == kPlanWarps - 1 ? last : min(last, begin + part);
+    int *count = s_count + w * experts;
+    const auto key_at = [&](int64_t i) {
+        if (i >= end) return -1;
+        const int64_t t = (int64_t)((unsigned)i / (unsigned)k);
+        const int e = index[t * ldi + (i - t * k)];
+        return e >= 0 && e < experts ? e : -1;
+    };
+    for (int64_t i0 = begin; i0 < end; i0 += 128) {
+        int e[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) e[u] = key_at(i0 + u * 32 + lane);
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (e[u] >= 0) atomicAdd(&count[e[u]], 1);
+    }
+    __syncthreads();
+    const int blocks = gridDim.x, b = blockIdx.x;
+    int carry = 0;
+    for (int e0 = 0; e0 < experts; e0 += kPlanThreads) {
+        const int e = e0 + threadIdx.x;
+        int mine = 0;
+        if (e < experts)
+            for (int v = 0; v < kPlanWarps; v++) {
+                const int c = s_count[v * experts + e];
+                s_count[v * experts + e] = mine;
+                mine += c;
+            }
+        if (!PLACE) {
+            if (e < experts) counts[(int64_t)b * experts + e] = mine;
+            continue;
+        }
+        int total = mine, before = 0;
+        if (blocks > 1 && e < experts) {
+            total = 0;
+#pragma unroll 8
+            for (int v = 0; v < blocks; v++) {
+                const int c = counts[(int64_t)v * experts + e];
+                before += v < b ? c : 0;
+                total += c;
+            }
+        }
+        const int start = carry + plan_scan(total, s_sum);
+        if (threadIdx.x == kPlanThreads - 1) s_sum[0] = start + total;
+        __syncthreads();
+        carry = s_sum[0];
+        __syncthreads();
+        if (e < experts) {
+            for (int v = 0; v < kPlanWarps; v++) s_count[v * experts + e] += start + before;
+            if (b == 0) {
+                offsets[e] = start;
+                if (e == experts - 1) offsets[experts] = start + total;
+            }
+        }
+    }
+    if (!PLACE) return;
+    __syncthreads();
+    for (int64_t i0 = begin; i0 < end; i0 += 128) {
+        int e[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) e[u] = key_at(i0 + u * 32 + lane);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int64_t i = i0 + u * 32 + lane;
+            const unsigned same = __match_any_sync(0xffffffffu, e[u]);
+            const int lower = __popc(same & ((1u << lane) - 1u));
+            int at = -1;
+            if (e[u] >= 0) at = count[e[u]] + lower;
+            __syncwarp();
+            if (e[u] >= 0 && lower == 0) count[e[u]] += __popc(same);
+            __syncwarp();
+            if (i < end) {
+                const int64_t t = (int64_t)((unsigned)i / (unsigned)k);
+                slot[t * lds + (i - t * k)] = at;
+            }
+        }
+    }
+}
+
+struct PlanShape {
+    int64_t pairs, share;
+    int blocks;
+    size_t bytes;
+    PlanShape(int64_t tokens, int64_t k, int64_t experts) {
+        pairs = tokens * k;
+        const int64_t want = std::min<int64_t>(kPlanMostBlocks, std::max<int64_t>(1, (pairs + kPlanKeys - 1) / kPlanKeys));
+        const int64_t unit = 32 * kPlanWarps;  // whole steps of every warp
+        share = ((pairs + want - 1) / want + unit - 1) / unit * unit;
+        if (share == 0) share = unit;
+        blocks = (int)std::max<int64_t>(1, (pairs + share - 1) / share);
+        bytes = blocks > 1 ? sizeof(int) * (size_t)blocks * (size_t)experts : 0;
+    }
+};
+
+// ---- dispatch --------------------------------------------------------------------------------------
+
+// Threads along a token's row as row_shape lays them out: the row is read once and written to every place of the token.
+template <typename T, int N, int U>
+__global__ void __launch_bounds__(kRowThreads)
+    dispatch_kernel(int tokens, int k, int nv, const T *__restrict__ x, int64_t ldx, const int *__restrict__ slot, int64_t lds,
+                    int64_t rows, T *__restrict__ xs, int64_t ldxs, int log) {
+    const int64_t t = (int64_t)blockIdx.x * (kRowThreads >> log) + (threadIdx.x >> log);
+    if (t >= tokens) return;
+    const int v0 = (int)(blockIdx.y * (U << log) + (threadIdx.x & ((1 << log) - 1)));
+    Pack<T, N> p[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int v = v0 + (u << log);
+        if (v < nv) p[u] = load_pack<T, N>(x + t * ldx + (int64_t)v * N);
+    }
+    for (int j = 0; j < k; j++) {
+        const int at = __ldg(slot + t * lds + j);
+        if (at < 0 || at >= rows) continue;
+        T *dst = xs + at * ldxs;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int v = v0 + (u << log);
+            if (v < nv) store_pack<T, N>(dst + (int64_t)v * N, p[u]);
+        }
+    }
+}
+
+// ---- combine ---------------------------------------------------------------------------------------
+
+// out[t] = sum over j of weight[t, j] y[slot[t, j]] + beta out[t], in 32 bits in the order of j, rounded once.  Four rows of y
+// are requested at a time.
+template <typename T, int N, int U>
+__global__ void __launch_bounds__(kRowThreads)
+    combine_kernel(int tokens, int k, int nv, const T *__restrict__ y, int64_t ldy, int64_t rows, const int *__restrict__ slot,
+                   int64_t lds, const float *__restrict__ weight, int64_t ldw, float beta, T *__restrict__ out, int64_t ldo,
+                   int log) {
+    const int64_t t = (int64_t)blockIdx.x * (kRowThreads >> log) + (threadIdx.x >> log);
+    if (t >= tokens) return;
+    const int v0 = (int)(blockIdx.y * (U << log) + (threadIdx.x & ((1 << log) - 1)));
+    float acc[U][N] = {};
+    constexpr int kAhead = 4;
+    for (int j0 = 0; j0 < k; j0 += kAhead) {
+        Pack<T, N> p[kAhead][U];
+        int at[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            at[j] = j0 + j < k ? __ldg(slot + t * lds + j0 + j) : -1;
+            if (at[j] >= rows) at[j] = -1;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int v = v0 + (u << log);
+                if (at[j] >= 0 && v < nv) p[j][u] = load_pack<T, N>(y + at[j] * ldy + (int64_t)v * N);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            if (at[j] < 0) continue;
+            const float w = weight ? __ldg(weight + t * ldw + j0 + j) : 1.f;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int i = 0; i < N; i++) acc[u][i] = fmaf(w, to_float(p[j][u].v[i]), acc[u][i]);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int v = v0 + (u << log);
+        if (v >= nv) continue;
+        T *dst = out + t * ldo + (int64_t)v * N;
+        Pack<T, N> r;
+        if (beta != 0.f) r = *reinterpret_cast<const Pack<T, N> *>(dst);
+#pragma unroll
+        for (int i = 0; i < N; i++) r.v[i] = from_float<T>(beta != 0.f ? fmaf(beta, to_float(r.v[i]), acc[u][i]) : acc[u][i]);
+        store_pack<T, N>(dst, r);
+    }
+}
+
+// dy[slot[t, j]] = weight[t, j] dout[t] and dweight[t, j] = <dout[t], y[slot[t, j]]>.  A group of threads of one block has the
+// whole row of a token, so that the inner products end in it: lanes, then warps, in a fixed order.
+template <typename T, int N>
+__global__ void __launch_bounds__(kRowThreads)
+    combine_grad_kernel(int tokens, int k, int nv, const T *__restrict__ dout, int64_t ldo, const T *__restrict__ y, int64_t ldy,
+                        int64_t rows, const int *__restrict__ slot, int64_t lds, const float *__restrict__ weight, int64_t ldw,
+                        T *__restrict__ dy, int64_t lddy, float *__restrict__ dweight, int64_t lddw, int log) {
+    __shared__ float s_dot[kRowThreads / 32][4];
+    const int64_t t = (int64_t)blockIdx.x * (kRowThreads >> log) + (threadIdx.x >> log);
+    const bool mine = t < tokens;  // a block's threads stay together for the barriers
+    const int group = 1 << log, me = threadIdx.x & (group - 1);
+    constexpr int kAtOnce = 4;
+    for (int j0 = 0; j0 < k; j0 += kAtOnce) {
+        int at[kAtOnce];
+        float w[kAtOnce], dot[kAtOnce] = {};
+#pragma unroll
+        for (int j = 0; j < kAtOnce; j++) {
+            at[j] = mine && j0 + j < k ? __ldg(slot + t * lds + j0 + j) : -1;
+            if (at[j] >= rows) at[j] = -1;
+            w[j] = at[j] >= 0 && weight ? __ldg(weight + t * ldw + j0 + j) : 1.f;
+        }
+        for (int v = me; mine && v < nv; v += group) {
+            const Pack<T, N> d = load_pack<T, N>(dout + t * ldo + (int64_t)v * N);
+            Pack<T, N> p[kAtOnce];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; j++)
+                if (at[j] >= 0) p[j] = load_pack<T, N>(y + at[j] * ldy + (int64_t)v * N);
+#pragma unroll
+            for (int j = 0; j < kAtOnce; j++) {
+                if (at[j] < 0) continue;
+                Pack<T, N> o;
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const float f = to_float(d.v[i]);
+                    dot[j] = fmaf(f, to_float(p[j].v[i]), dot[j]);
+                    o.v[i] = from_float<T>(w[j] * f);
+                }
+                store_pack<T, N>(dy + at[j] * lddy + (int64_t)v * N, o);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kAtOnce; j++)
+            for (int o = min(16, group >> 1); o; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+        if (group > 32) {
+            if ((threadIdx.x & 31) == 0)
+#pragma unroll
+                for (int j = 0; j < kAtOnce; j++) s_dot[threadIdx.x >> 5][j] = dot[j];
+            __syncthreads();
+            if (me == 0)
+#pragma unroll
+                for (int j = 0; j < kAtOnce; j++) {
+                    dot[j] = 0.f;
+                    for (int i = 0; i < group / 32; i++) dot[j] += s_dot[(threadIdx.x >> 5) + i][j];
+                }
+            __syncthreads();
+        }
+        if (me == 0 && mine)
+#pragma unroll
+            for (int j = 0; j < kAtOnce; j++)
+                if (j0 + j < k) dweight[t * lddw + j0 + j] = at[j] >= 0 ? dot[j] : 0.f;
+    }
+}
+
+// sizes that the calls on rows of experts share
+static bool rows_fit(int64_t tokens, int64_t k, int64_t width, int64_t rows) {
+    return tokens >= 0 && k >= 1 && k <= kMostRows && tokens <= kMostRows && tokens * k <= kMostRows && width >= 0 &&
+           width <= kMostWidth && rows >= 0 && rows <= kMostRows;
+}
+
+}  // namespace asb
+
+using namespace asb;
+
+extern "C" alphasparse_status_t alphasparse_cuda_expert_plan_buffer_size(int64_t tokens, int64_t k, int64_t experts, size_t *bytes) {
+    if (!bytes) return ALPHA_SPARSE_STATUS_NOT_INITIALIZED;
+    if (!rows_fit(tokens, k, 0, 0) || experts < 1) return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    if (experts > kMostExperts) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+    *bytes = PlanShape(tokens, k, experts).bytes;
+    return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+
+extern "C" alphasparse_status_t alphasparse_cuda_expert_plan(int64_t tokens, int64_t k, int64_t experts, const int32_t *index,
+                                                             int64_t ldi, int32_t *offsets, int32_t *slot, int64_t lds,
+                                                             void *buffer, size_t buffer_bytes) {
+    if (!rows_fit(tokens, k, 0, 0) || experts < 1) return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    if (experts > kMostExperts) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+    const PlanShape sh(tokens, k, experts);
+    if (sh.bytes && buffer && (buffer_bytes < sh.bytes || address(buffer) % sizeof(int))) {
+        record_error("alphasparse_cuda_expert_plan: the workspace is smaller than alphasparse_cuda_expert_plan_buffer_size says, or not on a 4-byte boundary");
+        return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    }
+    const alphasparse_status_t s = check_operands(
+        "alphasparse_cuda_expert_plan", {{index, tokens, k, ldi, sizeof(int), false},
+                                         {offsets, 1, experts + 1, experts + 1, sizeof(int), true},
+                                         {slot, tokens, k, lds, sizeof(int), true},
+                                         {buffer, 1, (int64_t)(sh.bytes / sizeof(int)), 0, sizeof(int), true}});
+    if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+    cudaStream_t st = current_stream();
+    const size_t smem = sizeof(int) * kPlanWarps * (size_t)experts;
+    int *counts = static_cast<int *>(buffer);
+    if (sh.blocks > 1) {
+        ASB_CUDA_OR(cudaFuncSetAttribute(plan_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(int) * kPlanWarps * kMostExperts)),
+                    ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+        plan_kernel<false><<<sh.blocks, kPlanThreads, smem, st>>>(sh.pairs, sh.share, (int)experts, (int)k, index, ldi, counts, nullptr, nullptr, 0);
+        count_launch();
+    }
+    ASB_CUDA_OR(cudaFuncSetAttribute(plan_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(int) * kPlanWarps * kMostExperts)),
+                ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    plan_kernel<true><<<sh.blocks, kPlanThreads, smem, st>>>(sh.pairs, sh.share, (int)experts, (int)k, index, ldi, counts, offsets, slot, lds);
+    count_launch();
+    ASB_CUDA_OR(cudaGetLastError(), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+
+extern "C" alphasparse_status_t alphasparse_cuda_expert_dispatch(alphasparse_cuda_type_t type, int64_t tokens, int64_t k, int64_t width,
+                                                                 const void *x, int64_t ldx, const int32_t *slot, int64_t lds,
+                                                                 int64_t rows, void *xs, int64_t ldxs) {
+    const size_t eb = type_bytes(type);
+    if (!eb || !rows_fit(tokens, k, width, rows)) return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    if (tokens == 0 || width == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
+    const alphasparse_status_t s = check_operands("alphasparse_cuda_expert_dispatch", {{x, tokens, width, ldx, eb, false},
+                                                                                      {slot, tokens, k, lds, sizeof(int), false},
+                                                                                      {xs, rows, width, ldxs, eb, true}});
+    if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+    const int vb = vector_bytes(eb, {address(x), (uint64_t)ldx * eb, address(xs), (uint64_t)ldxs * eb, (uint64_t)width * eb});
+    const int64_t nv = width * (int64_t)eb / vb;
+    const RowShape shape = row_shape(tokens, nv);
+    cudaStream_t st = current_stream();
+    const auto run = [&](auto t) {
+        using T = decltype(t);
+        with_pack<T>(vb, [&](auto n) {
+            constexpr int N = decltype(n)::value;
+            const auto kernel = shape.unroll == 1 ? dispatch_kernel<T, N, 1> : dispatch_kernel<T, N, 4>;
+            kernel<<<shape.grid, kRowThreads, 0, st>>>((int)tokens, (int)k, (int)nv, (const T *)x, ldx, slot, lds, rows, (T *)xs, ldxs, shape.log);
+        });
+    };
+    ASB_BY_TYPE(type, run)
+    count_launch();
+    ASB_CUDA_OR(cudaGetLastError(), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+
+extern "C" alphasparse_status_t alphasparse_cuda_expert_combine(alphasparse_cuda_type_t type, int64_t tokens, int64_t k, int64_t width,
+                                                                int64_t rows, const void *y, int64_t ldy, const int32_t *slot,
+                                                                int64_t lds, const float *weight, int64_t ldw, float beta,
+                                                                void *out, int64_t ldo) {
+    const size_t eb = type_bytes(type);
+    if (!eb || !rows_fit(tokens, k, width, rows)) return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    if (tokens == 0 || width == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
+    const alphasparse_status_t s = check_operands("alphasparse_cuda_expert_combine", {{y, rows, width, ldy, eb, false},
+                                                                                     {slot, tokens, k, lds, sizeof(int), false},
+                                                                                     {weight, weight ? tokens : 0, k, ldw, sizeof(float), false},
+                                                                                     {out, tokens, width, ldo, eb, true}});
+    if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+    const int vb = vector_bytes(eb, {address(y), (uint64_t)ldy * eb, address(out), (uint64_t)ldo * eb, (uint64_t)width * eb});
+    const int64_t nv = width * (int64_t)eb / vb;
+    RowShape shape = row_shape(tokens, nv);
+    cudaStream_t st = current_stream();
+    const auto run = [&](auto t) {
+        using T = decltype(t);
+        with_pack<T>(vb, [&](auto n) {
+            constexpr int N = decltype(n)::value;
+            const auto kernel = shape.unroll == 1 ? combine_kernel<T, N, 1> : combine_kernel<T, N, 4>;
+            kernel<<<shape.grid, kRowThreads, 0, st>>>((int)tokens, (int)k, (int)nv, (const T *)y, ldy, rows, slot, lds, weight, ldw, beta, (T *)out, ldo, shape.log);
+        });
+    };
+    ASB_BY_TYPE(type, run)
+    count_launch();
+    ASB_CUDA_OR(cudaGetLastError(), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+
+extern "C" alphasparse_status_t alphasparse_cuda_expert_combine_grad(alphasparse_cuda_type_t type, int64_t tokens, int64_t k, int64_t width,
+                                                                     int64_t rows, const void *dout, int64_t ldo, const void *y,
+                                                                     int64_t ldy, const int32_t *slot, int64_t lds,
+                                                                     const float *weight, int64_t ldw, void *dy, int64_t lddy,
+                                                                     float *dweight, int64_t lddw) {
+    const size_t eb = type_bytes(type);
+    if (!eb || !rows_fit(tokens, k, width, rows)) return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    if (tokens == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
+    const alphasparse_status_t s = check_operands("alphasparse_cuda_expert_combine_grad",
+                                                  {{dout, tokens, width, ldo, eb, false},
+                                                   {y, rows, width, ldy, eb, false},
+                                                   {slot, tokens, k, lds, sizeof(int), false},
+                                                   {weight, weight ? tokens : 0, k, ldw, sizeof(float), false},
+                                                   {dy, rows, width, lddy, eb, true},
+                                                   {dweight, tokens, k, lddw, sizeof(float), true}});
+    if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+    const int vb = vector_bytes(eb, {address(dout), (uint64_t)ldo * eb, address(y), (uint64_t)ldy * eb, address(dy),
+                                     (uint64_t)lddy * eb, (uint64_t)width * eb});
+    const int64_t nv = width * (int64_t)eb / vb;
+    int log = 0;
+    while ((1 << log) < kRowThreads && (int64_t)1 << log < nv) log++;
+    const unsigned blocks = (unsigned)((tokens + (kRowThreads >> log) - 1) / (kRowThreads >> log));
+    cudaStream_t st = current_stream();
+    const auto run = [&](auto t) {
+        using T = decltype(t);
+        with_pack<T>(vb, [&](auto n) {
+            constexpr int N = decltype(n)::value;
+            combine_grad_kernel<T, N><<<blocks, kRowThreads, 0, st>>>((int)tokens, (int)k, (int)nv, (const T *)dout, ldo, (const T *)y, ldy, rows,
+                                                                   slot, lds, weight, ldw, (T *)dy, lddy, dweight, lddw, log);
+        });
+    };
+    ASB_BY_TYPE(type, run)
+    count_launch();
+    ASB_CUDA_OR(cudaGetLastError(), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    return ALPHA_SPARSE_STATUS_SUCCESS;
+}

@@ -1,0 +1,148 @@
+// What the operators on rows of dense blocks (embedding.cu, route.cu, experts.cu, expert_mm.cu) share: element types,
+// vector access, checks of arguments.  Not part of the C ABI.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "internal.h"
+
+namespace asb {
+
+// ---- element types ---------------------------------------------------------------------------
+
+template <typename T> __device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float(float v) { return v; }
+template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+
+// N consecutive elements, moved in accesses of at most 16 bytes
+template <typename T, int N>
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
+    T v[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T *p) {
+    Pack<T, N> r;
+    constexpr int bytes = sizeof(T) * N;
+    if constexpr (bytes >= 16) {
+#pragma unroll
+        for (int i = 0; i < bytes / 16; i++)
+            reinterpret_cast<uint4 *>(&r)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    } else if constexpr (bytes == 8) {
+        *reinterpret_cast<uint2 *>(&r) = __ldg(reinterpret_cast<const uint2 *>(p));
+    } else if constexpr (bytes == 4) {
+        *reinterpret_cast<unsigned *>(&r) = __ldg(reinterpret_cast<const unsigned *>(p));
+    } else {
+        *reinterpret_cast<unsigned short *>(&r) = __ldg(reinterpret_cast<const unsigned short *>(p));
+    }
+    return r;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r) {
+    constexpr int bytes = sizeof(T) * N;
+    if constexpr (bytes >= 16) {
+#pragma unroll
+        for (int i = 0; i < bytes / 16; i++) reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(&r)[i];
+    } else if constexpr (bytes == 8) {
+        *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(&r);
+    } else if constexpr (bytes == 4) {
+        *reinterpret_cast<unsigned *>(p) = *reinterpret_cast<const unsigned *>(&r);
+    } else {
+        *reinterpret_cast<unsigned short *>(p) = *reinterpret_cast<const unsigned short *>(&r);
+    }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> zero_pack() {
+    Pack<T, N> r;
+#pragma unroll
+    for (int i = 0; i < N; i++) r.v[i] = from_float<T>(0.f);
+    return r;
+}
+
+// ---- arguments -------------------------------------------------------------------------------
+
+// 0 for a value that names no type
+inline size_t type_bytes(alphasparse_cuda_type_t t) {
+    return t == ALPHA_SPARSE_CUDA_TYPE_F32 ? 4 : t == ALPHA_SPARSE_CUDA_TYPE_F16 || t == ALPHA_SPARSE_CUDA_TYPE_BF16 ? 2 : 0;
+}
+inline size_t index_bytes(alphasparse_cuda_index_t t) {
+    return t == ALPHA_SPARSE_CUDA_INDEX_I32 ? 4 : t == ALPHA_SPARSE_CUDA_INDEX_I64 ? 8 : 0;
+}
+
+constexpr int64_t kMostRows = 0x7fffffff - 4096;  // row counts and positions fit an int with room for a tile's overhang
+constexpr int64_t kMostWidth = 1 << 24;
+constexpr int64_t kMostStride = 0x7fffffff;
+constexpr int kMostExperts = 1024;
+constexpr int kMostTopK = 32;
+
+// One operand: `rows` rows of `width` elements of `elem` bytes, `ld` elements apart.
+struct Operand {
+    const void *p;
+    int64_t rows, width, ld;
+    size_t elem;
+    bool written;
+    uintptr_t begin() const { return reinterpret_cast<uintptr_t>(p); }
+    uintptr_t end() const {
+        return begin() + (rows > 0 ? (((uintptr_t)rows - 1) * (uintptr_t)ld + (uintptr_t)width) * elem : 0);
+    }
+    bool empty() const { return rows <= 0 || width <= 0; }
+};
+
+// Checks operands in the order that they are given: there (NOT_INITIALIZED), leading dimension and alignment to the
+// element (INVALID_VALUE), no written operand in the place of another (INVALID_VALUE), memory of the current device
+// (INVALID_POINTER).  Operands without elements may be null.  An optional operand is left out by the caller.
+alphasparse_status_t check_operands(const char *call, std::initializer_list<Operand> operands);
+
+// Largest of 16, 8, 4 and the element's own bytes that divides everything given (addresses, strides and widths in bytes).
+inline int vector_bytes(size_t elem, std::initializer_list<uint64_t> all) {
+    uint64_t any = 0;
+    for (uint64_t v : all) any |= v;
+    return any % 16 == 0 ? 16 : any % 8 == 0 ? 8 : any % 4 == 0 ? 4 : (int)elem;
+}
+// Calls f with the number of elements of T that make `vb` bytes, as a compile-time constant
+template <typename T, typename F>
+void with_pack(int vb, F f) {
+    if (vb == 16) f(std::integral_constant<int, 16 / sizeof(T)>{});
+    else if (vb == 8) f(std::integral_constant<int, 8 / sizeof(T)>{});
+    else if (vb == 4) f(std::integral_constant<int, 4 / sizeof(T)>{});
+    else f(std::integral_constant<int, 1>{});
+}
+
+inline uint64_t address(const void *p) { return (uint64_t)reinterpret_cast<uintptr_t>(p); }
+
+// A row of `nv` vectors by a group of 2^log threads, `unroll` vectors a thread and piece of the row.  Few vectors in all:
+// one a thread, so that the call is done in one round trip to memory; many: four, so that enough are in flight.
+struct RowShape {
+    int log, unroll;
+    dim3 grid;
+};
+constexpr int kRowThreads = 256;
+inline RowShape row_shape(int64_t rows, int64_t nv) {
+    RowShape s;
+    s.unroll = rows * nv <= 148 * 2048 ? 1 : 4;
+    s.log = 0;
+    while ((1 << s.log) < kRowThreads && (int64_t)s.unroll << s.log < nv) s.log++;
+    const int64_t per_block = kRowThreads >> s.log, piece = (int64_t)s.unroll << s.log;
+    s.grid = dim3((unsigned)((rows + per_block - 1) / per_block), (unsigned)((nv + piece - 1) / piece));
+    return s;
+}
+
+}  // namespace asb
+
+// Calls f with a value of the element type that `type` names
+#define ASB_BY_TYPE(type, f)                                                     \
+    switch (type) {                                                              \
+        case ALPHA_SPARSE_CUDA_TYPE_F32: f((float)0); break;                     \
+        case ALPHA_SPARSE_CUDA_TYPE_F16: f(__half()); break;                     \
+        case ALPHA_SPARSE_CUDA_TYPE_BF16: f(__nv_bfloat16()); break;             \
+    }

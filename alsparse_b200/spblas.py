@@ -253,3 +253,160 @@ def read_coo(kind, path):
         lib.alpha_free(p)
         return a
     return m.value, n.value, take(ri, C.c_int32), take(ci, C.c_int32), take(v, C.c_float if kind == "s" else C.c_double)
+
+
+# ---- products of matrices that are made at run time (device tensors) ------------------------------------------
+
+_TYPES = {"float32": capi.TYPE_F32, "float16": capi.TYPE_F16, "bfloat16": capi.TYPE_BF16}
+_INDICES = {"int32": capi.INDEX_I32, "int64": capi.INDEX_I64}
+
+
+def _type(a, names=_TYPES):
+    """Enum value of an array's element type; -1, which the library refuses, for one that has none."""
+    return names.get(str(a.dtype).replace("torch.", ""), -1)
+
+
+def _strides(a):
+    if isinstance(a, np.ndarray):
+        return tuple(s // a.itemsize for s in a.strides)
+    return tuple(a.stride())
+
+
+def _rows(a, dims=2):
+    """Leading dimension of a row-major array whose rows are contiguous, None if it is not one (the caller's view has to be
+    copied first).  Three dimensions: (distance of the matrices, leading dimension)."""
+    if a.ndim != dims:
+        return None
+    shape, s = tuple(a.shape), _strides(a)
+    if shape[-1] > 1 and s[-1] != 1:
+        return None
+    ld = s[-2] if shape[-2] > 1 else max(s[-2], shape[-1])
+    if dims == 2:
+        return ld
+    return (s[0] if shape[0] > 1 else max(s[0], ld * shape[1]), ld)
+
+
+def _is(a, name):
+    return str(a.dtype).replace("torch.", "") == name
+
+
+def _buffer(b):
+    """Address and bytes of a workspace: a contiguous array, or None."""
+    if b is None:
+        return None, 0
+    return _ptr(b), b.nbytes if isinstance(b, np.ndarray) else b.numel() * b.element_size()
+
+
+def embedding(tokens, table, scale, y):
+    """alphasparse_cuda_embedding: y[i] = scale * table[tokens[i]].  tokens: one dimension of int32 or int64, any stride;
+    table (vocab, width) and y (tokens, width) of one type, rows contiguous.  Returns the status."""
+    ldt, ldy = _rows(table), _rows(y)
+    if tokens.ndim != 1 or ldt is None or ldy is None or y.dtype != table.dtype or tuple(y.shape) != (tokens.shape[0], table.shape[1]):
+        return capi.INVALID_VALUE
+    return capi.load().alphasparse_cuda_embedding(_type(tokens, _INDICES), _type(table), tokens.shape[0], _ptr(tokens),
+                                                  _strides(tokens)[0] if tokens.shape[0] > 1 else 1, table.shape[0], table.shape[1],
+                                                  scale, _ptr(table), ldt, _ptr(y), ldy)
+
+
+def embedding_grad_buffer_size(tokens, vocab, width):
+    """(status, bytes of the workspace) of embedding_grad."""
+    n = C.c_size_t()
+    st = capi.load().alphasparse_cuda_embedding_grad_buffer_size(tokens, vocab, width, C.byref(n))
+    return st, n.value
+
+
+def embedding_grad(tokens, dy, alpha, beta, dtable, buffer):
+    """alphasparse_cuda_embedding_grad: dtable[v] = alpha * (sum of dy[i] where tokens[i] == v) + beta * dtable[v].
+    Returns the status."""
+    lddy, ldt = _rows(dy), _rows(dtable)
+    if tokens.ndim != 1 or lddy is None or ldt is None or tuple(dy.shape) != (tokens.shape[0], dtable.shape[1]):
+        return capi.INVALID_VALUE
+    at, size = _buffer(buffer)
+    return capi.load().alphasparse_cuda_embedding_grad(_type(tokens, _INDICES), _type(dy), _type(dtable), tokens.shape[0], _ptr(tokens),
+                                                       _strides(tokens)[0] if tokens.shape[0] > 1 else 1, dtable.shape[0], dtable.shape[1],
+                                                       alpha, _ptr(dy), lddy, beta, _ptr(dtable), ldt, at, size)
+
+
+def route(score, logits, bias, groups, top_groups, renormalize, scale, index, weight):
+    """alphasparse_cuda_route: the experts index (tokens, k; int32) of each row of logits (tokens, experts) and their
+    weights (tokens, k; float32); bias: (experts,) float32 or None.  Returns the status."""
+    ldl, ldi, ldw = _rows(logits), _rows(index), _rows(weight)
+    if ldl is None or ldi is None or ldw is None or not _is(index, "int32") or not _is(weight, "float32") or tuple(index.shape) != tuple(weight.shape) \
+            or index.shape[0] != logits.shape[0]:
+        return capi.INVALID_VALUE
+    if bias is not None and (not _is(bias, "float32") or tuple(bias.shape) != (logits.shape[1],) or (bias.shape[0] > 1 and _strides(bias)[0] != 1)):
+        return capi.INVALID_VALUE
+    return capi.load().alphasparse_cuda_route(score, _type(logits), logits.shape[0], logits.shape[1], _ptr(logits), ldl, _ptr(bias), groups,
+                                              top_groups, index.shape[1], 1 if renormalize else 0, scale, _ptr(index), ldi, _ptr(weight), ldw)
+
+
+def route_grad(score, logits, index, renormalize, scale, dweight, dlogits):
+    """alphasparse_cuda_route_grad: dlogits from the gradient dweight of the weights of index.  Returns the status."""
+    ldl, ldi, ldw, ldd = _rows(logits), _rows(index), _rows(dweight), _rows(dlogits)
+    if None in (ldl, ldi, ldw, ldd) or not _is(index, "int32") or not _is(dweight, "float32") or dlogits.dtype != logits.dtype \
+            or tuple(dlogits.shape) != tuple(logits.shape) or tuple(index.shape) != tuple(dweight.shape) or index.shape[0] != logits.shape[0]:
+        return capi.INVALID_VALUE
+    return capi.load().alphasparse_cuda_route_grad(score, _type(logits), logits.shape[0], logits.shape[1], _ptr(logits), ldl, index.shape[1],
+                                                   _ptr(index), ldi, 1 if renormalize else 0, scale, _ptr(dweight), ldw, _ptr(dlogits), ldd)
+
+
+def expert_plan_buffer_size(tokens, k, experts):
+    """(status, bytes of the workspace) of expert_plan; 0 for a few thousand pairs."""
+    n = C.c_size_t()
+    st = capi.load().alphasparse_cuda_expert_plan_buffer_size(tokens, k, experts, C.byref(n))
+    return st, n.value
+
+
+def expert_plan(index, offsets, slot, buffer):
+    """alphasparse_cuda_expert_plan: offsets (experts + 1) and slot (tokens, k) of index (tokens, k), all int32.  Returns
+    the status."""
+    ldi, lds = _rows(index), _rows(slot)
+    if ldi is None or lds is None or tuple(slot.shape) != tuple(index.shape) or offsets.ndim != 1 or (offsets.shape[0] > 1 and _strides(offsets)[0] != 1) \
+            or not all(_is(a, "int32") for a in (index, offsets, slot)):
+        return capi.INVALID_VALUE
+    at, size = _buffer(buffer)
+    return capi.load().alphasparse_cuda_expert_plan(index.shape[0], index.shape[1], offsets.shape[0] - 1, _ptr(index), ldi, _ptr(offsets),
+                                                    _ptr(slot), lds, at, size)
+
+
+def expert_dispatch(x, slot, xs):
+    """alphasparse_cuda_expert_dispatch: xs[slot[t, j]] = x[t].  Returns the status."""
+    ldx, lds, ldxs = _rows(x), _rows(slot), _rows(xs)
+    if None in (ldx, lds, ldxs) or not _is(slot, "int32") or xs.dtype != x.dtype or slot.shape[0] != x.shape[0] or xs.shape[1] != x.shape[1]:
+        return capi.INVALID_VALUE
+    return capi.load().alphasparse_cuda_expert_dispatch(_type(x), x.shape[0], slot.shape[1], x.shape[1], _ptr(x), ldx, _ptr(slot), lds,
+                                                        xs.shape[0], _ptr(xs), ldxs)
+
+
+def _weights(weight, slot):
+    """Leading dimension of the weights of slot (0 for None), or None if they do not fit it."""
+    if weight is None:
+        return 0
+    return _rows(weight) if _is(weight, "float32") and tuple(weight.shape) == tuple(slot.shape) else None
+
+
+def expert_combine(y, slot, weight, beta, out):
+    """alphasparse_cuda_expert_combine: out[t] = sum over j of weight[t, j] * y[slot[t, j]] + beta * out[t]; weight None: ones.
+    Returns the status."""
+    ldy, lds, ldo = _rows(y), _rows(slot), _rows(out)
+    if None in (ldy, lds, ldo) or not _is(slot, "int32") or out.dtype != y.dtype or out.shape[0] != slot.shape[0] or out.shape[1] != y.shape[1]:
+        return capi.INVALID_VALUE
+    ldw = _weights(weight, slot)
+    if ldw is None:
+        return capi.INVALID_VALUE
+    return capi.load().alphasparse_cuda_expert_combine(_type(y), slot.shape[0], slot.shape[1], y.shape[1], y.shape[0], _ptr(y), ldy, _ptr(slot),
+                                                       lds, _ptr(weight), ldw, beta, _ptr(out), ldo)
+
+
+def expert_combine_grad(dout, y, slot, weight, dy, dweight):
+    """alphasparse_cuda_expert_combine_grad: dy[slot[t, j]] = weight[t, j] * dout[t], dweight[t, j] = <dout[t], y[slot[t, j]]>.
+    Returns the status."""
+    ldo, ldy, lds, lddy, lddw = _rows(dout), _rows(y), _rows(slot), _rows(dy), _rows(dweight)
+    if None in (ldo, ldy, lds, lddy, lddw) or not _is(slot, "int32") or not _is(dweight, "float32") or dout.dtype != y.dtype or dy.dtype != y.dtype \
+            or tuple(dy.shape) != tuple(y.shape) or tuple(dout.shape) != (slot.shape[0], y.shape[1]) or tuple(dweight.shape) != tuple(slot.shape):
+        return capi.INVALID_VALUE
+    ldw = _weights(weight, slot)
+    if ldw is None:
+        return capi.INVALID_VALUE
+    return capi.load().alphasparse_cuda_expert_combine_grad(_type(y), slot.shape[0], slot.shape[1], y.shape[1], y.shape[0], _ptr(dout), ldo,
+                                                            _ptr(y), ldy, _ptr(slot), lds, _ptr(weight), ldw, _ptr(dy), lddy, _ptr(dweight), lddw)

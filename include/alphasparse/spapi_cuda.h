@@ -195,6 +195,103 @@ alphasparse_status_t alphasparse_d_mv_exchange(const double alpha, const alphasp
                                                const struct alpha_matrix_descr descr,
                                                alphasparse_cuda_exchange_t ex, const double beta, double *y);
 
+/* ---- products of matrices that are made at run time ------------------------------------------------
+ * No counterpart in the reference.  A sparse matrix that comes out of a computation on the device and is multiplied
+ * by once gets no handle: the one-hot matrix of an embedding lookup, the k entries per token that a router makes,
+ * the block-diagonal matrix of the experts' weights.  The calls below take what such a matrix is made of.
+ *
+ * All of them: every pointer is memory of the current device (or managed), else ALPHA_SPARSE_STATUS_INVALID_POINTER;
+ * work is enqueued on the library stream and the call returns without waiting; nothing is allocated, kept from call to
+ * call or shared between calls (workspaces are the caller's: two calls that may overlap, and two captured graphs that
+ * may run at the same time, take two), so the calls can be captured.  Dense operands are row-major with a leading
+ * dimension of at most 2^31 - 1 elements and any alignment that their elements allow; 16-byte aligned rows are fastest.
+ * A missing operand is ALPHA_SPARSE_STATUS_NOT_INITIALIZED; sizes and enums out of range, leading dimensions below
+ * the width and an output that lies in the place of another operand are ALPHA_SPARSE_STATUS_INVALID_VALUE.  Operands
+ * without elements may be NULL.  Row counts go to 2^31 - 4097, widths to 2^24.  Sums are formed in 32 bits in a
+ * fixed order and rounded once: the same call gives the same bits.  Values that stand where nothing selects them are
+ * not read, so a NaN there does not reach a result. */
+typedef enum {
+    ALPHA_SPARSE_CUDA_TYPE_F32 = 0,
+    ALPHA_SPARSE_CUDA_TYPE_F16 = 1,
+    ALPHA_SPARSE_CUDA_TYPE_BF16 = 2
+} alphasparse_cuda_type_t;
+typedef enum { ALPHA_SPARSE_CUDA_INDEX_I32 = 0, ALPHA_SPARSE_CUDA_INDEX_I64 = 1 } alphasparse_cuda_index_t;
+typedef enum { ALPHA_SPARSE_CUDA_SCORE_SOFTMAX = 0, ALPHA_SPARSE_CUDA_SCORE_SIGMOID = 1 } alphasparse_cuda_score_t;
+
+/* Embedding lookup: y[i] = scale * table[token[i * inctoken]], i < tokens; y and table hold elements of `type`.  A
+ * token outside [0, vocab) selects nothing: its row of y is zero (padding; tokens of another part of a table that
+ * is divided over GPUs). */
+alphasparse_status_t alphasparse_cuda_embedding(alphasparse_cuda_index_t index_type, alphasparse_cuda_type_t type,
+                                                int64_t tokens, const void *token, int64_t inctoken, int64_t vocab,
+                                                int64_t width, float scale, const void *table, int64_t ldt, void *y,
+                                                int64_t ldy);
+
+/* Its gradient: dtable[v] = alpha * (sum of dy[i] over the tokens i that name v, in their order) + beta * dtable[v].
+ * dy holds elements of `type`, dtable of `table_type` (the same, or F32).  beta = 0 does not read dtable and
+ * writes all of it, rows that no token names as zeros; beta = 1 leaves those rows alone.  buffer: a workspace
+ * on a 16-byte boundary, as large as _buffer_size says (it grows with the tokens and the vocabulary). */
+alphasparse_status_t alphasparse_cuda_embedding_grad_buffer_size(int64_t tokens, int64_t vocab, int64_t width,
+                                                                 size_t *bytes);
+alphasparse_status_t alphasparse_cuda_embedding_grad(alphasparse_cuda_index_t index_type, alphasparse_cuda_type_t type,
+                                                     alphasparse_cuda_type_t table_type, int64_t tokens,
+                                                     const void *token, int64_t inctoken, int64_t vocab, int64_t width,
+                                                     float alpha, const void *dy, int64_t lddy, float beta,
+                                                     void *dtable, int64_t ldt, void *buffer, size_t buffer_bytes);
+
+/* Routing: for each of `tokens` rows of `experts` logits, the k experts with the highest keys, highest first, equal keys
+ * lowest index first, and their weights.
+ *   score s      softmax over the row, or sigmoid of each logit
+ *   key          the logit; with a bias (`experts` floats) s + bias.  Keys are compared as 64-bit arithmetic has them.
+ *   groups       the experts stand in `groups` equal runs; only the top_groups best runs are chosen from.  A run is worth
+ *                its highest key, with a bias the sum of its two highest.  groups = 1: no limit.
+ *   weight       scale * s, or with renormalize scale * s / (sum of the chosen s); the bias is not in it
+ * An expert whose logit or key is minus infinity is never chosen; where fewer than k are left the remaining indices are
+ * -1 and their weights 0.  A NaN key comes before all others, and NaN scores give NaN weights.  Up to 1024 experts,
+ * k up to 32 and at most the experts of top_groups runs, up to 32 runs. */
+alphasparse_status_t alphasparse_cuda_route(alphasparse_cuda_score_t score, alphasparse_cuda_type_t type,
+                                            int64_t tokens, int64_t experts, const void *logits, int64_t ldl,
+                                            const float *bias, int64_t groups, int64_t top_groups, int64_t k,
+                                            int renormalize, float scale, int32_t *index, int64_t ldi, float *weight,
+                                            int64_t ldw);
+
+/* Gradient of the weights with respect to the logits (the choice and the bias have none): index as routing left it,
+ * dweight the gradient of its weights.  Writes every element of dlogits.  Indices outside [0, experts) and those of
+ * logits of minus infinity count as empty. */
+alphasparse_status_t alphasparse_cuda_route_grad(alphasparse_cuda_score_t score, alphasparse_cuda_type_t type,
+                                                 int64_t tokens, int64_t experts, const void *logits, int64_t ldl,
+                                                 int64_t k, const int32_t *index, int64_t ldi, int renormalize,
+                                                 float scale, const float *dweight, int64_t ldw, void *dlogits,
+                                                 int64_t ldd);
+
+/* The order of the experts' rows: the pairs (token, choice) whose index lies in [0, experts) sorted by expert, those of one
+ * expert by token and choice.  offsets[e] (experts + 1 ints) is the first row of expert e, slot[t, j] the row of
+ * pair (t, j) or -1.  Up to 1024 experts, tokens * k to 2^31 - 4097. */
+alphasparse_status_t alphasparse_cuda_expert_plan_buffer_size(int64_t tokens, int64_t k, int64_t experts, size_t *bytes);
+alphasparse_status_t alphasparse_cuda_expert_plan(int64_t tokens, int64_t k, int64_t experts, const int32_t *index,
+                                                  int64_t ldi, int32_t *offsets, int32_t *slot, int64_t lds,
+                                                  void *buffer, size_t buffer_bytes);
+
+/* xs[slot[t, j]] = x[t]; rows of xs that no slot names, those behind the last among them, are left as they were.  A slot
+ * outside [0, rows) is empty.  The gradient of x is alphasparse_cuda_expert_combine of the gradient of xs with weight =
+ * NULL. */
+alphasparse_status_t alphasparse_cuda_expert_dispatch(alphasparse_cuda_type_t type, int64_t tokens, int64_t k,
+                                                      int64_t width, const void *x, int64_t ldx, const int32_t *slot,
+                                                      int64_t lds, int64_t rows, void *xs, int64_t ldxs);
+
+/* out[t] = sum over j of weight[t, j] * y[slot[t, j]] + beta * out[t]; weight = NULL: ones; beta = 0 does not read out. */
+alphasparse_status_t alphasparse_cuda_expert_combine(alphasparse_cuda_type_t type, int64_t tokens, int64_t k,
+                                                     int64_t width, int64_t rows, const void *y, int64_t ldy,
+                                                     const int32_t *slot, int64_t lds, const float *weight, int64_t ldw,
+                                                     float beta, void *out, int64_t ldo);
+
+/* Its gradients: dy[slot[t, j]] = weight[t, j] * dout[t] (other rows of dy are left as they were) and dweight[t, j] =
+ * <dout[t], y[slot[t, j]]>, 0 for an empty slot. */
+alphasparse_status_t alphasparse_cuda_expert_combine_grad(alphasparse_cuda_type_t type, int64_t tokens, int64_t k,
+                                                          int64_t width, int64_t rows, const void *dout, int64_t ldo,
+                                                          const void *y, int64_t ldy, const int32_t *slot, int64_t lds,
+                                                          const float *weight, int64_t ldw, void *dy, int64_t lddy,
+                                                          float *dweight, int64_t lddw);
+
 /* Error word of a handle's kernels.  Kernels that wait (the row-tile kernel waits for its bulk copies) give up
  * after a bounded number of polls, leave y untouched for their tile and record a code here: 1 = a tile larger
  * than the kernel was configured for, 2 = a bulk copy did not complete in time.  A call with host vectors
