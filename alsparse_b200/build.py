@@ -21,7 +21,7 @@ LIB = os.path.join(HERE, "libalphasparse_b200.so")
 SYNTH_SRC = os.path.join(HERE, "synth", "synth.c")
 SYNTH_LIB = os.path.join(HERE, "synth", "libsynth.so")
 CUDA_SOURCES = ["core.cu", "spmv.cu", "spmv_band.cu", "spmv_bins.cu", "spmm.cu", "exchange.cu", "coo2csr.cu", "transfer.cu", "host_util.cu", "host_args.cu",
-                "embedding.cu", "route.cu", "experts.cu"]
+                "embedding.cu", "route.cu", "experts.cu", "expert_mm.cu"]
 
 
 def _newer(target, deps):

@@ -130,6 +130,9 @@ def prototypes():
     p["alphasparse_cuda_expert_dispatch"] = (C.c_int, [C.c_int, _L, _L, _L, _P, _L, _P, _L, _L, _P, _L])
     p["alphasparse_cuda_expert_combine"] = (C.c_int, [C.c_int, _L, _L, _L, _L, _P, _L, _P, _L, _P, _L, _F, _P, _L])
     p["alphasparse_cuda_expert_combine_grad"] = (C.c_int, [C.c_int, _L, _L, _L, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L])
+    p["alphasparse_cuda_expert_mm"] = (C.c_int, [C.c_int, C.c_int, _L, _L, _P, _L, _L, _P, _L, _P, _L, _L, _P, _L])
+    p["alphasparse_cuda_expert_mm_grad"] = (C.c_int, [C.c_int, C.c_int, _L, _L, _P, _L, _L, _P, _L, _P, _L, _F, _P, _L, _L])
+    p["alphasparse_cuda_expert_mm_status"] = (C.c_int, [C.POINTER(C.c_int), C.c_int])
     p["alphasparse_cuda_kernel_status"] = (C.c_int, [_H, C.POINTER(C.c_int), C.c_int])
     p["alphasparse_cuda_profile_kernel"] = (C.c_int, [_H, C.c_int])
     p["alphasparse_cuda_kernel_ms"] = (C.c_int, [_H, C.POINTER(C.c_float)])

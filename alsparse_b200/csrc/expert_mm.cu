@@ -1,0 +1,694 @@
+// Products of the experts: rows [offsets[e], offsets[e + 1]) of a dense block times the weights of expert e (a block-diagonal
+// matrix times a dense block), and the gradient of the weights.  No counterpart in the reference.
+//
+// expert_mm_kernel: tcgen05.mma with operands brought by TMA into a ring of stages, accumulators in TMEM, one persistent
+// block per SM.  One warp issues copies, one the products, four empty the accumulators; two accumulators, so that a tile is
+// written while the next is multiplied.  The offsets stay on the device: every block forms the same table of row tiles.
+// expert_mm_plain_kernel: 32-bit operands, and addresses or strides that TMA does not take (no multiple of 16 bytes).
+#include <cuda.h>
+#include <stdio.h>
+
+#include <algorithm>
+
+#include "rows.h"
+
+namespace asb {
+
+// Set by a kernel whose bounded wait ran out (alphasparse_cuda_expert_mm_status).
+static __device__ int g_expert_mm_status;
+
+// D[m, n] = sum over k of A[m, k] B[n, k].  What the three dimensions are:
+enum MmForm {
+    kRowsFirst,  // m: rows of an expert, n: its output features      (many rows an expert)
+    kRowsLast,   // m: output features, n: rows of an expert           (few rows an expert: no tile of 128 rows to fill)
+    kGradient    // m: columns of dy, n: columns of x, k: rows         (dW = dy^T x)
+};
+
+// First and last row of an expert, whatever the offsets hold
+__device__ __forceinline__ void rows_of(const int *__restrict__ offsets, int e, int64_t rows, int *lo, int *hi) {
+    const int64_t a = min(max((int64_t)__ldg(offsets + e), (int64_t)0), rows);
+    *lo = (int)a;
+    *hi = (int)min(max((int64_t)__ldg(offsets + e + 1), a), rows);
+}
+
+// first[e] = row tiles of the experts before e, e = 0 .. experts; by one warp.  Offsets that name more rows than there are
+// (they do not ascend) give no tiles at all.
+__device__ __forceinline__ void count_row_tiles(const int *__restrict__ offsets, int experts, int64_t rows, int tile, int *first) {
+    const int lane = threadIdx.x & 31;
+    int carry = 0;
+    int64_t named = 0;
+    for (int e0 = 0; e0 < experts; e0 += 32) {
+        int n = 0, lo = 0, hi = 0;
+        if (e0 + lane < experts) {
+            rows_of(offsets, e0 + lane, rows, &lo, &hi);
+            n = (hi - lo + tile - 1) / tile;
+        }
+        int64_t here = hi - lo;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) here += __shfl_xor_sync(0xffffffffu, here, o);
+        named += here;
+        if (named > rows) {
+            carry = 0;
+            break;
+        }
+        int inc = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (e0 + lane < experts) first[e0 + lane] = carry + inc - n;
+        carry += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) first[experts] = carry;
+}
+
+// the expert of row tile r
+__device__ __forceinline__ int expert_of(const int *first, int experts, int r) {
+    int lo = 0, hi = experts - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first[mid] <= r) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// ---- without tensor cores ------------------------------------------------------------------------
+
+constexpr int kPlainTile = 64, kPlainStep = 16;
+
+// One block per tile of 64 x 64, a thread 4 x 4 of it.  AK / BK: consecutive k are consecutive in memory.
+template <typename T, typename TO, bool GRAD, bool AK, bool BK>
+__global__ void __launch_bounds__(256)
+    expert_mm_plain_kernel(const int *__restrict__ offsets, int experts, int64_t rows, int m_size, int n_size, int k_size,
+                           const T *__restrict__ a, int64_t lda, int64_t stride_a, const T *__restrict__ b, int64_t ldb,
+                           int64_t stride_b, float beta, TO *__restrict__ c, int64_t ldc, int64_t stride_c) {
+    __shared__ int s_first[kMostExperts + 1];
+    __shared__ __align__(16) float s_a[kPlainStep][kPlainTile + 4], s_b[kPlainStep][kPlainTile + 4];  // read four at a time
+    int e, lo, hi, m0, m_end, k_end;
+    const int n0 = blockIdx.x * kPlainTile;
+    if (GRAD) {
+        e = blockIdx.z;
+        rows_of(offsets, e, rows, &lo, &hi);
+        m0 = blockIdx.y * kPlainTile, m_end = m_size, k_end = hi - lo;
+    } else {
+        if (threadIdx.x < 32) count_row_tiles(offsets, experts, rows, kPlainTile, s_first);
+        __syncthreads();
+        const int r = (int)(blockIdx.y + blockIdx.z * gridDim.y);
+        if (r >= s_first[experts]) return;
+        e = expert_of(s_first, experts, r);
+        rows_of(offsets, e, rows, &lo, &hi);
+        m0 = (r - s_first[e]) * kPlainTile, m_end = hi - lo, k_end = k_size;
+    }
+    // the operand that is indexed by rows begins at the expert's first
+    const T *pa = a + lo * lda + e * stride_a;
+    const T *pb = b + (GRAD ? lo * ldb : 0) + e * stride_b;
+    float acc[4][4] = {};
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    for (int k0 = 0; k0 < k_end; k0 += kPlainStep) {
+#pragma unroll
+        for (int i = threadIdx.x; i < kPlainTile * kPlainStep; i += 256) {
+            const int am = AK ? i / kPlainStep : i % kPlainTile, ak = AK ? i % kPlainStep : i / kPlainTile;
+            s_a[ak][am] = m0 + am < m_end && k0 + ak < k_end ? to_float(AK ? pa[(int64_t)(m0 + am) * lda + k0 + ak] : pa[(int64_t)(k0 + ak) * lda + m0 + am]) : 0.f;
+            const int bn = BK ? i / kPlainStep : i % kPlainTile, bk = BK ? i % kPlainStep : i / kPlainTile;
+            s_b[bk][bn] = n0 + bn < n_size && k0 + bk < k_end ? to_float(BK ? pb[(int64_t)(n0 + bn) * ldb + k0 + bk] : pb[(int64_t)(k0 + bk) * ldb + n0 + bn]) : 0.f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kPlainStep; k++) {
+            const float4 va = *reinterpret_cast<const float4 *>(&s_a[k][ty * 4]), vb = *reinterpret_cast<const float4 *>(&s_b[k][tx * 4]);
+            const float fa[4] = {va.x, va.y, va.z, va.w}, fb[4] = {vb.x, vb.y, vb.z, vb.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(fa[i], fb[j], acc[i][j]);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int m = m0 + ty * 4 + i;
+        if (m >= m_end) continue;
+        TO *row = c + (GRAD ? e * stride_c + m * ldc : (int64_t)(lo + m) * ldc);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int n = n0 + tx * 4 + j;
+            if (n < n_size) row[n] = from_float<TO>(beta != 0.f ? fmaf(beta, to_float(row[n]), acc[i][j]) : acc[i][j]);
+        }
+    }
+}
+
+// ---- tensor cores --------------------------------------------------------------------------------
+
+constexpr int kMmThreads = 192;  // copies, products, four warps for the accumulators
+constexpr int kMmM = 128, kMmK = 64;
+constexpr int kMmMostStages = 8;
+constexpr unsigned long long kMmLimitNs = 2000000000ull;
+
+__device__ __forceinline__ unsigned smem_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void barrier_init(uint64_t *b, unsigned count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_address(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint64_t *b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_address(b)) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint64_t *b, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_address(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ unsigned long long now_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+// Waits for the phase of the given parity; false when it ran out of time or another thread of the block did.
+__device__ __forceinline__ bool barrier_wait(uint64_t *b, unsigned parity, volatile int *s_stop) {
+    unsigned long long begin = 0;
+    for (unsigned i = 0;; i++) {
+        unsigned done;
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(done)
+                     : "r"(smem_address(b)), "r"(parity)
+                     : "memory");
+        if (done) return true;
+        if ((i & 15) == 15) {
+            if (*s_stop) return false;
+            const unsigned long long t = now_ns();
+            if (!begin) begin = t;
+            else if (t - begin > kMmLimitNs) {
+                *s_stop = 1;
+                return false;
+            }
+        }
+    }
+}
+// ... by a whole warp, with one answer for all lanes
+__device__ __forceinline__ bool warp_wait(uint64_t *b, unsigned parity, volatile int *s_stop) {
+    return __all_sync(0xffffffffu, barrier_wait(b, parity, s_stop));
+}
+__device__ __forceinline__ void copy_tile(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *b) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                     smem_address(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_address(b))
+                 : "memory");
+}
+// Shared-memory descriptor of an operand whose rows are 128 bytes, swizzled by 128 bytes.  K-major: rows of 64 k, groups of
+// eight rows 1024 bytes apart.  M/N-major: rows of 64 m (or n) per k, groups of eight k 1024 bytes apart, and the next 64 m
+// 8192 bytes on (a box of 64 k).
+__device__ __forceinline__ uint64_t operand_descriptor(unsigned address, bool k_major) {
+    return (uint64_t)((address & 0x3ffff) >> 4) | (uint64_t)(k_major ? 1 : 8192 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void multiply(unsigned d, uint64_t a, uint64_t b, unsigned instruction, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
+                 "l"(b), "r"(instruction), "r"((unsigned)add)
+                 : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_address(b)) : "memory");
+}
+__device__ __forceinline__ void load_accumulators(unsigned address, float (&v)[32]) {
+    unsigned r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(address)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+
+struct MmShape {
+    const int *offsets;
+    int experts;
+    int64_t rows;
+    int features;      // kRowsFirst / kRowsLast: columns of the output; kGradient: columns of dy (rows of an expert's output)
+    int columns;       // kGradient: columns of x
+    int reduced;       // length of the sum (kGradient: the expert's rows)
+    int n, stages;     // tile of the second operand, depth of the ring
+    int feature_tiles, column_tiles;
+    unsigned b_bytes;  // shared memory of a stage's second operand
+    unsigned instruction, tmem, acc_stride;
+    bool vectors;      // rows of the output begin on 16-byte boundaries
+    float beta;
+};
+
+struct MmTile {
+    int expert, lo, hi, m0, n0, steps;
+};
+
+template <int FORM>
+__device__ __forceinline__ MmTile mm_tile(const MmShape &s, const int *s_first, int t) {
+    MmTile q;
+    if (FORM == kGradient) {
+        const int per = s.feature_tiles * s.column_tiles;
+        q.expert = t / per;
+        const int i = t - q.expert * per, f = i / s.column_tiles;
+        rows_of(s.offsets, q.expert, s.rows, &q.lo, &q.hi);
+        q.m0 = f * kMmM, q.n0 = (i - f * s.column_tiles) * s.n;
+        q.steps = (q.hi - q.lo + kMmK - 1) / kMmK;
+    } else {
+        const int r = t / s.feature_tiles, f = t - r * s.feature_tiles;
+        q.expert = expert_of(s_first, s.experts, r);
+        rows_of(s.offsets, q.expert, s.rows, &q.lo, &q.hi);
+        const int row_tile = r - s_first[q.expert];
+        q.lo += row_tile * (FORM == kRowsFirst ? kMmM : s.n);
+        q.m0 = FORM == kRowsFirst ? q.lo : f * kMmM;
+        q.n0 = FORM == kRowsFirst ? f * s.n : q.lo;
+        q.steps = (s.reduced + kMmK - 1) / kMmK;
+    }
+    return q;
+}
+
+// W_K: consecutive sums of the weights are consecutive in memory (K-major), else consecutive features are
+template <int FORM, bool W_K, typename T, typename TO>
+__global__ void __launch_bounds__(kMmThreads, 1)
+    expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MmShape s,
+                     TO *__restrict__ out, int64_t ldo, int64_t stride_o) {
+    constexpr bool a_k = FORM == kRowsFirst || (FORM == kRowsLast && W_K), b_k = FORM == kRowsLast || (FORM == kRowsFirst && W_K);
+    constexpr unsigned a_bytes = kMmM * kMmK * sizeof(T);
+    extern __shared__ __align__(16) char s_raw[];
+    __shared__ int s_first[kMostExperts + 1];
+    __shared__ uint64_t s_full[kMmMostStages], s_empty[kMmMostStages], s_acc_full[2], s_acc_empty[2];
+    __shared__ unsigned s_tmem;
+    __shared__ int s_stop_word;
+    volatile int *s_stop = &s_stop_word;
+    char *ring = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
+    const unsigned stage_bytes = a_bytes + s.b_bytes;
+    float4 *staging = reinterpret_cast<float4 *>(ring + (size_t)s.stages * stage_bytes);  // 4 KB for each of four warps
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (w == 0) {
+        if (lane == 0) {
+            for (int i = 0; i < s.stages; i++) barrier_init(&s_full[i], 1), barrier_init(&s_empty[i], 1);
+            for (int i = 0; i < 2; i++) barrier_init(&s_acc_full[i], 1), barrier_init(&s_acc_empty[i], 4);
+            s_stop_word = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+    } else if (w == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(&s_tmem)), "r"(s.tmem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else if (w == 2 && FORM != kGradient) {
+        count_row_tiles(s.offsets, s.experts, s.rows, FORM == kRowsFirst ? kMmM : s.n, s_first);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = s_tmem;
+    const int tiles = FORM == kGradient ? s.experts * s.feature_tiles * s.column_tiles : s_first[s.experts] * s.feature_tiles;
+
+    if (w == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            unsigned phase = 0;
+            bool good = true;
+            for (int t = blockIdx.x; good && t < tiles; t += gridDim.x) {
+                const MmTile q = mm_tile<FORM>(s, s_first, t);
+                for (int k = 0; k < q.steps; k++) {
+                    if (!(good = barrier_wait(&s_empty[stage], phase ^ 1, s_stop))) break;
+                    char *a = ring + (size_t)stage * stage_bytes, *b = a + a_bytes;
+                    uint64_t *full = &s_full[stage];
+                    barrier_expect(full, stage_bytes);
+                    const int k0 = k * kMmK;
+                    if (FORM == kGradient) {
+                        for (int g = 0; g < kMmM / 64; g++) copy_tile(a + g * 8192, &map_a, q.m0 + g * 64, q.lo + k0, 0, full);
+                        for (int g = 0; g < (int)(s.b_bytes >> 13); g++) copy_tile(b + g * 8192, &map_b, q.n0 + g * 64, q.lo + k0, 0, full);
+                    } else {
+                        if (a_k) copy_tile(a, &map_a, k0, q.m0, FORM == kRowsFirst ? 0 : q.expert, full);
+                        else
+                            for (int g = 0; g < kMmM / 64; g++) copy_tile(a + g * 8192, &map_a, q.m0 + g * 64, k0, q.expert, full);
+                        if (b_k) copy_tile(b, &map_b, k0, q.n0, FORM == kRowsLast ? 0 : q.expert, full);
+                        else
+                            for (int g = 0; g < (int)(s.b_bytes >> 13); g++) copy_tile(b + g * 8192, &map_b, q.n0 + g * 64, k0, q.expert, full);
+                    }
+                    if (++stage == s.stages) stage = 0, phase ^= 1;
+                }
+            }
+        }
+    } else if (w == 1) {
+        int stage = 0, count = 0;
+        unsigned phase = 0;
+        bool good = true;
+        for (int t = blockIdx.x; good && t < tiles; t += gridDim.x) {
+            const MmTile q = mm_tile<FORM>(s, s_first, t);
+            if (q.steps == 0) continue;
+            const int slot = count & 1;
+            if (!(good = warp_wait(&s_acc_empty[slot], ((count >> 1) & 1) ^ 1, s_stop))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            count++;
+            const int length = FORM == kGradient ? q.hi - q.lo : s.reduced;
+            for (int k = 0; k < q.steps; k++) {
+                if (!(good = warp_wait(&s_full[stage], phase, s_stop))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                char *a = ring + (size_t)stage * stage_bytes;
+                const int left = length - k * kMmK;
+                if (FORM == kGradient && left < kMmK) {
+                    // rows of the next expert (or behind the last) came along: zeros in both operands, so that nothing
+                    // that stands there, NaN included, gets into the sum
+                    const int per_box = (kMmK - left) * 8, boxes = (int)(stage_bytes >> 13);
+                    for (int i = lane; i < per_box * boxes; i += 32) {
+                        const int box = i / per_box;
+                        *reinterpret_cast<uint4 *>(a + (size_t)box * 8192 + left * 128 + (i - box * per_box) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                if (lane == 0) {
+                    const uint64_t da = operand_descriptor(smem_address(a), a_k), db = operand_descriptor(smem_address(a + a_bytes), b_k);
+                    const int parts = min(4, (left + 15) / 16);
+                    for (int i = 0; i < parts; i++)
+                        multiply(tmem + slot * s.acc_stride, da + (uint64_t)(i * (a_k ? 32 : 2048) >> 4), db + (uint64_t)(i * (b_k ? 32 : 2048) >> 4),
+                                 s.instruction, k > 0 || i > 0);
+                    commit(&s_empty[stage]);
+                    if (k == q.steps - 1) commit(&s_acc_full[slot]);
+                }
+                __syncwarp();
+                if (++stage == s.stages) stage = 0, phase ^= 1;
+            }
+        }
+    } else {
+        const int part = w & 3;  // the quarter of the accumulators' lanes that this warp may read
+        int count = 0;
+        for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+            const MmTile q = mm_tile<FORM>(s, s_first, t);
+            const int slot = count & 1;
+            if (q.steps > 0) {
+                if (!warp_wait(&s_acc_full[slot], (count >> 1) & 1, s_stop)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                count++;
+            }
+            const unsigned from = tmem + slot * s.acc_stride + ((unsigned)(part * 32) << 16);
+            if (FORM == kRowsLast) {
+                // a lane is a feature, a column a row of the output: 32 consecutive features of a row at a time
+                const int f = q.m0 + part * 32 + lane, n = min(s.n, q.hi - q.lo);
+                for (int c = 0; c < n; c += 32) {
+                    float v[32];
+                    load_accumulators(from + c, v);
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (c + i < n && f < s.features) out[(int64_t)(q.lo + c + i) * ldo + f] = from_float<TO>(v[i]);
+                }
+            } else {
+                // a lane is a row of the output; 32 columns at a time pass through shared memory, so that rows are written
+                // in whole sectors by neighbouring lanes
+                float4 *mine = staging + part * 256;
+                TO *base = out + (FORM == kGradient ? q.expert * stride_o + (int64_t)q.m0 * ldo : (int64_t)q.m0 * ldo);
+                const int m_end = FORM == kGradient ? s.features - q.m0 : q.hi - q.lo;
+                const int n_end = min(s.n, (FORM == kGradient ? s.columns : s.features) - q.n0);
+                constexpr int E = 16 / sizeof(TO), across = 32 / E, down = 32 / across;
+                for (int c = 0; c < n_end; c += 32) {
+                    float v[32];
+                    if (q.steps > 0) load_accumulators(from + c, v);
+                    else {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] = 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) mine[lane * 8 + (i ^ (lane & 7))] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    __syncwarp();
+                    const int column = lane % across;
+#pragma unroll
+                    for (int i = 0; i < 32 / down; i++) {
+                        const int r = i * down + lane / across, m = part * 32 + r, n = c + column * E;
+                        if (m >= m_end || n >= n_end) continue;
+                        float x[E];
+#pragma unroll
+                        for (int j = 0; j < E / 4; j++) {
+                            const float4 p = mine[r * 8 + ((column * (E / 4) + j) ^ (r & 7))];
+                            x[4 * j] = p.x, x[4 * j + 1] = p.y, x[4 * j + 2] = p.z, x[4 * j + 3] = p.w;
+                        }
+                        TO *dst = base + (int64_t)m * ldo + q.n0 + n;
+                        if (s.vectors && n + E <= n_end) {
+                            Pack<TO, E> o;
+                            if (s.beta != 0.f) o = *reinterpret_cast<const Pack<TO, E> *>(dst);
+#pragma unroll
+                            for (int j = 0; j < E; j++)
+                                o.v[j] = from_float<TO>(s.beta != 0.f ? fmaf(s.beta, to_float(o.v[j]), x[j]) : x[j]);
+                            store_pack<TO, E>(dst, o);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < E; j++)
+                                if (n + j < n_end) dst[j] = from_float<TO>(s.beta != 0.f ? fmaf(s.beta, to_float(dst[j]), x[j]) : x[j]);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            if (q.steps > 0) {
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) barrier_arrive(&s_acc_empty[slot]);
+            }
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (*s_stop) {
+        // a wait ran out: what is still on its way into shared memory gets time to arrive before the block goes
+        if (threadIdx.x == 0) {
+            atomicExch(&g_expert_mm_status, 1);
+            const unsigned long long begin = now_ns();
+            while (now_ns() - begin < 10000000ull) __nanosleep(1000);
+        }
+        __syncthreads();
+    }
+    if (w == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(s.tmem));
+    }
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled() {
+    static const EncodeTiled f = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return f;
+}
+
+// `width` x `rows` x `count` elements of 16 bits, boxes of 64 x box_rows
+static bool make_map(CUtensorMap *map, alphasparse_cuda_type_t type, const void *p, int64_t width, int64_t rows, int64_t ld,
+                     int64_t count, int64_t stride, int box_rows) {
+    const EncodeTiled f = encode_tiled();
+    if (!f) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)rows, (cuuint64_t)count};
+    // distances of dimensions of one element are never used, but have to be legal
+    const cuuint64_t strides[2] = {(cuuint64_t)(rows > 1 ? ld * 2 : (width * 2 + 15) / 16 * 16), (cuuint64_t)(count > 1 ? stride * 2 : 16)};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+    return f(map, type == ALPHA_SPARSE_CUDA_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+             const_cast<void *>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static bool takes_tma(const void *p, int64_t ld, int64_t rows, int64_t stride, int64_t count) {
+    return address(p) % 16 == 0 && (rows <= 1 || ld % 8 == 0) && (count <= 1 || (stride % 8 == 0 && stride < (int64_t)1 << 38));
+}
+
+static cudaError_t multiprocessors(int *n) {
+    int dev;
+    const cudaError_t e = cudaGetDevice(&dev);
+    return e != cudaSuccess ? e : cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, dev);
+}
+
+// Fills what follows from the tile, and launches.
+template <int FORM, bool W_K, typename T, typename TO>
+static cudaError_t launch_mm(alphasparse_cuda_type_t type, MmShape s, int64_t most_tiles, const CUtensorMap &a, const CUtensorMap &b, TO *out,
+                             int64_t ldo, int64_t stride_o, cudaStream_t st) {
+    constexpr bool a_k = FORM == kRowsFirst || (FORM == kRowsLast && W_K), b_k = FORM == kRowsLast || (FORM == kRowsFirst && W_K);
+    constexpr int most_smem = 232448 - 8192, staging = 16384;  // the tables and barriers are in what is left
+    s.b_bytes = (unsigned)(b_k ? s.n * kMmK : (s.n + 63) / 64 * 64 * kMmK) * 2;
+    const unsigned stage = kMmM * kMmK * 2 + s.b_bytes;
+    s.stages = std::min<int>(kMmMostStages, (most_smem - 1024 - staging) / (int)stage);
+    const unsigned format = type == ALPHA_SPARSE_CUDA_TYPE_BF16 ? 1 : 0;
+    s.instruction = 1u << 4 | format << 7 | format << 10 | (a_k ? 0u : 1u << 15) | (b_k ? 0u : 1u << 16) | (unsigned)(s.n >> 3) << 17 |
+                    (unsigned)(kMmM >> 4) << 24;
+    s.acc_stride = 32;
+    while ((int)s.acc_stride < s.n) s.acc_stride *= 2;
+    s.tmem = 2 * s.acc_stride;
+    s.vectors = address(out) % 16 == 0 && ldo * (int64_t)sizeof(TO) % 16 == 0 && (FORM != kGradient || stride_o * (int64_t)sizeof(TO) % 16 == 0);
+    const auto kernel = expert_mm_kernel<FORM, W_K, T, TO>;
+    const int smem = 1024 + s.stages * (int)stage + staging;
+    int sms = 0;
+    cudaError_t e = multiprocessors(&sms);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    kernel<<<(unsigned)std::min<int64_t>(sms, most_tiles), kMmThreads, smem, st>>>(a, b, s, out, ldo, stride_o);
+    return cudaGetLastError();
+}
+
+static int64_t up_to(int64_t v, int64_t unit) { return (v + unit - 1) / unit * unit; }
+
+}  // namespace asb
+
+using namespace asb;
+
+static bool mm_sizes_fit(int64_t experts, int64_t rows, int64_t a, int64_t b) {
+    return experts >= 1 && rows >= 0 && rows <= kMostRows && a >= 0 && a <= kMostWidth && b >= 0 && b <= kMostWidth;
+}
+
+// the weights of all experts as one operand: rows within an expert are checked here
+static alphasparse_status_t check_weights(const char *call, int64_t out, int64_t in, int64_t ld, int64_t stride, int64_t experts) {
+    if ((out > 1 && ld < in) || ld > kMostStride || (experts > 1 && stride < (out > 0 ? (out - 1) * ld + in : 0)) || stride >= (int64_t)1 << 40) {
+        char msg[160];
+        snprintf(msg, sizeof(msg), "%s: leading dimension below the width, or matrices of the experts that overlap", call);
+        record_error(msg);
+        return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    }
+    return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+static Operand weights_operand(const void *w, int64_t experts, int64_t out, int64_t in, int64_t ld, int64_t stride, size_t elem, bool written) {
+    const bool any = experts > 0 && out > 0 && in > 0;
+    return Operand{w, any ? 1 : 0, any ? (experts - 1) * stride + (out - 1) * ld + in : 0, 0, elem, written};
+}
+
+extern "C" alphasparse_status_t alphasparse_cuda_expert_mm(alphasparse_operation_t operation, alphasparse_cuda_type_t type, int64_t experts,
+                                                           int64_t rows, const int32_t *offsets, int64_t out, int64_t in, const void *x,
+                                                           int64_t ldx, const void *w, int64_t ldw, int64_t stride_w, void *y, int64_t ldy) {
+    const size_t eb = type_bytes(type);
+    if (!eb || !mm_sizes_fit(experts, rows, out, in)) return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    if (operation != ALPHA_SPARSE_OPERATION_NON_TRANSPOSE && operation != ALPHA_SPARSE_OPERATION_TRANSPOSE) return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    if (experts > kMostExperts) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+    const bool trans = operation == ALPHA_SPARSE_OPERATION_TRANSPOSE;
+    const int64_t features = trans ? out : in, reduced = trans ? in : out;
+    if (rows == 0 || features == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
+    alphasparse_status_t status = check_weights("alphasparse_cuda_expert_mm", out, in, ldw, stride_w, experts);
+    if (status != ALPHA_SPARSE_STATUS_SUCCESS) return status;
+    status = check_operands("alphasparse_cuda_expert_mm", {{offsets, 1, experts + 1, experts + 1, sizeof(int), false},
+                                                           {x, rows, reduced, ldx, eb, false},
+                                                           weights_operand(w, experts, out, in, ldw, stride_w, eb, false),
+                                                           {y, rows, features, ldy, eb, true}});
+    if (status != ALPHA_SPARSE_STATUS_SUCCESS) return status;
+    cudaStream_t st = current_stream();
+    cudaError_t e = cudaSuccess;
+    if (eb == 2 && reduced > 0 && takes_tma(x, ldx, rows, 0, 1) && takes_tma(w, ldw, out, stride_w, experts)) {
+        MmShape s{};
+        s.offsets = offsets, s.experts = (int)experts, s.rows = rows, s.features = (int)features, s.reduced = (int)reduced;
+        // Few rows an expert: they make the narrow side of the tile.
+        const int64_t mean = (rows + experts - 1) / experts;
+        const bool last = mean <= 64;
+        CUtensorMap mx, mw;
+        bool made;
+        if (last) {
+            s.n = mean <= 16 ? 32 : mean <= 32 ? 64 : 128;
+            s.feature_tiles = (int)((features + kMmM - 1) / kMmM);
+            made = make_map(&mx, type, x, reduced, rows, ldx, 1, 0, s.n) && make_map(&mw, type, w, in, out, ldw, experts, stride_w, trans ? kMmM : kMmK);
+        } else {
+            // equal tiles of at most 256 features
+            s.feature_tiles = (int)((features + 255) / 256);
+            s.n = (int)up_to((features + s.feature_tiles - 1) / s.feature_tiles, 16);
+            made = make_map(&mx, type, x, reduced, rows, ldx, 1, 0, kMmM) && make_map(&mw, type, w, in, out, ldw, experts, stride_w, trans ? s.n : kMmK);
+        }
+        if (!made) {
+            record_error("alphasparse_cuda_expert_mm: no tensor map");
+            return ALPHA_SPARSE_STATUS_EXECUTION_FAILED;
+        }
+        const int64_t row_tiles = rows / (last ? s.n : kMmM) + std::min(experts, rows), tiles = row_tiles * s.feature_tiles;
+        if (tiles > 0x7fffffff - 4096) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+        const auto go = [&](auto t) {
+            using T = decltype(t);
+            if (last && trans) e = launch_mm<kRowsLast, true, T, T>(type, s, tiles, mw, mx, (T *)y, ldy, 0, st);
+            else if (last) e = launch_mm<kRowsLast, false, T, T>(type, s, tiles, mw, mx, (T *)y, ldy, 0, st);
+            else if (trans) e = launch_mm<kRowsFirst, true, T, T>(type, s, tiles, mx, mw, (T *)y, ldy, 0, st);
+            else e = launch_mm<kRowsFirst, false, T, T>(type, s, tiles, mx, mw, (T *)y, ldy, 0, st);
+        };
+        if (type == ALPHA_SPARSE_CUDA_TYPE_F16) go(__half());
+        else go(__nv_bfloat16());
+    } else {
+        const int64_t row_tiles = rows / kPlainTile + std::min(experts, rows);
+        const dim3 grid((unsigned)((features + kPlainTile - 1) / kPlainTile), (unsigned)std::min<int64_t>(row_tiles, 32768),
+                        (unsigned)((row_tiles + 32767) / 32768));
+        const auto go = [&](auto t) {
+            using T = decltype(t);
+            const auto kernel = trans ? expert_mm_plain_kernel<T, T, false, true, true> : expert_mm_plain_kernel<T, T, false, true, false>;
+            kernel<<<grid, 256, 0, st>>>(offsets, (int)experts, rows, 0, (int)features, (int)reduced, (const T *)x, ldx, 0, (const T *)w, ldw, stride_w,
+                                         0.f, (T *)y, ldy, 0);
+            e = cudaGetLastError();
+        };
+        ASB_BY_TYPE(type, go)
+    }
+    ASB_CUDA_OR(e, ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    count_launch();
+    return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+
+extern "C" alphasparse_status_t alphasparse_cuda_expert_mm_grad(alphasparse_cuda_type_t type, alphasparse_cuda_type_t weight_type, int64_t experts,
+                                                                int64_t rows, const int32_t *offsets, int64_t out, int64_t in, const void *dy,
+                                                                int64_t lddy, const void *x, int64_t ldx, float beta, void *dw, int64_t ldw,
+                                                                int64_t stride_w) {
+    const size_t eb = type_bytes(type), ob = type_bytes(weight_type);
+    if (!eb || !ob || !mm_sizes_fit(experts, rows, out, in)) return ALPHA_SPARSE_STATUS_INVALID_VALUE;
+    if (experts > kMostExperts || (weight_type != type && weight_type != ALPHA_SPARSE_CUDA_TYPE_F32)) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+    if (out == 0 || in == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
+    alphasparse_status_t status = check_weights("alphasparse_cuda_expert_mm_grad", out, in, ldw, stride_w, experts);
+    if (status != ALPHA_SPARSE_STATUS_SUCCESS) return status;
+    status = check_operands("alphasparse_cuda_expert_mm_grad", {{offsets, 1, experts + 1, experts + 1, sizeof(int), false},
+                                                                {dy, rows, out, lddy, eb, false},
+                                                                {x, rows, in, ldx, eb, false},
+                                                                weights_operand(dw, experts, out, in, ldw, stride_w, ob, true)});
+    if (status != ALPHA_SPARSE_STATUS_SUCCESS) return status;
+    cudaStream_t st = current_stream();
+    cudaError_t e = cudaSuccess;
+    if (eb == 2 && rows > 0 && takes_tma(dy, lddy, rows, 0, 1) && takes_tma(x, ldx, rows, 0, 1)) {
+        MmShape s{};
+        s.offsets = offsets, s.experts = (int)experts, s.rows = rows, s.features = (int)out, s.columns = (int)in, s.beta = beta;
+        s.feature_tiles = (int)((out + kMmM - 1) / kMmM);
+        s.column_tiles = (int)((in + 255) / 256);
+        s.n = (int)up_to((in + s.column_tiles - 1) / s.column_tiles, 16);
+        CUtensorMap my, mx;
+        if (!make_map(&my, type, dy, out, rows, lddy, 1, 0, kMmK) || !make_map(&mx, type, x, in, rows, ldx, 1, 0, kMmK)) {
+            record_error("alphasparse_cuda_expert_mm_grad: no tensor map");
+            return ALPHA_SPARSE_STATUS_EXECUTION_FAILED;
+        }
+        const int64_t tiles = experts * s.feature_tiles * s.column_tiles;
+        if (tiles > 0x7fffffff - 4096) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+        const auto go = [&](auto t) {
+            using T = decltype(t);
+            if (weight_type == ALPHA_SPARSE_CUDA_TYPE_F32) e = launch_mm<kGradient, false, T, float>(type, s, tiles, my, mx, (float *)dw, ldw, stride_w, st);
+            else e = launch_mm<kGradient, false, T, T>(type, s, tiles, my, mx, (T *)dw, ldw, stride_w, st);
+        };
+        if (type == ALPHA_SPARSE_CUDA_TYPE_F16) go(__half());
+        else go(__nv_bfloat16());
+    } else {
+        if ((out + kPlainTile - 1) / kPlainTile > 65535) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+        const dim3 grid((unsigned)((in + kPlainTile - 1) / kPlainTile), (unsigned)((out + kPlainTile - 1) / kPlainTile), (unsigned)experts);
+        const auto go = [&](auto t) {
+            using T = decltype(t);
+            if (weight_type == ALPHA_SPARSE_CUDA_TYPE_F32)
+                expert_mm_plain_kernel<T, float, true, false, false><<<grid, 256, 0, st>>>(offsets, (int)experts, rows, (int)out, (int)in, 0, (const T *)dy, lddy, 0,
+                                                                                        (const T *)x, ldx, 0, beta, (float *)dw, ldw, stride_w);
+            else
+                expert_mm_plain_kernel<T, T, true, false, false><<<grid, 256, 0, st>>>(offsets, (int)experts, rows, (int)out, (int)in, 0, (const T *)dy, lddy, 0,
+                                                                                    (const T *)x, ldx, 0, beta, (T *)dw, ldw, stride_w);
+            e = cudaGetLastError();
+        };
+        ASB_BY_TYPE(type, go)
+    }
+    ASB_CUDA_OR(e, ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    count_launch();
+    return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+
+extern "C" alphasparse_status_t alphasparse_cuda_expert_mm_status(int *status, int clear) {
+    if (!status) return ALPHA_SPARSE_STATUS_NOT_INITIALIZED;
+    cudaStream_t st = current_stream();
+    void *word = nullptr;
+    ASB_CUDA_OR(cudaGetSymbolAddress(&word, g_expert_mm_status), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    ASB_CUDA_OR(cudaMemcpyAsync(status, word, sizeof(int), cudaMemcpyDeviceToHost, st), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    ASB_CUDA_OR(cudaStreamSynchronize(st), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    if (clear) ASB_CUDA_OR(cudaMemsetAsync(word, 0, sizeof(int), st), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    return ALPHA_SPARSE_STATUS_SUCCESS;
+}

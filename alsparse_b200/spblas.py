@@ -410,3 +410,33 @@ def expert_combine_grad(dout, y, slot, weight, dy, dweight):
         return capi.INVALID_VALUE
     return capi.load().alphasparse_cuda_expert_combine_grad(_type(y), slot.shape[0], slot.shape[1], y.shape[1], y.shape[0], _ptr(dout), ldo,
                                                             _ptr(y), ldy, _ptr(slot), lds, _ptr(weight), ldw, _ptr(dy), lddy, _ptr(dweight), lddw)
+
+
+def expert_mm(operation, offsets, x, w, y):
+    """alphasparse_cuda_expert_mm: y[r] = x[r] * op(w[e]) for the rows r from offsets[e] to offsets[e + 1]; w (experts, out, in).
+    Returns the status."""
+    ldx, ldy, lw = _rows(x), _rows(y), _rows(w, 3)
+    if None in (ldx, ldy, lw) or x.dtype != w.dtype or y.dtype != w.dtype or x.shape[0] != y.shape[0] or not _is(offsets, "int32") \
+            or tuple(offsets.shape) != (w.shape[0] + 1,) or (offsets.shape[0] > 1 and _strides(offsets)[0] != 1):
+        return capi.INVALID_VALUE
+    if (x.shape[1], y.shape[1]) != ((w.shape[2], w.shape[1]) if operation == TRANSPOSE else (w.shape[1], w.shape[2])):
+        return capi.INVALID_VALUE
+    return capi.load().alphasparse_cuda_expert_mm(operation, _type(w), w.shape[0], x.shape[0], _ptr(offsets), w.shape[1], w.shape[2], _ptr(x), ldx,
+                                                  _ptr(w), lw[1], lw[0], _ptr(y), ldy)
+
+
+def expert_mm_grad(offsets, dy, x, beta, dw):
+    """alphasparse_cuda_expert_mm_grad: dw[e] = dy[rows of e]^T x[rows of e] + beta * dw[e].  Returns the status."""
+    ldx, lddy, lw = _rows(x), _rows(dy), _rows(dw, 3)
+    if None in (ldx, lddy, lw) or x.dtype != dy.dtype or x.shape[0] != dy.shape[0] or tuple(dw.shape[1:]) != (dy.shape[1], x.shape[1]) \
+            or not _is(offsets, "int32") or tuple(offsets.shape) != (dw.shape[0] + 1,) or (offsets.shape[0] > 1 and _strides(offsets)[0] != 1):
+        return capi.INVALID_VALUE
+    return capi.load().alphasparse_cuda_expert_mm_grad(_type(x), _type(dw), dw.shape[0], x.shape[0], _ptr(offsets), dw.shape[1], dw.shape[2],
+                                                       _ptr(dy), lddy, _ptr(x), ldx, beta, _ptr(dw), lw[1], lw[0])
+
+
+def expert_mm_status(clear=False):
+    """alphasparse_cuda_expert_mm_status: (status, 1 if a wait of a product ran out)."""
+    v = C.c_int()
+    st = capi.load().alphasparse_cuda_expert_mm_status(C.byref(v), 1 if clear else 0)
+    return st, v.value

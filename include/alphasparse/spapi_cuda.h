@@ -292,6 +292,30 @@ alphasparse_status_t alphasparse_cuda_expert_combine_grad(alphasparse_cuda_type_
                                                           const float *weight, int64_t ldw, void *dy, int64_t lddy,
                                                           float *dweight, int64_t lddw);
 
+/* Products of the experts' rows: y[r] = x[r] * op(w[e]) for the rows r in [offsets[e], offsets[e + 1]), e < experts.  w[e] is
+ * row-major, out x in, at w + e * stride_w.  ALPHA_SPARSE_OPERATION_TRANSPOSE: x has `in` columns and y `out` (weights
+ * stored an output feature a row); NON_TRANSPOSE: x has `out` columns and y `in` (weights stored the other way
+ * round, and the gradient of x from that of y).  offsets (experts + 1 ints on the device) ascend within [0, rows]; rows of y
+ * outside them are left as they were.  The matrices of two experts do not overlap.  F16 and BF16 whose rows begin on 16-byte
+ * boundaries run on the tensor cores; F32 and others on the ordinary units, for completeness.  Up to 1024 experts. */
+alphasparse_status_t alphasparse_cuda_expert_mm(alphasparse_operation_t operation, alphasparse_cuda_type_t type,
+                                                int64_t experts, int64_t rows, const int32_t *offsets, int64_t out,
+                                                int64_t in, const void *x, int64_t ldx, const void *w, int64_t ldw,
+                                                int64_t stride_w, void *y, int64_t ldy);
+
+/* Gradient of the weights (operation TRANSPOSE): dw[e] = (sum over the rows r of e of dy[r]^T x[r]) + beta * dw[e], elements
+ * of weight_type (that of dy and x, or F32); an expert without rows gets beta * dw[e].  For weights stored the other
+ * way round exchange dy with x and out with in. */
+alphasparse_status_t alphasparse_cuda_expert_mm_grad(alphasparse_cuda_type_t type, alphasparse_cuda_type_t weight_type,
+                                                     int64_t experts, int64_t rows, const int32_t *offsets, int64_t out,
+                                                     int64_t in, const void *dy, int64_t lddy, const void *x,
+                                                     int64_t ldx, float beta, void *dw, int64_t ldw, int64_t stride_w);
+
+/* The kernels of the two calls above wait for their copies, each wait for two seconds at most.  Waits for the library stream
+ * and stores 1 if such a wait has run out on the current device (the outputs of that call are not complete), else 0;
+ * clear != 0 resets it. */
+alphasparse_status_t alphasparse_cuda_expert_mm_status(int *status, int clear);
+
 /* Error word of a handle's kernels.  Kernels that wait (the row-tile kernel waits for its bulk copies) give up
  * after a bounded number of polls, leave y untouched for their tile and record a code here: 1 = a tile larger
  * than the kernel was configured for, 2 = a bulk copy did not complete in time.  A call with host vectors

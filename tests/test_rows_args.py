@@ -104,3 +104,36 @@ def test_shapes_and_types_of_the_python_calls():
     assert spblas.expert_dispatch(y, i[:3], f((8, 8), np.float32)) == capi.INVALID_VALUE
     assert spblas.expert_combine(f((8, 8), np.float32), i, f((4, 3), np.float32), 0.0, y) == capi.INVALID_VALUE
     assert spblas.expert_combine_grad(y, f((8, 8), np.float32), i, w, f((8, 7), np.float32), w.copy()) == capi.INVALID_VALUE
+
+
+@pytest.mark.parametrize("change,want", [({0: 2}, capi.INVALID_VALUE), ({1: 5}, capi.INVALID_VALUE), ({2: 0}, capi.INVALID_VALUE), ({2: 5000}, capi.NOT_SUPPORTED),
+                                         ({3: -1}, capi.INVALID_VALUE), ({4: None}, capi.NOT_INITIALIZED), ({5: 1 << 25}, capi.INVALID_VALUE), ({7: None}, capi.NOT_INITIALIZED),
+                                         ({9: None}, capi.NOT_INITIALIZED), ({12: None}, capi.NOT_INITIALIZED), ({8: 15}, capi.INVALID_VALUE), ({10: 15}, capi.INVALID_VALUE),
+                                         ({11: 16 * 31}, capi.INVALID_VALUE), ({13: 31}, capi.INVALID_VALUE), ({12: A}, capi.INVALID_VALUE), ({12: 3 * A + 64}, capi.INVALID_VALUE),
+                                         ({3: 0, 7: None, 12: None}, capi.SUCCESS), ({5: 0}, capi.SUCCESS)])
+def test_expert_mm(change, want):
+    args = [capi.TRANSPOSE, capi.TYPE_BF16, 4, 100, 2 * A, 32, 16, A, 16, 3 * A, 16, 512, 5 * A, 32]
+    for at, v in change.items():
+        args[at] = v
+    assert call("expert_mm", *args) == want
+
+
+@pytest.mark.parametrize("change,want", [({0: 5}, capi.INVALID_VALUE), ({1: capi.TYPE_F16}, capi.NOT_SUPPORTED), ({1: -1}, capi.INVALID_VALUE), ({4: None}, capi.NOT_INITIALIZED),
+                                         ({7: None}, capi.NOT_INITIALIZED), ({12: None}, capi.NOT_INITIALIZED), ({13: 15}, capi.INVALID_VALUE), ({14: 100}, capi.INVALID_VALUE),
+                                         ({12: A}, capi.INVALID_VALUE), ({5: 0, 12: None}, capi.SUCCESS)])
+def test_expert_mm_grad(change, want):
+    args = [capi.TYPE_BF16, capi.TYPE_F32, 4, 100, 2 * A, 32, 16, A, 32, 3 * A, 16, 0.0, 5 * A, 16, 512]
+    for at, v in change.items():
+        args[at] = v
+    assert call("expert_mm_grad", *args) == want
+
+
+def test_shapes_and_types_of_the_experts_products():
+    f = np.zeros
+    o, x, w, y = f(3, np.int32), f((6, 8), np.float16), f((2, 4, 8), np.float16), f((6, 4), np.float16)
+    for args in ((capi.TRANSPOSE, o[:2], x, w, y), (capi.NON_TRANSPOSE, o, x, w, y), (capi.TRANSPOSE, o, x[:5], w, y), (capi.TRANSPOSE, o, x, w.astype(np.float32), y),
+                 (capi.TRANSPOSE, o, x, w[0], y), (capi.TRANSPOSE, o, x[:, ::2], w, y)):
+        assert spblas.expert_mm(*args) == capi.INVALID_VALUE
+    assert spblas.expert_mm_grad(o, y, x, 0.0, f((2, 8, 4), np.float16)) == capi.INVALID_VALUE
+    assert spblas.expert_mm_grad(o, y, x[:5], 0.0, w) == capi.INVALID_VALUE
+    assert call("expert_mm_status", None, 0) == capi.NOT_INITIALIZED
