@@ -256,56 +256,88 @@ def read_coo(kind, path):
 
 
 # ---- products of matrices that are made at run time (device tensors) ------------------------------------------
+# Calls of a few microseconds: each operand's properties are read once.
 
 _TYPES = {"float32": capi.TYPE_F32, "float16": capi.TYPE_F16, "bfloat16": capi.TYPE_BF16}
 _INDICES = {"int32": capi.INDEX_I32, "int64": capi.INDEX_I64}
+_NONE = -1                # element type that the library has no name for: it refuses the value
+_KINDS = {}               # element type of torch or numpy -> (enum of a value, enum of an index), -1 for none
 
 
-def _type(a, names=_TYPES):
-    """Enum value of an array's element type; -1, which the library refuses, for one that has none."""
-    return names.get(str(a.dtype).replace("torch.", ""), -1)
+def _kind(a):
+    kind = _KINDS.get(a.dtype)
+    if kind is None:
+        name = str(a.dtype).replace("torch.", "")
+        kind = _KINDS[a.dtype] = (_TYPES.get(name, _NONE), _INDICES.get(name, _NONE))
+    return kind
 
 
-def _strides(a):
+def _type(a):
+    return _kind(a)[0]
+
+
+def _f32(a):
+    return _kind(a)[0] == capi.TYPE_F32
+
+
+def _i32s(a):
+    return _kind(a)[1] == capi.INDEX_I32
+
+
+def _layout(a):
+    """(shape, strides in elements, address) of a numpy array or a torch tensor."""
     if isinstance(a, np.ndarray):
-        return tuple(s // a.itemsize for s in a.strides)
-    return tuple(a.stride())
+        return a.shape, tuple(s // a.itemsize for s in a.strides), a.ctypes.data
+    return a.shape, a.stride(), a.data_ptr()
 
 
-def _rows(a, dims=2):
-    """Leading dimension of a row-major array whose rows are contiguous, None if it is not one (the caller's view has to be
-    copied first).  Three dimensions: (distance of the matrices, leading dimension)."""
-    if a.ndim != dims:
+def _matrix(a):
+    """(rows, columns, leading dimension, address) of a row-major array whose rows are contiguous, None if it is not one (the
+    caller's view has to be copied first)."""
+    shape, s, at = _layout(a)
+    if len(s) != 2:
         return None
-    shape, s = tuple(a.shape), _strides(a)
-    if shape[-1] > 1 and s[-1] != 1:
+    rows, width = shape
+    ld, step = s
+    if step != 1 and width > 1:
         return None
-    ld = s[-2] if shape[-2] > 1 else max(s[-2], shape[-1])
-    if dims == 2:
-        return ld
-    return (s[0] if shape[0] > 1 else max(s[0], ld * shape[1]), ld)
+    return rows, width, ld if rows > 1 else max(ld, width), at
 
 
-def _is(a, name):
-    return str(a.dtype).replace("torch.", "") == name
+def _vector(a):
+    """(elements, distance, address) of an array of one dimension, None if it has another number of them."""
+    shape, s, at = _layout(a)
+    if len(s) != 1:
+        return None
+    return shape[0], s[0] if shape[0] > 1 else 1, at
+
+
+def _matrices(a):
+    """(matrices, rows, columns, leading dimension, distance of the matrices, address) of an array of three dimensions."""
+    shape, s, at = _layout(a)
+    if len(s) != 3:
+        return None
+    n, rows, width = shape
+    if s[2] != 1 and width > 1:
+        return None
+    ld = s[1] if rows > 1 else max(s[1], width)
+    return n, rows, width, ld, s[0] if n > 1 else max(s[0], ld * rows), at
 
 
 def _buffer(b):
     """Address and bytes of a workspace: a contiguous array, or None."""
     if b is None:
         return None, 0
-    return _ptr(b), b.nbytes if isinstance(b, np.ndarray) else b.numel() * b.element_size()
+    return _ptr(b), b.nbytes
 
 
 def embedding(tokens, table, scale, y):
     """alphasparse_cuda_embedding: y[i] = scale * table[tokens[i]].  tokens: one dimension of int32 or int64, any stride;
     table (vocab, width) and y (tokens, width) of one type, rows contiguous.  Returns the status."""
-    ldt, ldy = _rows(table), _rows(y)
-    if tokens.ndim != 1 or ldt is None or ldy is None or y.dtype != table.dtype or tuple(y.shape) != (tokens.shape[0], table.shape[1]):
+    t, e, o = _vector(tokens), _matrix(table), _matrix(y)
+    if t is None or e is None or o is None or y.dtype != table.dtype or o[0] != t[0] or o[1] != e[1]:
         return capi.INVALID_VALUE
-    return capi.load().alphasparse_cuda_embedding(_type(tokens, _INDICES), _type(table), tokens.shape[0], _ptr(tokens),
-                                                  _strides(tokens)[0] if tokens.shape[0] > 1 else 1, table.shape[0], table.shape[1],
-                                                  scale, _ptr(table), ldt, _ptr(y), ldy)
+    return capi.load().alphasparse_cuda_embedding(_kind(tokens)[1], _kind(table)[0], t[0], t[2], t[1], e[0], e[1], scale, e[3], e[2], o[3], o[2])
 
 
 def embedding_grad_buffer_size(tokens, vocab, width):
@@ -318,36 +350,38 @@ def embedding_grad_buffer_size(tokens, vocab, width):
 def embedding_grad(tokens, dy, alpha, beta, dtable, buffer):
     """alphasparse_cuda_embedding_grad: dtable[v] = alpha * (sum of dy[i] where tokens[i] == v) + beta * dtable[v].
     Returns the status."""
-    lddy, ldt = _rows(dy), _rows(dtable)
-    if tokens.ndim != 1 or lddy is None or ldt is None or tuple(dy.shape) != (tokens.shape[0], dtable.shape[1]):
+    t, d, o = _vector(tokens), _matrix(dy), _matrix(dtable)
+    if t is None or d is None or o is None or d[0] != t[0] or d[1] != o[1]:
         return capi.INVALID_VALUE
     at, size = _buffer(buffer)
-    return capi.load().alphasparse_cuda_embedding_grad(_type(tokens, _INDICES), _type(dy), _type(dtable), tokens.shape[0], _ptr(tokens),
-                                                       _strides(tokens)[0] if tokens.shape[0] > 1 else 1, dtable.shape[0], dtable.shape[1],
-                                                       alpha, _ptr(dy), lddy, beta, _ptr(dtable), ldt, at, size)
+    return capi.load().alphasparse_cuda_embedding_grad(_kind(tokens)[1], _kind(dy)[0], _kind(dtable)[0], t[0], t[2], t[1], o[0], o[1], alpha,
+                                                       d[3], d[2], beta, o[3], o[2], at, size)
 
 
 def route(score, logits, bias, groups, top_groups, renormalize, scale, index, weight):
     """alphasparse_cuda_route: the experts index (tokens, k; int32) of each row of logits (tokens, experts) and their
     weights (tokens, k; float32); bias: (experts,) float32 or None.  Returns the status."""
-    ldl, ldi, ldw = _rows(logits), _rows(index), _rows(weight)
-    if ldl is None or ldi is None or ldw is None or not _is(index, "int32") or not _is(weight, "float32") or tuple(index.shape) != tuple(weight.shape) \
-            or index.shape[0] != logits.shape[0]:
+    x, i, w = _matrix(logits), _matrix(index), _matrix(weight)
+    if x is None or i is None or w is None or not _i32s(index) or not _f32(weight) or i[:2] != w[:2] or i[0] != x[0]:
         return capi.INVALID_VALUE
-    if bias is not None and (not _is(bias, "float32") or tuple(bias.shape) != (logits.shape[1],) or (bias.shape[0] > 1 and _strides(bias)[0] != 1)):
-        return capi.INVALID_VALUE
-    return capi.load().alphasparse_cuda_route(score, _type(logits), logits.shape[0], logits.shape[1], _ptr(logits), ldl, _ptr(bias), groups,
-                                              top_groups, index.shape[1], 1 if renormalize else 0, scale, _ptr(index), ldi, _ptr(weight), ldw)
+    b = None
+    if bias is not None:
+        b = _vector(bias)
+        if b is None or not _f32(bias) or b[:2] != (x[1], 1):
+            return capi.INVALID_VALUE
+        b = b[2]
+    return capi.load().alphasparse_cuda_route(score, _kind(logits)[0], x[0], x[1], x[3], x[2], b, groups, top_groups, i[1],
+                                              1 if renormalize else 0, scale, i[3], i[2], w[3], w[2])
 
 
 def route_grad(score, logits, index, renormalize, scale, dweight, dlogits):
     """alphasparse_cuda_route_grad: dlogits from the gradient dweight of the weights of index.  Returns the status."""
-    ldl, ldi, ldw, ldd = _rows(logits), _rows(index), _rows(dweight), _rows(dlogits)
-    if None in (ldl, ldi, ldw, ldd) or not _is(index, "int32") or not _is(dweight, "float32") or dlogits.dtype != logits.dtype \
-            or tuple(dlogits.shape) != tuple(logits.shape) or tuple(index.shape) != tuple(dweight.shape) or index.shape[0] != logits.shape[0]:
+    x, i, w, d = _matrix(logits), _matrix(index), _matrix(dweight), _matrix(dlogits)
+    if x is None or i is None or w is None or d is None or not _i32s(index) or not _f32(dweight) or dlogits.dtype != logits.dtype \
+            or d[:2] != x[:2] or i[:2] != w[:2] or i[0] != x[0]:
         return capi.INVALID_VALUE
-    return capi.load().alphasparse_cuda_route_grad(score, _type(logits), logits.shape[0], logits.shape[1], _ptr(logits), ldl, index.shape[1],
-                                                   _ptr(index), ldi, 1 if renormalize else 0, scale, _ptr(dweight), ldw, _ptr(dlogits), ldd)
+    return capi.load().alphasparse_cuda_route_grad(score, _kind(logits)[0], x[0], x[1], x[3], x[2], i[1], i[3], i[2], 1 if renormalize else 0,
+                                                   scale, w[3], w[2], d[3], d[2])
 
 
 def expert_plan_buffer_size(tokens, k, experts):
@@ -360,79 +394,73 @@ def expert_plan_buffer_size(tokens, k, experts):
 def expert_plan(index, offsets, slot, buffer):
     """alphasparse_cuda_expert_plan: offsets (experts + 1) and slot (tokens, k) of index (tokens, k), all int32.  Returns
     the status."""
-    ldi, lds = _rows(index), _rows(slot)
-    if ldi is None or lds is None or tuple(slot.shape) != tuple(index.shape) or offsets.ndim != 1 or (offsets.shape[0] > 1 and _strides(offsets)[0] != 1) \
-            or not all(_is(a, "int32") for a in (index, offsets, slot)):
+    i, s, o = _matrix(index), _matrix(slot), _vector(offsets)
+    if i is None or s is None or o is None or i[:2] != s[:2] or o[1] != 1 or not _i32s(index) or not _i32s(offsets) or not _i32s(slot):
         return capi.INVALID_VALUE
     at, size = _buffer(buffer)
-    return capi.load().alphasparse_cuda_expert_plan(index.shape[0], index.shape[1], offsets.shape[0] - 1, _ptr(index), ldi, _ptr(offsets),
-                                                    _ptr(slot), lds, at, size)
+    return capi.load().alphasparse_cuda_expert_plan(i[0], i[1], o[0] - 1, i[3], i[2], o[2], s[3], s[2], at, size)
 
 
 def expert_dispatch(x, slot, xs):
     """alphasparse_cuda_expert_dispatch: xs[slot[t, j]] = x[t].  Returns the status."""
-    ldx, lds, ldxs = _rows(x), _rows(slot), _rows(xs)
-    if None in (ldx, lds, ldxs) or not _is(slot, "int32") or xs.dtype != x.dtype or slot.shape[0] != x.shape[0] or xs.shape[1] != x.shape[1]:
+    a, s, o = _matrix(x), _matrix(slot), _matrix(xs)
+    if a is None or s is None or o is None or not _i32s(slot) or xs.dtype != x.dtype or s[0] != a[0] or o[1] != a[1]:
         return capi.INVALID_VALUE
-    return capi.load().alphasparse_cuda_expert_dispatch(_type(x), x.shape[0], slot.shape[1], x.shape[1], _ptr(x), ldx, _ptr(slot), lds,
-                                                        xs.shape[0], _ptr(xs), ldxs)
+    return capi.load().alphasparse_cuda_expert_dispatch(_kind(x)[0], a[0], s[1], a[1], a[3], a[2], s[3], s[2], o[0], o[3], o[2])
 
 
 def _weights(weight, slot):
-    """Leading dimension of the weights of slot (0 for None), or None if they do not fit it."""
+    """(leading dimension, address) of the weights of the slots (0, None for None), or None if they do not fit them."""
     if weight is None:
-        return 0
-    return _rows(weight) if _is(weight, "float32") and tuple(weight.shape) == tuple(slot.shape) else None
+        return 0, None
+    w = _matrix(weight)
+    return (w[2], w[3]) if w is not None and _f32(weight) and w[:2] == slot[:2] else None
 
 
 def expert_combine(y, slot, weight, beta, out):
     """alphasparse_cuda_expert_combine: out[t] = sum over j of weight[t, j] * y[slot[t, j]] + beta * out[t]; weight None: ones.
     Returns the status."""
-    ldy, lds, ldo = _rows(y), _rows(slot), _rows(out)
-    if None in (ldy, lds, ldo) or not _is(slot, "int32") or out.dtype != y.dtype or out.shape[0] != slot.shape[0] or out.shape[1] != y.shape[1]:
+    a, s, o = _matrix(y), _matrix(slot), _matrix(out)
+    if a is None or s is None or o is None or not _i32s(slot) or out.dtype != y.dtype or o[0] != s[0] or o[1] != a[1]:
         return capi.INVALID_VALUE
-    ldw = _weights(weight, slot)
-    if ldw is None:
+    w = _weights(weight, s)
+    if w is None:
         return capi.INVALID_VALUE
-    return capi.load().alphasparse_cuda_expert_combine(_type(y), slot.shape[0], slot.shape[1], y.shape[1], y.shape[0], _ptr(y), ldy, _ptr(slot),
-                                                       lds, _ptr(weight), ldw, beta, _ptr(out), ldo)
+    return capi.load().alphasparse_cuda_expert_combine(_kind(y)[0], s[0], s[1], a[1], a[0], a[3], a[2], s[3], s[2], w[1], w[0], beta, o[3], o[2])
 
 
 def expert_combine_grad(dout, y, slot, weight, dy, dweight):
     """alphasparse_cuda_expert_combine_grad: dy[slot[t, j]] = weight[t, j] * dout[t], dweight[t, j] = <dout[t], y[slot[t, j]]>.
     Returns the status."""
-    ldo, ldy, lds, lddy, lddw = _rows(dout), _rows(y), _rows(slot), _rows(dy), _rows(dweight)
-    if None in (ldo, ldy, lds, lddy, lddw) or not _is(slot, "int32") or not _is(dweight, "float32") or dout.dtype != y.dtype or dy.dtype != y.dtype \
-            or tuple(dy.shape) != tuple(y.shape) or tuple(dout.shape) != (slot.shape[0], y.shape[1]) or tuple(dweight.shape) != tuple(slot.shape):
+    o, a, s, d, g = _matrix(dout), _matrix(y), _matrix(slot), _matrix(dy), _matrix(dweight)
+    if o is None or a is None or s is None or d is None or g is None or not _i32s(slot) or not _f32(dweight) or dout.dtype != y.dtype \
+            or dy.dtype != y.dtype or d[:2] != a[:2] or o[:2] != (s[0], a[1]) or g[:2] != s[:2]:
         return capi.INVALID_VALUE
-    ldw = _weights(weight, slot)
-    if ldw is None:
+    w = _weights(weight, s)
+    if w is None:
         return capi.INVALID_VALUE
-    return capi.load().alphasparse_cuda_expert_combine_grad(_type(y), slot.shape[0], slot.shape[1], y.shape[1], y.shape[0], _ptr(dout), ldo,
-                                                            _ptr(y), ldy, _ptr(slot), lds, _ptr(weight), ldw, _ptr(dy), lddy, _ptr(dweight), lddw)
+    return capi.load().alphasparse_cuda_expert_combine_grad(_kind(y)[0], s[0], s[1], a[1], a[0], o[3], o[2], a[3], a[2], s[3], s[2], w[1], w[0],
+                                                            d[3], d[2], g[3], g[2])
 
 
 def expert_mm(operation, offsets, x, w, y):
     """alphasparse_cuda_expert_mm: y[r] = x[r] * op(w[e]) for the rows r from offsets[e] to offsets[e + 1]; w (experts, out, in).
     Returns the status."""
-    ldx, ldy, lw = _rows(x), _rows(y), _rows(w, 3)
-    if None in (ldx, ldy, lw) or x.dtype != w.dtype or y.dtype != w.dtype or x.shape[0] != y.shape[0] or not _is(offsets, "int32") \
-            or tuple(offsets.shape) != (w.shape[0] + 1,) or (offsets.shape[0] > 1 and _strides(offsets)[0] != 1):
+    o, a, m, b = _vector(offsets), _matrix(x), _matrices(w), _matrix(y)
+    if o is None or a is None or m is None or b is None or x.dtype != w.dtype or y.dtype != w.dtype or a[0] != b[0] or not _i32s(offsets) \
+            or o[:2] != (m[0] + 1, 1) or (a[1], b[1]) != ((m[2], m[1]) if operation == TRANSPOSE else (m[1], m[2])):
         return capi.INVALID_VALUE
-    if (x.shape[1], y.shape[1]) != ((w.shape[2], w.shape[1]) if operation == TRANSPOSE else (w.shape[1], w.shape[2])):
-        return capi.INVALID_VALUE
-    return capi.load().alphasparse_cuda_expert_mm(operation, _type(w), w.shape[0], x.shape[0], _ptr(offsets), w.shape[1], w.shape[2], _ptr(x), ldx,
-                                                  _ptr(w), lw[1], lw[0], _ptr(y), ldy)
+    return capi.load().alphasparse_cuda_expert_mm(operation, _kind(w)[0], m[0], a[0], o[2], m[1], m[2], a[3], a[2], m[5], m[3], m[4], b[3], b[2])
 
 
 def expert_mm_grad(offsets, dy, x, beta, dw):
     """alphasparse_cuda_expert_mm_grad: dw[e] = dy[rows of e]^T x[rows of e] + beta * dw[e].  Returns the status."""
-    ldx, lddy, lw = _rows(x), _rows(dy), _rows(dw, 3)
-    if None in (ldx, lddy, lw) or x.dtype != dy.dtype or x.shape[0] != dy.shape[0] or tuple(dw.shape[1:]) != (dy.shape[1], x.shape[1]) \
-            or not _is(offsets, "int32") or tuple(offsets.shape) != (dw.shape[0] + 1,) or (offsets.shape[0] > 1 and _strides(offsets)[0] != 1):
+    o, d, a, m = _vector(offsets), _matrix(dy), _matrix(x), _matrices(dw)
+    if o is None or d is None or a is None or m is None or x.dtype != dy.dtype or d[0] != a[0] or m[1:3] != (d[1], a[1]) or not _i32s(offsets) \
+            or o[:2] != (m[0] + 1, 1):
         return capi.INVALID_VALUE
-    return capi.load().alphasparse_cuda_expert_mm_grad(_type(x), _type(dw), dw.shape[0], x.shape[0], _ptr(offsets), dw.shape[1], dw.shape[2],
-                                                       _ptr(dy), lddy, _ptr(x), ldx, beta, _ptr(dw), lw[1], lw[0])
+    return capi.load().alphasparse_cuda_expert_mm_grad(_kind(x)[0], _kind(dw)[0], m[0], a[0], o[2], m[1], m[2], d[3], d[2], a[3], a[2], beta, m[5],
+                                                       m[3], m[4])
 
 
 def expert_mm_status(clear=False):
