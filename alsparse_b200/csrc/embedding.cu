@@ -356,7 +356,7 @@ extern "C" alphasparse_status_t alphasparse_cuda_embedding(alphasparse_cuda_inde
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     const int vb = vector_bytes(eb, {address(table), (uint64_t)ldt * eb, address(y), (uint64_t)ldy * eb, (uint64_t)width * eb});
     const int64_t nv = width * (int64_t)eb / vb;
-    const RowShape shape = row_shape(tokens, nv);
+    const RowShape shape = row_shape(tokens, nv, in_flight(vb));
     cudaStream_t st = current_stream();
     const auto run = [&](auto t) {
         using T = decltype(t);
@@ -364,7 +364,7 @@ extern "C" alphasparse_status_t alphasparse_cuda_embedding(alphasparse_cuda_inde
             using I = decltype(i);
             with_pack<T>(vb, [&](auto n) {
                 constexpr int N = decltype(n)::value;
-                const auto kernel = shape.unroll == 1 ? embedding_kernel<T, I, N, 1> : embedding_kernel<T, I, N, 4>;
+                const auto kernel = shape.unroll == 1 ? embedding_kernel<T, I, N, 1> : embedding_kernel<T, I, N, in_flight(N * sizeof(T))>;
                 kernel<<<shape.grid, kRowThreads, 0, st>>>((int)tokens, (const I *)token, inctoken, vocab, (int)nv, scale,
                                                          (const T *)table, ldt, (T *)y, ldy, shape.log);
             });

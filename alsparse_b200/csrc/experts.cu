@@ -172,10 +172,14 @@ __global__ void __launch_bounds__(kRowThreads)
 
 // ---- combine ---------------------------------------------------------------------------------------
 
-// out[t] = sum over j of weight[t, j] y[slot[t, j]] + beta out[t], in 32 bits in the order of j, rounded once.  Four rows of y
-// are requested at a time.
+// out[t] = sum over j of weight[t, j] y[slot[t, j]] + beta out[t], in 32 bits in the order of j, rounded once.  Eight rows of y
+// are requested at a time, 16 bytes of each by a thread: 128 bytes in flight at 64 registers.  (12,001 tokens of 6 rows of 2048
+// fp16: four rows of 64 bytes at 138 registers, one block per SM, 94 us; so COMBINE_US us.)
+constexpr __host__ __device__ int combine_unroll(int bytes) { return bytes >= 16 ? 1 : bytes >= 8 ? 2 : bytes >= 4 ? 4 : 8; }
+constexpr int kCombineAhead = 8;
+
 template <typename T, int N, int U>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 4)
     combine_kernel(int tokens, int k, int nv, const T *__restrict__ y, int64_t ldy, int64_t rows, const int *__restrict__ slot,
                    int64_t lds, const float *__restrict__ weight, int64_t ldw, float beta, T *__restrict__ out, int64_t ldo,
                    int log) {
@@ -183,22 +187,23 @@ __global__ void __launch_bounds__(kRowThreads)
     if (t >= tokens) return;
     const int v0 = (int)(blockIdx.y * (U << log) + (threadIdx.x & ((1 << log) - 1)));
     float acc[U][N] = {};
-    constexpr int kAhead = 4;
-    for (int j0 = 0; j0 < k; j0 += kAhead) {
-        Pack<T, N> p[kAhead][U];
-        int at[kAhead];
+    for (int j0 = 0; j0 < k; j0 += kCombineAhead) {
+        Pack<T, N> p[kCombineAhead][U];
+        int at[kCombineAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; j++) {
+        for (int j = 0; j < kCombineAhead; j++) {
             at[j] = j0 + j < k ? __ldg(slot + t * lds + j0 + j) : -1;
             if (at[j] >= rows) at[j] = -1;
+        }
+#pragma unroll
+        for (int j = 0; j < kCombineAhead; j++)
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int v = v0 + (u << log);
                 if (at[j] >= 0 && v < nv) p[j][u] = load_pack<T, N>(y + at[j] * ldy + (int64_t)v * N);
             }
-        }
 #pragma unroll
-        for (int j = 0; j < kAhead; j++) {
+        for (int j = 0; j < kCombineAhead; j++) {
             if (at[j] < 0) continue;
             const float w = weight ? __ldg(weight + t * ldw + j0 + j) : 1.f;
 #pragma unroll
@@ -221,65 +226,87 @@ __global__ void __launch_bounds__(kRowThreads)
 }
 
 // dy[slot[t, j]] = weight[t, j] dout[t] and dweight[t, j] = <dout[t], y[slot[t, j]]>.  A group of threads of one block has the
-// whole row of a token, so that the inner products end in it: lanes, then warps, in a fixed order.
+// whole row of a token, so that the inner products end in it: lanes, then warps, in a fixed order.  Eight rows at a time,
+// as above; their eight inner products are added up over a warp together, each step halving what a lane holds.
 template <typename T, int N>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 3)
     combine_grad_kernel(int tokens, int k, int nv, const T *__restrict__ dout, int64_t ldo, const T *__restrict__ y, int64_t ldy,
                         int64_t rows, const int *__restrict__ slot, int64_t lds, const float *__restrict__ weight, int64_t ldw,
                         T *__restrict__ dy, int64_t lddy, float *__restrict__ dweight, int64_t lddw, int log) {
-    __shared__ float s_dot[kRowThreads / 32][4];
+    __shared__ float s_dot[kRowThreads / 32][kCombineAhead];
     const int64_t t = (int64_t)blockIdx.x * (kRowThreads >> log) + (threadIdx.x >> log);
     const bool mine = t < tokens;  // a block's threads stay together for the barriers
-    const int group = 1 << log, me = threadIdx.x & (group - 1);
-    constexpr int kAtOnce = 4;
-    for (int j0 = 0; j0 < k; j0 += kAtOnce) {
-        int at[kAtOnce];
-        float w[kAtOnce], dot[kAtOnce] = {};
+    const int group = 1 << log, me = threadIdx.x & (group - 1), lane = threadIdx.x & 31;
+    constexpr int U = combine_unroll(N * sizeof(T));
+    for (int j0 = 0; j0 < k; j0 += kCombineAhead) {
+        int at[kCombineAhead];
+        float dot[kCombineAhead] = {};
 #pragma unroll
-        for (int j = 0; j < kAtOnce; j++) {
+        for (int j = 0; j < kCombineAhead; j++) {
             at[j] = mine && j0 + j < k ? __ldg(slot + t * lds + j0 + j) : -1;
             if (at[j] >= rows) at[j] = -1;
-            w[j] = at[j] >= 0 && weight ? __ldg(weight + t * ldw + j0 + j) : 1.f;
         }
-        for (int v = me; mine && v < nv; v += group) {
-            const Pack<T, N> d = load_pack<T, N>(dout + t * ldo + (int64_t)v * N);
-            Pack<T, N> p[kAtOnce];
+        for (int v0 = me; mine && v0 < nv; v0 += group * U) {
+            Pack<T, N> d[U], p[kCombineAhead][U];
 #pragma unroll
-            for (int j = 0; j < kAtOnce; j++)
-                if (at[j] >= 0) p[j] = load_pack<T, N>(y + at[j] * ldy + (int64_t)v * N);
+            for (int u = 0; u < U; u++)
+                if (v0 + u * group < nv) d[u] = load_pack<T, N>(dout + t * ldo + (int64_t)(v0 + u * group) * N);
 #pragma unroll
-            for (int j = 0; j < kAtOnce; j++) {
+            for (int j = 0; j < kCombineAhead; j++)
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (at[j] >= 0 && v0 + u * group < nv) p[j][u] = load_pack<T, N>(y + at[j] * ldy + (int64_t)(v0 + u * group) * N);
+#pragma unroll
+            for (int j = 0; j < kCombineAhead; j++) {
                 if (at[j] < 0) continue;
-                Pack<T, N> o;
+                const float w = weight ? __ldg(weight + t * ldw + j0 + j) : 1.f;
 #pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const float f = to_float(d.v[i]);
-                    dot[j] = fmaf(f, to_float(p[j].v[i]), dot[j]);
-                    o.v[i] = from_float<T>(w[j] * f);
+                for (int u = 0; u < U; u++) {
+                    if (v0 + u * group >= nv) continue;
+                    Pack<T, N> o;
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const float f = to_float(d[u].v[i]);
+                        dot[j] = fmaf(f, to_float(p[j][u].v[i]), dot[j]);
+                        o.v[i] = from_float<T>(w * f);
+                    }
+                    store_pack<T, N>(dy + at[j] * lddy + (int64_t)(v0 + u * group) * N, o);
                 }
-                store_pack<T, N>(dy + at[j] * lddy + (int64_t)v * N, o);
             }
         }
+        if (group < 32) {
 #pragma unroll
-        for (int j = 0; j < kAtOnce; j++)
-            for (int o = min(16, group >> 1); o; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
-        if (group > 32) {
-            if ((threadIdx.x & 31) == 0)
+            for (int j = 0; j < kCombineAhead; j++)
+                for (int o = group >> 1; o; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+            if (me == 0 && mine)
 #pragma unroll
-                for (int j = 0; j < kAtOnce; j++) s_dot[threadIdx.x >> 5][j] = dot[j];
-            __syncthreads();
-            if (me == 0)
-#pragma unroll
-                for (int j = 0; j < kAtOnce; j++) {
-                    dot[j] = 0.f;
-                    for (int i = 0; i < group / 32; i++) dot[j] += s_dot[(threadIdx.x >> 5) + i][j];
-                }
-            __syncthreads();
+                for (int j = 0; j < kCombineAhead; j++)
+                    if (j0 + j < k) dweight[t * lddw + j0 + j] = at[j] >= 0 ? dot[j] : 0.f;
+            continue;
         }
-        if (me == 0 && mine)
+        float half[4], quarter[2], one;
 #pragma unroll
-            for (int j = 0; j < kAtOnce; j++)
-                if (j0 + j < k) dweight[t * lddw + j0 + j] = at[j] >= 0 ? dot[j] : 0.f;
+        for (int j = 0; j < 4; j++) {
+            const float other = __shfl_xor_sync(0xffffffffu, lane & 16 ? dot[j] : dot[j + 4], 16);
+            half[j] = (lane & 16 ? dot[j + 4] : dot[j]) + other;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const float other = __shfl_xor_sync(0xffffffffu, lane & 8 ? half[j] : half[j + 2], 8);
+            quarter[j] = (lane & 8 ? half[j + 2] : half[j]) + other;
+        }
+        one = (lane & 4 ? quarter[1] : quarter[0]) + __shfl_xor_sync(0xffffffffu, lane & 4 ? quarter[0] : quarter[1], 4);
+        one += __shfl_xor_sync(0xffffffffu, one, 2);
+        one += __shfl_xor_sync(0xffffffffu, one, 1);
+        // lanes 4 i to 4 i + 3 hold the warp's sum of product i
+        if ((lane & 3) == 0) s_dot[threadIdx.x >> 5][lane >> 2] = one;
+        __syncthreads();
+        if (me < kCombineAhead && mine && j0 + me < k) {
+            float sum = 0.f;
+            for (int i = 0; i < group / 32; i++) sum += s_dot[(threadIdx.x >> 5) + i][me];
+            dweight[t * lddw + j0 + me] = sum;  // 0 for an empty slot: nothing was added
+        }
+        __syncthreads();
     }
 }
 
@@ -346,13 +373,13 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_dispatch(alphasparse_cud
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     const int vb = vector_bytes(eb, {address(x), (uint64_t)ldx * eb, address(xs), (uint64_t)ldxs * eb, (uint64_t)width * eb});
     const int64_t nv = width * (int64_t)eb / vb;
-    const RowShape shape = row_shape(tokens, nv);
+    const RowShape shape = row_shape(tokens, nv, in_flight(vb));
     cudaStream_t st = current_stream();
     const auto run = [&](auto t) {
         using T = decltype(t);
         with_pack<T>(vb, [&](auto n) {
             constexpr int N = decltype(n)::value;
-            const auto kernel = shape.unroll == 1 ? dispatch_kernel<T, N, 1> : dispatch_kernel<T, N, 4>;
+            const auto kernel = shape.unroll == 1 ? dispatch_kernel<T, N, 1> : dispatch_kernel<T, N, in_flight(N * sizeof(T))>;
             kernel<<<shape.grid, kRowThreads, 0, st>>>((int)tokens, (int)k, (int)nv, (const T *)x, ldx, slot, lds, rows, (T *)xs, ldxs, shape.log);
         });
     };
@@ -376,13 +403,13 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_combine(alphasparse_cuda
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     const int vb = vector_bytes(eb, {address(y), (uint64_t)ldy * eb, address(out), (uint64_t)ldo * eb, (uint64_t)width * eb});
     const int64_t nv = width * (int64_t)eb / vb;
-    RowShape shape = row_shape(tokens, nv);
+    const RowShape shape = row_shape(tokens, nv, combine_unroll(vb));
     cudaStream_t st = current_stream();
     const auto run = [&](auto t) {
         using T = decltype(t);
         with_pack<T>(vb, [&](auto n) {
             constexpr int N = decltype(n)::value;
-            const auto kernel = shape.unroll == 1 ? combine_kernel<T, N, 1> : combine_kernel<T, N, 4>;
+            const auto kernel = shape.unroll == 1 ? combine_kernel<T, N, 1> : combine_kernel<T, N, combine_unroll(N * sizeof(T))>;
             kernel<<<shape.grid, kRowThreads, 0, st>>>((int)tokens, (int)k, (int)nv, (const T *)y, ldy, rows, slot, lds, weight, ldw, beta, (T *)out, ldo, shape.log);
         });
     };

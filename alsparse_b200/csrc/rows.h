@@ -120,16 +120,20 @@ void with_pack(int vb, F f) {
 
 inline uint64_t address(const void *p) { return (uint64_t)reinterpret_cast<uintptr_t>(p); }
 
+// Vectors of `bytes` bytes that a thread has in flight: 64 bytes of them.  (16,383 rows of 1001 floats, 4-byte vectors: four
+// take 28.6 us, sixteen LOOKUP_RAGGED us.)
+constexpr __host__ __device__ int in_flight(int bytes) { return bytes >= 16 ? 4 : bytes >= 8 ? 8 : 16; }
+
 // A row of `nv` vectors by a group of 2^log threads, `unroll` vectors a thread and piece of the row.  Few vectors in all:
-// one a thread, so that the call is done in one round trip to memory; many: four, so that enough are in flight.
+// one a thread, so that the call is done in one round trip to memory; many: `many`, so that enough are in flight.
 struct RowShape {
     int log, unroll;
     dim3 grid;
 };
 constexpr int kRowThreads = 256;
-inline RowShape row_shape(int64_t rows, int64_t nv) {
+inline RowShape row_shape(int64_t rows, int64_t nv, int many) {
     RowShape s;
-    s.unroll = rows * nv <= 148 * 2048 ? 1 : 4;
+    s.unroll = rows * nv <= 148 * 2048 ? 1 : many;
     s.log = 0;
     while ((1 << s.log) < kRowThreads && (int64_t)s.unroll << s.log < nv) s.log++;
     const int64_t per_block = kRowThreads >> s.log, piece = (int64_t)s.unroll << s.log;
