@@ -50,7 +50,8 @@ __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 
 struct RouteShape {
     int experts, k, groups, top_groups, group_size;
-    bool sigmoid, renorm;
+    int group_lanes;  // lanes that hold a group, where every group fills a power of two of them; else 0
+    bool sigmoid, renorm, packs;
     float scale;
 };
 
@@ -69,8 +70,69 @@ __device__ __forceinline__ void softmax_stats(const float (&x)[I], F *top, F *su
     *top = m, *sum = warp_sum(s);
 }
 
-// Experts of one token by keys of type F, in a warp; lane j gets the j-th choice, -1 where nothing is left.  Lane l holds
-// the logits of experts l, l + 32, ...  Returns false when 32-bit keys do not decide it.
+// Elements in one access of a lane's I logits
+template <typename T, int I>
+constexpr __host__ __device__ int route_pack() {
+    int p = 1;
+    while (p * 2 * (int)sizeof(T) <= 16 && I % (p * 2) == 0) p *= 2;
+    return p;
+}
+
+// Lane l takes the logits of experts l I, ..., l I + I - 1; minus infinity behind the last expert
+template <typename T, int I>
+__device__ __forceinline__ void load_logits(const T *row, int experts, bool packs, float (&x)[I]) {
+    const int first = (threadIdx.x & 31) * I;
+    constexpr int P = route_pack<T, I>();
+    if (packs && first + I <= experts) {
+#pragma unroll
+        for (int i = 0; i < I; i += P) {
+            const Pack<T, P> p = load_pack<T, P>(row + first + i);
+#pragma unroll
+            for (int j = 0; j < P; j++) x[i + j] = to_float(p.v[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < I; i++) x[i] = first + i < experts ? to_float(row[first + i]) : -INFINITY;
+    }
+}
+
+// The best runs, for lane g < groups: whether run g is among the top_groups, from the values and orders that the lanes of the
+// groups read out of shared memory (one padding element per group).  Returns the mask of the runs; *value and *rank: this
+// lane's run.
+template <typename F, bool BIAS>
+__device__ __forceinline__ unsigned best_groups(const RouteShape &sh, const F *s_key, F *value, int *rank) {
+    using O = decltype(order_of(F(0)));
+    const int lane = threadIdx.x & 31;
+    O worth = 0;
+    *value = -INFINITY;
+    if (lane < sh.groups) {
+        O first = 0, second = 0;
+        F v1 = -INFINITY, v2 = -INFINITY;
+        const F *mine = s_key + lane * (sh.group_size + 1);
+        for (int i = 0; i < sh.group_size; i++) {
+            const F v = mine[i];
+            const O o = order_of(v);
+            if (o > first) second = first, v2 = v1, first = o, v1 = v;
+            else if (o > second) second = o, v2 = v;
+        }
+        *value = BIAS && second != 0 ? v1 + v2 : v1;
+        worth = first == 0 ? 0 : order_of(*value);
+    }
+    int ahead = 0;
+    for (int g = 0; g < sh.groups; g++) {
+        const O w = __shfl_sync(kAll, worth, g);
+        ahead += w > worth || (w == worth && g < lane);
+    }
+    *rank = lane < sh.groups ? ahead : sh.groups;
+    return __ballot_sync(kAll, lane < sh.groups && ahead < sh.top_groups);
+}
+
+// Keys of 32 bits are off by a few units in the last place of a score (at most 1; exp and quotient are the fast ones, within
+// some eight units of it in all) and of the sum with the bias: two that are further apart than this stand as they do in 64.
+__device__ __forceinline__ bool apart(float a, float b) { return a - b > 4e-6f * (1.f + fabsf(b)); }
+
+// Experts of one token by keys of type F, in a warp; lane j gets the j-th choice, -1 where nothing is left.  The plain way: the
+// largest key that is left, k times.  Returns false when 32-bit keys do not decide it.
 template <typename F, int I, bool BIAS>
 __device__ __forceinline__ bool choose(const RouteShape &sh, const float (&x)[I], const float *bias, F top, F sum,
                                        F *s_key, int *choice) {
@@ -78,53 +140,35 @@ __device__ __forceinline__ bool choose(const RouteShape &sh, const float (&x)[I]
     constexpr bool check = BIAS && sizeof(F) == 4;
     const int lane = threadIdx.x & 31;
     O key[I];
+    int group = lane * I / sh.group_size, within = lane * I - group * sh.group_size;
+    const int group0 = group, within0 = within;
 #pragma unroll
     for (int i = 0; i < I; i++) {
-        const int e = i * 32 + lane;
+        const int e = lane * I + i;
         F v = (F)x[i];
         if (BIAS && e < sh.experts && x[i] != -INFINITY)
             v = (sh.sigmoid ? (F)1 / ((F)1 + exp_of(-v)) : exp_of(v - top) / sum) + (F)__ldg(bias + e);
         key[i] = e < sh.experts ? order_of(v) : 0;
         // the values themselves go through shared memory to the lanes of the groups
-        if (sh.groups > 1 && e < sh.experts) s_key[e + e / sh.group_size] = v;
+        if (sh.groups > 1 && e < sh.experts) s_key[e + group] = v;
+        if (++within == sh.group_size) within = 0, group++;
     }
-    // keys of 32 bits are off by a few units in the last place of a score (at most 1) and of the sum with the bias
-    const float near = 4e-6f;
     if (sh.groups > 1) {
         __syncwarp();
-        O worth = 0;
-        F value = -INFINITY;
-        if (lane < sh.groups) {
-            O first = 0, second = 0;
-            F v1 = -INFINITY, v2 = -INFINITY;
-            const F *mine = s_key + lane * (sh.group_size + 1);
-            for (int i = 0; i < sh.group_size; i++) {
-                const F v = mine[i];
-                const O o = order_of(v);
-                if (o > first) second = first, v2 = v1, first = o, v1 = v;
-                else if (o > second) second = o, v2 = v;
-            }
-            value = BIAS && second != 0 ? v1 + v2 : v1;
-            worth = first == 0 ? 0 : order_of(value);
-        }
-        int ahead = 0;
-        for (int g = 0; g < sh.groups; g++) {
-            const O w = __shfl_sync(kAll, worth, g);
-            ahead += w > worth || (w == worth && g < lane);
-        }
-        const bool kept = lane < sh.groups && ahead < sh.top_groups;
-        const unsigned mask = __ballot_sync(kAll, kept);
-        if (check && sh.top_groups < sh.groups) {
+        F value;
+        int rank;
+        const unsigned mask = best_groups<F, BIAS>(sh, s_key, &value, &rank);
+        if (check) {
             // the last group that is in and the first that is not
-            const unsigned in = __ballot_sync(kAll, lane < sh.groups && ahead == sh.top_groups - 1);
-            const unsigned out = __ballot_sync(kAll, lane < sh.groups && ahead == sh.top_groups);
+            const unsigned in = __ballot_sync(kAll, rank == sh.top_groups - 1), out = __ballot_sync(kAll, rank == sh.top_groups);
             const float a = (float)__shfl_sync(kAll, value, __ffs(in) - 1), b = (float)__shfl_sync(kAll, value, __ffs(out) - 1);
-            if (!(a - b > 2.f * near * (1.f + fabsf(a)) || b == -INFINITY)) return false;
+            if (!apart(.5f * a, .5f * b) && b != -INFINITY) return false;  // sums of two keys: twice as far off
         }
+        group = group0, within = within0;
 #pragma unroll
         for (int i = 0; i < I; i++) {
-            const int e = i * 32 + lane;
-            if (e < sh.experts && !(mask >> (e / sh.group_size) & 1u)) key[i] = 0;
+            if (!(mask >> (group & 31) & 1u)) key[i] = 0;
+            if (++within == sh.group_size) within = 0, group++;
         }
         __syncwarp();
     }
@@ -137,7 +181,7 @@ __device__ __forceinline__ bool choose(const RouteShape &sh, const float (&x)[I]
         const O w = warp_max(best);
         if (check) {
             const float v = key_of((unsigned)w);
-            if (j > 0 && w != 0 && !(before - v > near * (1.f + fabsf(v)))) return false;
+            if (j > 0 && w != 0 && !apart(before, v)) return false;
             before = v;
         }
         if (w == 0 || j == sh.k) break;
@@ -145,17 +189,140 @@ __device__ __forceinline__ bool choose(const RouteShape &sh, const float (&x)[I]
         if (best == w) {
 #pragma unroll
             for (int i = I - 1; i >= 0; i--)
-                if (key[i] == w) e = i * 32 + lane;
+                if (key[i] == w) e = lane * I + i;
         }
         e = (int)__reduce_min_sync(kAll, (unsigned)e);
         if (lane == j) *choice = e;
-        if ((e & 31) == lane) {
+        if (e >= lane * I && e < lane * I + I) {
             best = 0;
 #pragma unroll
             for (int i = 0; i < I; i++) {
-                if (e == i * 32 + lane) key[i] = 0;
+                if (e == lane * I + i) key[i] = 0;
                 best = key[i] > best ? key[i] : best;
             }
+        }
+    }
+    return true;
+}
+
+// The same in 64 bits, for the tokens that need it; out of line, so that it costs the others no registers
+template <typename T, int I>
+__device__ __noinline__ int choose_in_64(const RouteShape &sh, const T *row, const float *bias, double *s_key) {
+    float x[I];
+    load_logits<T, I>(row, sh.experts, sh.packs, x);
+    double top = 0, sum = 1;
+    if (!sh.sigmoid) softmax_stats<double, I>(x, &top, &sum);
+    int choice;
+    choose<double, I, true>(sh, x, bias, top, sum, s_key, &choice);
+    return choice;
+}
+
+// Sorts the lane's keys, highest first, by a merging network (Batcher's odd-even merge sort; comparisons that reach behind I
+// are left out, which sorts any I)
+template <int I>
+__device__ __forceinline__ void sort_keys(unsigned long long (&key)[I]) {
+#pragma unroll
+    for (int p = 1; p < I; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < I; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; i++)
+                    if (i + j + q < I && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const unsigned long long a = key[i + j], b = key[i + j + q];
+                        key[i + j] = a > b ? a : b;
+                        key[i + j + q] = a > b ? b : a;
+                    }
+}
+
+// 32-bit keys, up to eight a lane: each lane sorts its own (order above, the complement of the index below, so that equal
+// keys go by index), then the highest head is taken k times.  (256 experts in 8 groups, 8 of them, 32,768 tokens: the
+// plain way 104 us, so ROUTE_US us.)
+template <int I, bool BIAS>
+__device__ __forceinline__ bool choose_sorted(const RouteShape &sh, const float (&x)[I], const float *bias, float top, float sum,
+                                              float *s_key, int *choice) {
+    const int lane = threadIdx.x & 31;
+    const float over = 1.f / sum;
+    unsigned long long key[I];
+    unsigned order[I];
+    int group = 0, within = 0;
+    const bool through_memory = sh.groups > 1 && sh.group_lanes == 0;
+    if (through_memory) group = lane * I / sh.group_size, within = lane * I - group * sh.group_size;
+    const int group0 = group, within0 = within;
+#pragma unroll
+    for (int i = 0; i < I; i++) {
+        const int e = lane * I + i;
+        float v = x[i];
+        if (BIAS && e < sh.experts)
+            v = x[i] == -INFINITY ? x[i] : (sh.sigmoid ? __fdividef(1.f, 1.f + __expf(-v)) : __expf(v - top) * over) + __ldg(bias + e);
+        order[i] = order_of(v);
+        if (through_memory) {
+            if (e < sh.experts) s_key[e + group] = v;
+            if (++within == sh.group_size) within = 0, group++;
+        }
+    }
+    if (through_memory) {
+        __syncwarp();
+        float value;
+        int rank;
+        const unsigned mask = best_groups<float, BIAS>(sh, s_key, &value, &rank);
+        if (BIAS) {
+            const unsigned in = __ballot_sync(kAll, rank == sh.top_groups - 1), out = __ballot_sync(kAll, rank == sh.top_groups);
+            const float a = __shfl_sync(kAll, value, __ffs(in) - 1), b = __shfl_sync(kAll, value, __ffs(out) - 1);
+            if (!apart(.5f * a, .5f * b) && b != -INFINITY) return false;
+        }
+        group = group0, within = within0;
+#pragma unroll
+        for (int i = 0; i < I; i++) {
+            if (!(mask >> (group & 31) & 1u)) order[i] = 0;
+            if (++within == sh.group_size) within = 0, group++;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < I; i++) key[i] = (unsigned long long)order[i] << 32 | (0xffffffffu - (unsigned)(lane * I + i));
+    sort_keys<I>(key);
+    if (sh.groups > 1 && sh.group_lanes != 0) {
+        // the two highest of the run, by the lanes that hold it
+        unsigned first = (unsigned)(key[0] >> 32), second = I > 1 ? (unsigned)(key[I > 1 ? 1 : 0] >> 32) : 0u;
+        for (int o = 1; o < sh.group_lanes; o <<= 1) {
+            const unsigned f = __shfl_xor_sync(kAll, first, o), g = __shfl_xor_sync(kAll, second, o);
+            second = max(min(first, f), max(second, g));
+            first = max(first, f);
+        }
+        unsigned worth = first;
+        if (BIAS && first != 0) worth = order_of(key_of(first) + (second != 0 ? key_of(second) : 0.f));
+        const int mine = lane / sh.group_lanes;
+        int ahead = 0;
+        for (int g = 0; g < sh.groups; g++) {
+            const unsigned w = __shfl_sync(kAll, worth, g * sh.group_lanes);
+            ahead += w > worth || (w == worth && g < mine);
+        }
+        const bool there = mine < sh.groups, kept = there && ahead < sh.top_groups;
+        if (BIAS) {
+            const unsigned last = __reduce_min_sync(kAll, kept ? worth : 0xffffffffu), next = __reduce_max_sync(kAll, there && !kept ? worth : 0u);
+            if (next != 0 && !apart(.5f * key_of(last), .5f * key_of(next))) return false;
+        }
+        if (!kept) key[0] = 0;  // never taken, so none behind it is either
+    }
+    *choice = -1;
+    float before = INFINITY;
+    for (int j = 0; j < sh.k + (BIAS ? 1 : 0); j++) {
+        const unsigned head = (unsigned)(key[0] >> 32), w = __reduce_max_sync(kAll, head);
+        if (w == 0) break;
+        if (BIAS) {
+            const float v = key_of(w);
+            if (j > 0 && !apart(before, v)) return false;
+            before = v;
+            if (j == sh.k) break;
+        }
+        const int from = __ffs(__ballot_sync(kAll, head == w)) - 1;  // equal keys: the lowest lane has the lowest index
+        const unsigned e = 0xffffffffu - __shfl_sync(kAll, (unsigned)key[0], from);
+        if (lane == j) *choice = (int)e;
+        if (lane == from) {
+#pragma unroll
+            for (int i = 0; i + 1 < I; i++) key[i] = key[i + 1];
+            key[I - 1] = 0;
         }
     }
     return true;
@@ -193,16 +360,18 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
     double *s_key = s_space + (size_t)w * (sh.experts + sh.groups);
     const T *row = logits + t * ldl;
     float x[I];
-#pragma unroll
-    for (int i = 0; i < I; i++) x[i] = i * 32 + lane < sh.experts ? to_float(row[i * 32 + lane]) : -INFINITY;
+    load_logits<T, I>(row, sh.experts, sh.packs, x);
     float top = 0.f, sum = 1.f;
     if (!sh.sigmoid && (BIAS || !sh.renorm)) softmax_stats<float, I>(x, &top, &sum);
     int choice;
-    if (!choose<float, I, BIAS>(sh, x, bias, top, sum, reinterpret_cast<float *>(s_key), &choice)) {
-        __syncwarp();
-        double top64 = 0, sum64 = 1;
-        if (!sh.sigmoid) softmax_stats<double, I>(x, &top64, &sum64);
-        choose<double, I, BIAS>(sh, x, bias, top64, sum64, s_key, &choice);
+    bool decided;
+    if constexpr (I <= 8) decided = choose_sorted<I, BIAS>(sh, x, bias, top, sum, reinterpret_cast<float *>(s_key), &choice);
+    else decided = choose<float, I, BIAS>(sh, x, bias, top, sum, reinterpret_cast<float *>(s_key), &choice);
+    if constexpr (BIAS) {
+        if (!decided) {
+            __syncwarp();
+            choice = choose_in_64<T, I>(sh, row, bias, s_key);
+        }
     }
     const bool live = choice >= 0;
     const float v = live ? to_float(row[choice]) : 0.f;
@@ -272,10 +441,20 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
 // Calls f with the number of logits a lane holds
 template <typename F>
 static void with_items(int experts, F f) {
-    if (experts <= 64) f(std::integral_constant<int, 2>{});
-    else if (experts <= 128) f(std::integral_constant<int, 4>{});
-    else if (experts <= 256) f(std::integral_constant<int, 8>{});
-    else if (experts <= 512) f(std::integral_constant<int, 16>{});
+    const int each = (experts + 31) / 32;
+    switch (each) {
+        case 1: return f(std::integral_constant<int, 1>{});
+        case 2: return f(std::integral_constant<int, 2>{});
+        case 3: return f(std::integral_constant<int, 3>{});
+        case 4: return f(std::integral_constant<int, 4>{});
+        case 5: return f(std::integral_constant<int, 5>{});
+        case 6: return f(std::integral_constant<int, 6>{});
+        case 7: return f(std::integral_constant<int, 7>{});
+        case 8: return f(std::integral_constant<int, 8>{});
+    }
+    if (each <= 12) f(std::integral_constant<int, 12>{});
+    else if (each <= 16) f(std::integral_constant<int, 16>{});
+    else if (each <= 24) f(std::integral_constant<int, 24>{});
     else f(std::integral_constant<int, 32>{});
 }
 
@@ -308,8 +487,8 @@ extern "C" alphasparse_status_t alphasparse_cuda_route(alphasparse_cuda_score_t 
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     // one group, or all of them: no limit
     const bool limited = top_groups < groups;
-    const RouteShape sh{(int)experts, (int)k, limited ? (int)groups : 1, (int)top_groups, (int)(experts / groups),
-                        score == ALPHA_SPARSE_CUDA_SCORE_SIGMOID, renormalize != 0, scale};
+    RouteShape sh{(int)experts, (int)k, limited ? (int)groups : 1, (int)top_groups, (int)(experts / groups), 0,
+                  score == ALPHA_SPARSE_CUDA_SCORE_SIGMOID, renormalize != 0, false, scale};
     cudaStream_t st = current_stream();
     const unsigned blocks = (unsigned)((tokens + kRouteWarps - 1) / kRouteWarps);
     const size_t smem = limited ? sizeof(double) * kRouteWarps * (size_t)(sh.experts + sh.groups) : 0;
@@ -317,6 +496,10 @@ extern "C" alphasparse_status_t alphasparse_cuda_route(alphasparse_cuda_score_t 
         using T = decltype(t);
         with_items(sh.experts, [&](auto items) {
             constexpr int I = decltype(items)::value;
+            constexpr uint64_t pack = route_pack<T, I>() * sizeof(T);
+            sh.packs = address(logits) % pack == 0 && (uint64_t)ldl * sizeof(T) % pack == 0;
+            const int lanes = sh.group_size / I;
+            sh.group_lanes = sh.group_size % I == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
             const auto kernel = bias ? route_kernel<T, I, true> : route_kernel<T, I, false>;
             kernel<<<blocks, kRouteWarps * 32, smem, st>>>(sh, (int)tokens, (const T *)logits, ldl, bias, index, ldi, weight, ldw);
         });
@@ -341,7 +524,7 @@ extern "C" alphasparse_status_t alphasparse_cuda_route_grad(alphasparse_cuda_sco
                                                        {dweight, tokens, k, ldw, sizeof(float), false},
                                                        {dlogits, tokens, experts, ldd, eb, true}});
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
-    const RouteShape sh{(int)experts, (int)k, 1, 1, (int)experts, score == ALPHA_SPARSE_CUDA_SCORE_SIGMOID, renormalize != 0, scale};
+    const RouteShape sh{(int)experts, (int)k, 1, 1, (int)experts, 0, score == ALPHA_SPARSE_CUDA_SCORE_SIGMOID, renormalize != 0, false, scale};
     cudaStream_t st = current_stream();
     const unsigned blocks = (unsigned)((tokens + kRouteWarps - 1) / kRouteWarps);
     const size_t smem = sizeof(float) * kRouteWarps * (size_t)sh.experts;

@@ -53,6 +53,23 @@ def test_route(dtype, score, biased, tokens, experts, groups, top_groups, k):
         _check(score, logits, bias, groups, top_groups, renorm, 2.5, k)
 
 
+@pytest.mark.parametrize("experts,groups,top_groups", [(24, 1, 1), (40, 2, 1), (128, 4, 2), (160, 8, 4), (160, 5, 2), (192, 6, 2), (192, 32, 9), (220, 4, 1), (224, 7, 3), (250, 10, 4),
+                                                       (256, 32, 8), (256, 2, 1), (300, 4, 2), (384, 8, 4), (768, 12, 5), (1000, 8, 3), (1024, 4, 2)])
+def test_every_number_of_experts_a_lane(experts, groups, top_groups):
+    g = gen(experts)
+    for dtype in (torch.float32, torch.bfloat16):
+        logits = normal(g, 300, experts, by=1.5)
+        logits[torch.rand(300, experts, generator=g, device="cuda") < 0.1] = -math.inf
+        logits[7, : experts // 2] = 0.25
+        logits = logits.to(dtype)
+        # rows that begin on 16-byte boundaries, and rows that do not
+        for x in (logits, strided(logits, experts + 3, 1)[0]):
+            for score in (SIGMOID, SOFTMAX):
+                for bias in (None, normal(g, experts, by=0.2)):
+                    _check(score, x, bias, groups, top_groups, True, 1.0, 6)
+                    _check(score, x, bias, 1, 1, False, 1.0, 6)
+
+
 @pytest.mark.parametrize("score", [SIGMOID, SOFTMAX])
 @pytest.mark.parametrize("biased", [False, True])
 def test_ties_go_to_the_lowest_index(score, biased):
