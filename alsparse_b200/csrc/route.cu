@@ -5,6 +5,8 @@
 // The choice is the one that 64-bit arithmetic makes.  Without a bias a score grows with its logit, so logits are compared,
 // exactly.  With a bias the keys score + bias are formed in 32 bits first, and a token of which two keys that matter lie
 // closer together than 32 bits can tell apart is decided again in 64 (about one token in a hundred of unrelated keys).
+#include <algorithm>
+
 #include "rows.h"
 
 namespace asb {
@@ -15,10 +17,8 @@ constexpr unsigned kAll = 0xffffffffu;
 // Keys as unsigned numbers of the same order.  0 stands for an expert that cannot be chosen (a logit or key of minus
 // infinity, a group left out, one already chosen); a NaN comes before everything else; the two zeros are one.
 __device__ __forceinline__ unsigned order_of(float key) {
-    if (key == -INFINITY) return 0u;
-    if (key != key) return 0xffffffffu;
-    const unsigned b = __float_as_uint(key + 0.f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    const unsigned b = __float_as_uint(key + 0.f), o = b ^ (unsigned)((int)b >> 31 | 0x80000000);
+    return key > -INFINITY ? o : key == -INFINITY ? 0u : 0xffffffffu;
 }
 __device__ __forceinline__ unsigned long long order_of(double key) {
     if (key == -INFINITY) return 0ull;
@@ -51,8 +51,9 @@ __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 struct RouteShape {
     int experts, k, groups, top_groups, group_size;
     int group_lanes;  // lanes that hold a group, where every group fills a power of two of them; else 0
-    bool sigmoid, renorm, packs;
+    bool sigmoid, renorm, packs, bias_packs;
     float scale;
+    int space;  // doubles of shared memory a warp
 };
 
 // softmax over the experts that are not masked: largest logit and sum of the exponentials; NaN goes through
@@ -64,9 +65,10 @@ __device__ __forceinline__ void softmax_stats(const float (&x)[I], F *top, F *su
     for (int i = 0; i < I; i++) m = fmax(m, (F)x[i]), nan |= x[i] != x[i];
     m = warp_most(m);
     if (__any_sync(kAll, nan)) m = NAN;
+    if (m == -INFINITY) m = 0;  // every expert is masked: exp gives zeros
     F s = 0;
 #pragma unroll
-    for (int i = 0; i < I; i++) s += x[i] == -INFINITY ? (F)0 : exp_of((F)x[i] - m);
+    for (int i = 0; i < I; i++) s += exp_of((F)x[i] - m);
     *top = m, *sum = warp_sum(s);
 }
 
@@ -237,32 +239,38 @@ __device__ __forceinline__ void sort_keys(unsigned long long (&key)[I]) {
 }
 
 // 32-bit keys, up to eight a lane: each lane sorts its own (order above, the complement of the index below, so that equal
-// keys go by index), then the highest head is taken k times.  (256 experts in 8 groups, 8 of them, 32,768 tokens: the
-// plain way 104 us, so ROUTE_US us.)
+// keys go by index) and leaves them in shared memory; the highest head is taken k times, its lane reads its next.  Bound by
+// instructions.  (256 experts in 8 groups, 8 of them, 32,768 tokens: the plain way 104 us, sorted keys moved up in
+// registers 55 us, so ROUTE_US us.)
 template <int I, bool BIAS>
 __device__ __forceinline__ bool choose_sorted(const RouteShape &sh, const float (&x)[I], const float *bias, float top, float sum,
-                                              float *s_key, int *choice) {
+                                              double *s_space, int *choice, float *logit) {
     const int lane = threadIdx.x & 31;
     const float over = 1.f / sum;
-    unsigned long long key[I];
-    unsigned order[I];
-    int group = 0, within = 0;
-    const bool through_memory = sh.groups > 1 && sh.group_lanes == 0;
-    if (through_memory) group = lane * I / sh.group_size, within = lane * I - group * sh.group_size;
-    const int group0 = group, within0 = within;
+    float v[I];
+    if (BIAS) {
+        load_logits<float, I>(bias, sh.experts, sh.bias_packs, v);  // minus infinity behind the last expert
 #pragma unroll
-    for (int i = 0; i < I; i++) {
-        const int e = lane * I + i;
-        float v = x[i];
-        if (BIAS && e < sh.experts)
-            v = x[i] == -INFINITY ? x[i] : (sh.sigmoid ? __fdividef(1.f, 1.f + __expf(-v)) : __expf(v - top) * over) + __ldg(bias + e);
-        order[i] = order_of(v);
-        if (through_memory) {
-            if (e < sh.experts) s_key[e + group] = v;
+        for (int i = 0; i < I; i++) {
+            const float s = (sh.sigmoid ? __fdividef(1.f, 1.f + __expf(-x[i])) : __expf(x[i] - top) * over) + v[i];
+            v[i] = x[i] == -INFINITY ? -INFINITY : s;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < I; i++) v[i] = x[i];
+    }
+    unsigned order[I];
+#pragma unroll
+    for (int i = 0; i < I; i++) order[i] = order_of(v[i]);
+    if (sh.groups > 1 && sh.group_lanes == 0) {
+        float *s_key = reinterpret_cast<float *>(s_space);
+        int group = lane * I / sh.group_size, within = lane * I - group * sh.group_size;
+        const int group0 = group, within0 = within;
+#pragma unroll
+        for (int i = 0; i < I; i++) {
+            if (lane * I + i < sh.experts) s_key[lane * I + i + group] = v[i];
             if (++within == sh.group_size) within = 0, group++;
         }
-    }
-    if (through_memory) {
         __syncwarp();
         float value;
         int rank;
@@ -270,7 +278,7 @@ __device__ __forceinline__ bool choose_sorted(const RouteShape &sh, const float 
         if (BIAS) {
             const unsigned in = __ballot_sync(kAll, rank == sh.top_groups - 1), out = __ballot_sync(kAll, rank == sh.top_groups);
             const float a = __shfl_sync(kAll, value, __ffs(in) - 1), b = __shfl_sync(kAll, value, __ffs(out) - 1);
-            if (!apart(.5f * a, .5f * b) && b != -INFINITY) return false;
+            if (!apart(.5f * a, .5f * b) && b != -INFINITY) return false;  // sums of two keys: twice as far off
         }
         group = group0, within = within0;
 #pragma unroll
@@ -278,7 +286,9 @@ __device__ __forceinline__ bool choose_sorted(const RouteShape &sh, const float 
             if (!(mask >> (group & 31) & 1u)) order[i] = 0;
             if (++within == sh.group_size) within = 0, group++;
         }
+        __syncwarp();
     }
+    unsigned long long key[I];
 #pragma unroll
     for (int i = 0; i < I; i++) key[i] = (unsigned long long)order[i] << 32 | (0xffffffffu - (unsigned)(lane * I + i));
     sort_keys<I>(key);
@@ -291,7 +301,10 @@ __device__ __forceinline__ bool choose_sorted(const RouteShape &sh, const float 
             first = max(first, f);
         }
         unsigned worth = first;
-        if (BIAS && first != 0) worth = order_of(key_of(first) + (second != 0 ? key_of(second) : 0.f));
+        if (BIAS) {
+            worth = order_of(key_of(first) + (second != 0 ? key_of(second) : 0.f));
+            if (first == 0) worth = 0;
+        }
         const int mine = lane / sh.group_lanes;
         int ahead = 0;
         for (int g = 0; g < sh.groups; g++) {
@@ -305,26 +318,34 @@ __device__ __forceinline__ bool choose_sorted(const RouteShape &sh, const float 
         }
         if (!kept) key[0] = 0;  // never taken, so none behind it is either
     }
-    *choice = -1;
-    float before = INFINITY;
-    for (int j = 0; j < sh.k + (BIAS ? 1 : 0); j++) {
-        const unsigned head = (unsigned)(key[0] >> 32), w = __reduce_max_sync(kAll, head);
-        if (w == 0) break;
-        if (BIAS) {
-            const float v = key_of(w);
-            if (j > 0 && !apart(before, v)) return false;
-            before = v;
-            if (j == sh.k) break;
-        }
-        const int from = __ffs(__ballot_sync(kAll, head == w)) - 1;  // equal keys: the lowest lane has the lowest index
-        const unsigned e = 0xffffffffu - __shfl_sync(kAll, (unsigned)key[0], from);
-        if (lane == j) *choice = (int)e;
-        if (lane == from) {
+    unsigned long long *mine = reinterpret_cast<unsigned long long *>(s_space) + lane;
 #pragma unroll
-            for (int i = 0; i + 1 < I; i++) key[i] = key[i + 1];
-            key[I - 1] = 0;
+    for (int i = 1; i < I; i++) mine[32 * i] = key[i];
+    unsigned long long head = key[0];
+    int next = 1;
+    unsigned taken = 0, at = 0, last = 0;
+    for (int j = 0; j < sh.k + (BIAS ? 1 : 0); j++) {
+        const unsigned w = __reduce_max_sync(kAll, (unsigned)(head >> 32));
+        if (w == 0) break;
+        if (BIAS && j == sh.k) {
+            last = w;
+            break;
+        }
+        const int from = __ffs(__ballot_sync(kAll, (unsigned)(head >> 32) == w)) - 1;  // equal keys: the lowest lane has the lowest index
+        const unsigned e = __shfl_sync(kAll, (unsigned)head, from);
+        if (lane == j) taken = w, at = e;
+        if (lane == from) {
+            head = next < I ? mine[32 * next] : 0ull;
+            next++;
         }
     }
+    if (BIAS) {
+        // each choice against the one behind it, the last against the best that was left out
+        const unsigned other = __shfl_down_sync(kAll, taken, 1), behind = lane == sh.k - 1 ? last : other;
+        if (__any_sync(kAll, taken != 0 && behind != 0 && !apart(key_of(taken), key_of(behind)))) return false;
+    }
+    *choice = taken != 0 ? (int)(0xffffffffu - at) : -1;
+    if (!BIAS) *logit = key_of(taken);
     return true;
 }
 
@@ -333,9 +354,7 @@ __device__ __forceinline__ bool choose_sorted(const RouteShape &sh, const float 
 __device__ __forceinline__ float weight_of(const RouteShape &sh, float v, bool live, float top, float sum) {
     float s;
     if (sh.renorm) {
-        bool nan = live && v != v;
-        float m = warp_most(live ? v : -INFINITY);
-        if (__any_sync(kAll, nan)) m = NAN;
+        const float m = key_of(__reduce_max_sync(kAll, live ? order_of(v) : 0u));  // a NaN leads the order
         if (sh.sigmoid) s = m < 0.f ? expf(v - m) / (1.f + expf(v)) : 1.f / (1.f + expf(-v));
         else s = expf(v - m);
         s = live ? s : 0.f;
@@ -348,24 +367,26 @@ __device__ __forceinline__ float weight_of(const RouteShape &sh, float v, bool l
     return s;
 }
 
-// A warp per token.
+// A warp per token.  (Four tokens a warp one after the other, their weights formed together and the next token's logits
+// requested ahead, was no faster: fewer warps to hide the chain of dependent steps of each.)
 template <typename T, int I, bool BIAS>
-__global__ void __launch_bounds__(kRouteWarps * 32)
+__global__ void __launch_bounds__(kRouteWarps * 32, I <= 8 ? 8 : 1)
     route_kernel(RouteShape sh, int tokens, const T *__restrict__ logits, int64_t ldl, const float *__restrict__ bias,
                  int *__restrict__ index, int64_t ldi, float *__restrict__ weight, int64_t ldw) {
     extern __shared__ double s_space[];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t t = (int64_t)blockIdx.x * kRouteWarps + w;
     if (t >= tokens) return;
-    double *s_key = s_space + (size_t)w * (sh.experts + sh.groups);
+    double *s_key = s_space + (size_t)w * sh.space;
     const T *row = logits + t * ldl;
     float x[I];
     load_logits<T, I>(row, sh.experts, sh.packs, x);
     float top = 0.f, sum = 1.f;
     if (!sh.sigmoid && (BIAS || !sh.renorm)) softmax_stats<float, I>(x, &top, &sum);
-    int choice;
+    int choice = -1;
+    float v = 0.f;  // the logit of the choice
     bool decided;
-    if constexpr (I <= 8) decided = choose_sorted<I, BIAS>(sh, x, bias, top, sum, reinterpret_cast<float *>(s_key), &choice);
+    if constexpr (I <= 8) decided = choose_sorted<I, BIAS>(sh, x, bias, top, sum, s_key, &choice, &v);
     else decided = choose<float, I, BIAS>(sh, x, bias, top, sum, reinterpret_cast<float *>(s_key), &choice);
     if constexpr (BIAS) {
         if (!decided) {
@@ -374,7 +395,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         }
     }
     const bool live = choice >= 0;
-    const float v = live ? to_float(row[choice]) : 0.f;
+    if ((BIAS || I > 8) && live) v = to_float(row[choice]);
     const float s = weight_of(sh, v, live, top, sum);
     if (lane < sh.k) {
         index[t * ldi + lane] = choice;
@@ -488,18 +509,19 @@ extern "C" alphasparse_status_t alphasparse_cuda_route(alphasparse_cuda_score_t 
     // one group, or all of them: no limit
     const bool limited = top_groups < groups;
     RouteShape sh{(int)experts, (int)k, limited ? (int)groups : 1, (int)top_groups, (int)(experts / groups), 0,
-                  score == ALPHA_SPARSE_CUDA_SCORE_SIGMOID, renormalize != 0, false, scale};
+                  score == ALPHA_SPARSE_CUDA_SCORE_SIGMOID, renormalize != 0, false, address(bias) % 16 == 0, scale, 0};
     cudaStream_t st = current_stream();
     const unsigned blocks = (unsigned)((tokens + kRouteWarps - 1) / kRouteWarps);
-    const size_t smem = limited ? sizeof(double) * kRouteWarps * (size_t)(sh.experts + sh.groups) : 0;
     const auto run = [&](auto t) {
         using T = decltype(t);
         with_items(sh.experts, [&](auto items) {
             constexpr int I = decltype(items)::value;
             constexpr uint64_t pack = route_pack<T, I>() * sizeof(T);
             sh.packs = address(logits) % pack == 0 && (uint64_t)ldl * sizeof(T) % pack == 0;
-            const int lanes = sh.group_size / I;
-            sh.group_lanes = sh.group_size % I == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+            const int across = sh.group_size / I;
+            sh.group_lanes = sh.group_size % I == 0 && (across & (across - 1)) == 0 ? across : 0;
+            sh.space = std::max(limited ? sh.experts + sh.groups : 0, I <= 8 ? 32 * I : 0);
+            const size_t smem = sizeof(double) * kRouteWarps * (size_t)sh.space;
             const auto kernel = bias ? route_kernel<T, I, true> : route_kernel<T, I, false>;
             kernel<<<blocks, kRouteWarps * 32, smem, st>>>(sh, (int)tokens, (const T *)logits, ldl, bias, index, ldi, weight, ldw);
         });
@@ -524,7 +546,7 @@ extern "C" alphasparse_status_t alphasparse_cuda_route_grad(alphasparse_cuda_sco
                                                        {dweight, tokens, k, ldw, sizeof(float), false},
                                                        {dlogits, tokens, experts, ldd, eb, true}});
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
-    const RouteShape sh{(int)experts, (int)k, 1, 1, (int)experts, 0, score == ALPHA_SPARSE_CUDA_SCORE_SIGMOID, renormalize != 0, false, scale};
+    const RouteShape sh{(int)experts, (int)k, 1, 1, (int)experts, 0, score == ALPHA_SPARSE_CUDA_SCORE_SIGMOID, renormalize != 0, false, false, scale, 0};
     cudaStream_t st = current_stream();
     const unsigned blocks = (unsigned)((tokens + kRouteWarps - 1) / kRouteWarps);
     const size_t smem = sizeof(float) * kRouteWarps * (size_t)sh.experts;
