@@ -1,9 +1,12 @@
 // Products of the experts: rows [offsets[e], offsets[e + 1]) of a dense block times the weights of expert e (a block-diagonal
 // matrix times a dense block), and the gradient of the weights.  No counterpart in the reference.
 //
-// expert_mm_kernel: tcgen05.mma with operands brought by TMA into a ring of stages, accumulators in TMEM, one persistent
-// block per SM.  One warp issues copies, one the products, four empty the accumulators; two accumulators, so that a tile is
-// written while the next is multiplied.  The offsets stay on the device: every block forms the same table of row tiles.
+// expert_mm_kernel: tcgen05.mma with operands brought by TMA into a ring of stages, accumulators in TMEM, persistent blocks,
+// one per SM.  One warp issues copies, one the products, four empty the accumulators; two accumulators, so that a tile is
+// written while the next is multiplied.  The rows of an expert are the narrow side of the tile: its width is any multiple
+// of 16, so an expert's rows are cut into equal tiles of at most 256 and little is multiplied for nothing.  With many rows
+// an expert two SMs work on one tile of 256 (cta_group::2), which halves what each fetches of the narrow operand.  The offsets
+// stay on the device: every block forms the same table of row tiles.
 // expert_mm_plain_kernel: 32-bit operands, and addresses or strides that TMA does not take (no multiple of 16 bytes).
 #include <cuda.h>
 #include <stdio.h>
@@ -19,9 +22,8 @@ static __device__ int g_expert_mm_status;
 
 // D[m, n] = sum over k of A[m, k] B[n, k].  What the three dimensions are:
 enum MmForm {
-    kRowsFirst,  // m: rows of an expert, n: its output features      (many rows an expert)
-    kRowsLast,   // m: output features, n: rows of an expert           (few rows an expert: no tile of 128 rows to fill)
-    kGradient    // m: columns of dy, n: columns of x, k: rows         (dW = dy^T x)
+    kRows,     // m: output features, n: rows of an expert, k: input features
+    kGradient  // m: columns of dy, n: columns of x, k: rows of an expert   (dW = dy^T x)
 };
 
 // First and last row of an expert, whatever the offsets hold
@@ -156,20 +158,36 @@ __device__ __forceinline__ void barrier_arrive(uint64_t *b) {
 __device__ __forceinline__ void barrier_expect(uint64_t *b, unsigned bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_address(b)), "r"(bytes) : "memory");
 }
+// True in one lane of a converged warp, always the same one.  The copies and products are issued under this and not under a
+// test of the lane's number: the compiler then keeps their operands in uniform registers (as it is, a product of
+// 128 x 32 x 16 was issued every 250 cycles under lane == 0).
+__device__ __forceinline__ bool elect_one() {
+    unsigned one;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
+}
 __device__ __forceinline__ unsigned long long now_ns() {
     unsigned long long t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-// Waits for the phase of the given parity; false when it ran out of time or another thread of the block did.
+// Waits for the phase of the given parity; false when it ran out of time or another thread of the block did.  CLUSTER: what the
+// pair's other block wrote before it arrived is seen (dear: about a microsecond).
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool barrier_wait(uint64_t *b, unsigned parity, volatile int *s_stop) {
     unsigned long long begin = 0;
     for (unsigned i = 0;; i++) {
         unsigned done;
-        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                     : "=r"(done)
-                     : "r"(smem_address(b)), "r"(parity)
-                     : "memory");
+        if constexpr (CLUSTER)
+            asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                         : "=r"(done)
+                         : "r"(smem_address(b)), "r"(parity)
+                         : "memory");
+        else
+            asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                         : "=r"(done)
+                         : "r"(smem_address(b)), "r"(parity)
+                         : "memory");
         if (done) return true;
         if ((i & 15) == 15) {
             if (*s_stop) return false;
@@ -183,14 +201,23 @@ __device__ __forceinline__ bool barrier_wait(uint64_t *b, unsigned parity, volat
     }
 }
 // ... by a whole warp, with one answer for all lanes
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_wait(uint64_t *b, unsigned parity, volatile int *s_stop) {
-    return __all_sync(0xffffffffu, barrier_wait(b, parity, s_stop));
+    return __all_sync(0xffffffffu, barrier_wait<CLUSTER>(b, parity, s_stop));
 }
-__device__ __forceinline__ void copy_tile(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *b) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-                     smem_address(dst)),
-                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_address(b))
-                 : "memory");
+// PAIR: `barrier` is an address of the cluster's, the other block's too
+template <bool PAIR>
+__device__ __forceinline__ void copy_tile(void *dst, const CUtensorMap *map, int x, int y, int z, unsigned barrier) {
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                         smem_address(dst)),
+                     "l"(map), "r"(x), "r"(y), "r"(z), "r"(barrier)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                         smem_address(dst)),
+                     "l"(map), "r"(x), "r"(y), "r"(z), "r"(barrier)
+                     : "memory");
 }
 // Shared-memory descriptor of an operand whose rows are 128 bytes, swizzled by 128 bytes.  K-major: rows of 64 k, groups of
 // eight rows 1024 bytes apart.  M/N-major: rows of 64 m (or n) per k, groups of eight k 1024 bytes apart, and the next 64 m
@@ -199,13 +226,41 @@ __device__ __forceinline__ uint64_t operand_descriptor(unsigned address, bool k_
     return (uint64_t)((address & 0x3ffff) >> 4) | (uint64_t)(k_major ? 1 : 8192 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
            (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
+template <bool PAIR>
 __device__ __forceinline__ void multiply(unsigned d, uint64_t a, uint64_t b, unsigned instruction, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
-                 "l"(b), "r"(instruction), "r"((unsigned)add)
-                 : "memory");
+    if constexpr (PAIR)
+        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+                     "l"(a), "l"(b), "r"(instruction), "r"((unsigned)add)
+                     : "memory");
+    else
+        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+                     "l"(a), "l"(b), "r"(instruction), "r"((unsigned)add)
+                     : "memory");
 }
+// An arrival on the barrier (PAIR: on that of both blocks) when the products issued so far are done
+template <bool PAIR>
 __device__ __forceinline__ void commit(uint64_t *b) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_address(b)) : "memory");
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_address(b)),
+                     "h"((unsigned short)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_address(b)) : "memory");
+}
+// The address, in the cluster's window, that `p` has in the pair's first block
+__device__ __forceinline__ unsigned address_in_first(const void *p) {
+    unsigned a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_address(p)));
+    return a;
+}
+// An arrival on the barrier of the pair's first block.  RELEASE: with what this thread wrote to memory before
+template <bool RELEASE>
+__device__ __forceinline__ void arrive_at_first(uint64_t *b) {
+    if constexpr (RELEASE) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(address_in_first(b)) : "memory");
+    else asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(address_in_first(b)) : "memory");
+}
+__device__ __forceinline__ void pair_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void load_accumulators(unsigned address, float (&v)[32]) {
     unsigned r[32];
@@ -227,181 +282,226 @@ struct MmShape {
     const int *offsets;
     int experts;
     int64_t rows;
-    int features;      // kRowsFirst / kRowsLast: columns of the output; kGradient: columns of dy (rows of an expert's output)
+    int features;      // kRows: columns of the output; kGradient: columns of dy
     int columns;       // kGradient: columns of x
-    int reduced;       // length of the sum (kGradient: the expert's rows)
-    int n, stages;     // tile of the second operand, depth of the ring
+    int reduced;       // kRows: length of the sum
+    int n, stages;     // widest tile, depth of the ring
     int feature_tiles, column_tiles;
-    unsigned b_bytes;  // shared memory of a stage's second operand
-    unsigned instruction, tmem, acc_stride;
+    unsigned stage_bytes, instruction, acc_stride;
     bool vectors;      // rows of the output begin on 16-byte boundaries
     float beta;
 };
 
 struct MmTile {
-    int expert, lo, hi, m0, n0, steps;
+    int expert, m0, n0, n;  // n0: first row (kRows) or column; n: width of the product, a multiple of 16 (two blocks: 32)
+    int lo, length;         // kGradient: the expert's first row, its rows; kRows: length = rows of the tile
+    int steps;
 };
 
-template <int FORM>
+template <int FORM, bool PAIR>
 __device__ __forceinline__ MmTile mm_tile(const MmShape &s, const int *s_first, int t) {
+    constexpr int M = PAIR ? 2 * kMmM : kMmM, unit = PAIR ? 32 : 16;
     MmTile q;
+    int hi;
     if (FORM == kGradient) {
         const int per = s.feature_tiles * s.column_tiles;
         q.expert = t / per;
         const int i = t - q.expert * per, f = i / s.column_tiles;
-        rows_of(s.offsets, q.expert, s.rows, &q.lo, &q.hi);
-        q.m0 = f * kMmM, q.n0 = (i - f * s.column_tiles) * s.n;
-        q.steps = (q.hi - q.lo + kMmK - 1) / kMmK;
+        rows_of(s.offsets, q.expert, s.rows, &q.lo, &hi);
+        q.m0 = f * M, q.n0 = (i - f * s.column_tiles) * s.n;
+        q.n = min(s.n, (s.columns - q.n0 + unit - 1) / unit * unit);
+        q.length = hi - q.lo;
+        q.steps = (q.length + kMmK - 1) / kMmK;
     } else {
         const int r = t / s.feature_tiles, f = t - r * s.feature_tiles;
         q.expert = expert_of(s_first, s.experts, r);
-        rows_of(s.offsets, q.expert, s.rows, &q.lo, &q.hi);
-        const int row_tile = r - s_first[q.expert];
-        q.lo += row_tile * (FORM == kRowsFirst ? kMmM : s.n);
-        q.m0 = FORM == kRowsFirst ? q.lo : f * kMmM;
-        q.n0 = FORM == kRowsFirst ? f * s.n : q.lo;
+        rows_of(s.offsets, q.expert, s.rows, &q.lo, &hi);
+        // equal shares of the expert's rows
+        const int tiles = s_first[q.expert + 1] - s_first[q.expert], share = ((hi - q.lo + tiles - 1) / tiles + unit - 1) / unit * unit;
+        q.n0 = q.lo + (r - s_first[q.expert]) * share;
+        q.length = min(share, hi - q.n0);
+        q.n = (q.length + unit - 1) / unit * unit;
+        q.m0 = f * M;
         q.steps = (s.reduced + kMmK - 1) / kMmK;
     }
     return q;
 }
 
-// W_K: consecutive sums of the weights are consecutive in memory (K-major), else consecutive features are
-template <int FORM, bool W_K, typename T, typename TO>
+// kGradient: step k ends within a group of 16 rows, the unit of the products
+__device__ __forceinline__ bool ragged(const MmTile &q, int k) { return q.length - k * kMmK < kMmK && (q.length & 15) != 0; }
+
+// W_K: consecutive terms of the sums are consecutive in memory (K-major weights), else consecutive features.  PAIR: two blocks
+// of a cluster on one tile: each fetches its 128 of the 256 m and its half of n, the first issues the products of both, the
+// accumulators of a block's 128 m are its own.  The copies of both report to the first block's barrier, but for the
+// last rows of an expert in kGradient: each block waits for its own and clears what does not belong to the expert, and the
+// second tells the first.
+template <int FORM, bool PAIR, bool W_K, typename T, typename TO>
 __global__ void __launch_bounds__(kMmThreads, 1)
-    expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MmShape s,
+    expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                     const __grid_constant__ CUtensorMap map_c, const MmShape s,
                      TO *__restrict__ out, int64_t ldo, int64_t stride_o) {
-    constexpr bool a_k = FORM == kRowsFirst || (FORM == kRowsLast && W_K), b_k = FORM == kRowsLast || (FORM == kRowsFirst && W_K);
+    constexpr bool a_k = FORM == kRows && W_K, b_k = FORM == kRows;
     constexpr unsigned a_bytes = kMmM * kMmK * sizeof(T);
     extern __shared__ __align__(16) char s_raw[];
     __shared__ int s_first[kMostExperts + 1];
-    __shared__ uint64_t s_full[kMmMostStages], s_empty[kMmMostStages], s_acc_full[2], s_acc_empty[2];
+    __shared__ uint64_t s_full[kMmMostStages], s_empty[kMmMostStages], s_own[kMmMostStages], s_ready[kMmMostStages], s_acc_full[2], s_acc_empty[2];
     __shared__ unsigned s_tmem;
     __shared__ int s_stop_word;
     volatile int *s_stop = &s_stop_word;
     char *ring = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
-    const unsigned stage_bytes = a_bytes + s.b_bytes;
-    float4 *staging = reinterpret_cast<float4 *>(ring + (size_t)s.stages * stage_bytes);  // 4 KB for each of four warps
-    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float4 *staging = reinterpret_cast<float4 *>(ring + (size_t)s.stages * s.stage_bytes);  // kGradient: 4 KB for each of four warps
+    const int w = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;  // clusters of two along x
+    const int worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
+    constexpr unsigned columns = 512;  // all of TMEM: one block per SM
 
     if (w == 0) {
         if (lane == 0) {
-            for (int i = 0; i < s.stages; i++) barrier_init(&s_full[i], 1), barrier_init(&s_empty[i], 1);
-            for (int i = 0; i < 2; i++) barrier_init(&s_acc_full[i], 1), barrier_init(&s_acc_empty[i], 4);
+            for (int i = 0; i < s.stages; i++) barrier_init(&s_full[i], 1), barrier_init(&s_empty[i], 1), barrier_init(&s_own[i], 1), barrier_init(&s_ready[i], 1);
+            for (int i = 0; i < 2; i++) barrier_init(&s_acc_full[i], 1), barrier_init(&s_acc_empty[i], PAIR ? 8 : 4);
             s_stop_word = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
     } else if (w == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(&s_tmem)), "r"(s.tmem) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    } else if (w == 2 && FORM != kGradient) {
-        count_row_tiles(s.offsets, s.experts, s.rows, FORM == kRowsFirst ? kMmM : s.n, s_first);
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(&s_tmem)), "r"(columns) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(&s_tmem)), "r"(columns) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
+    } else if (w == 2 && FORM == kRows) {
+        count_row_tiles(s.offsets, s.experts, s.rows, s.n, s_first);
     }
+    __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if constexpr (PAIR) pair_barrier();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = s_tmem;
     const int tiles = FORM == kGradient ? s.experts * s.feature_tiles * s.column_tiles : s_first[s.experts] * s.feature_tiles;
 
     if (w == 0) {
-        if (lane == 0) {
-            int stage = 0;
-            unsigned phase = 0;
-            bool good = true;
-            for (int t = blockIdx.x; good && t < tiles; t += gridDim.x) {
-                const MmTile q = mm_tile<FORM>(s, s_first, t);
-                for (int k = 0; k < q.steps; k++) {
-                    if (!(good = barrier_wait(&s_empty[stage], phase ^ 1, s_stop))) break;
-                    char *a = ring + (size_t)stage * stage_bytes, *b = a + a_bytes;
-                    uint64_t *full = &s_full[stage];
-                    barrier_expect(full, stage_bytes);
-                    const int k0 = k * kMmK;
-                    if (FORM == kGradient) {
-                        for (int g = 0; g < kMmM / 64; g++) copy_tile(a + g * 8192, &map_a, q.m0 + g * 64, q.lo + k0, 0, full);
-                        for (int g = 0; g < (int)(s.b_bytes >> 13); g++) copy_tile(b + g * 8192, &map_b, q.n0 + g * 64, q.lo + k0, 0, full);
-                    } else {
-                        if (a_k) copy_tile(a, &map_a, k0, q.m0, FORM == kRowsFirst ? 0 : q.expert, full);
-                        else
-                            for (int g = 0; g < kMmM / 64; g++) copy_tile(a + g * 8192, &map_a, q.m0 + g * 64, k0, q.expert, full);
-                        if (b_k) copy_tile(b, &map_b, k0, q.n0, FORM == kRowsLast ? 0 : q.expert, full);
-                        else
-                            for (int g = 0; g < (int)(s.b_bytes >> 13); g++) copy_tile(b + g * 8192, &map_b, q.n0 + g * 64, k0, q.expert, full);
-                    }
-                    if (++stage == s.stages) stage = 0, phase ^= 1;
-                }
-            }
-        }
-    } else if (w == 1) {
-        int stage = 0, count = 0;
+        int stage = 0;
         unsigned phase = 0;
         bool good = true;
-        for (int t = blockIdx.x; good && t < tiles; t += gridDim.x) {
-            const MmTile q = mm_tile<FORM>(s, s_first, t);
-            if (q.steps == 0) continue;
-            const int slot = count & 1;
-            if (!(good = warp_wait(&s_acc_empty[slot], ((count >> 1) & 1) ^ 1, s_stop))) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            count++;
-            const int length = FORM == kGradient ? q.hi - q.lo : s.reduced;
+        for (int t = worker; good && t < tiles; t += workers) {
+            const MmTile q = mm_tile<FORM, PAIR>(s, s_first, t);
+            const int half = PAIR ? q.n >> 1 : q.n, m0 = q.m0 + rank * kMmM, n0 = q.n0 + rank * half;
+            // kRows: boxes of 64 rows, then of 16; kGradient: boxes of 64 columns
+            const int wide = b_k ? half >> 6 : (half + 63) >> 6, narrow = b_k ? (half & 63) >> 4 : 0;
+            const unsigned bytes = a_bytes + (unsigned)wide * 8192u + (unsigned)narrow * 2048u;
             for (int k = 0; k < q.steps; k++) {
-                if (!(good = warp_wait(&s_full[stage], phase, s_stop))) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                char *a = ring + (size_t)stage * stage_bytes;
-                const int left = length - k * kMmK;
-                if (FORM == kGradient && left < kMmK) {
-                    // rows of the next expert (or behind the last) came along: zeros in both operands, so that nothing
-                    // that stands there, NaN included, gets into the sum
-                    const int per_box = (kMmK - left) * 8, boxes = (int)(stage_bytes >> 13);
-                    for (int i = lane; i < per_box * boxes; i += 32) {
-                        const int box = i / per_box;
-                        *reinterpret_cast<uint4 *>(a + (size_t)box * 8192 + left * 128 + (i - box * per_box) * 16) = make_uint4(0, 0, 0, 0);
+                if (!(good = warp_wait(&s_empty[stage], phase ^ 1, s_stop))) break;
+                char *a = ring + (size_t)stage * s.stage_bytes, *b = a + a_bytes;
+                const int k0 = k * kMmK;
+                const auto copy = [&](auto both, unsigned barrier) {
+                    constexpr bool B = decltype(both)::value;
+                    if (a_k) copy_tile<B>(a, &map_a, k0, m0, q.expert, barrier);
+                    else
+                        for (int g = 0; g < kMmM / 64; g++)
+                            copy_tile<B>(a + g * 8192, &map_a, m0 + g * 64, FORM == kGradient ? q.lo + k0 : k0, FORM == kGradient ? 0 : q.expert, barrier);
+                    for (int g = 0; g < wide; g++) {
+                        if (b_k) copy_tile<B>(b + g * 8192, &map_b, k0, n0 + g * 64, 0, barrier);
+                        else copy_tile<B>(b + g * 8192, &map_b, n0 + g * 64, q.lo + k0, 0, barrier);
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                }
-                if (lane == 0) {
-                    const uint64_t da = operand_descriptor(smem_address(a), a_k), db = operand_descriptor(smem_address(a + a_bytes), b_k);
-                    const int parts = min(4, (left + 15) / 16);
-                    for (int i = 0; i < parts; i++)
-                        multiply(tmem + slot * s.acc_stride, da + (uint64_t)(i * (a_k ? 32 : 2048) >> 4), db + (uint64_t)(i * (b_k ? 32 : 2048) >> 4),
-                                 s.instruction, k > 0 || i > 0);
-                    commit(&s_empty[stage]);
-                    if (k == q.steps - 1) commit(&s_acc_full[slot]);
+                    for (int g = 0; g < narrow; g++) copy_tile<B>(b + wide * 8192 + g * 2048, &map_c, k0, n0 + wide * 64 + g * 16, 0, barrier);
+                };
+                if (elect_one()) {
+                    if (PAIR && !(FORM == kGradient && ragged(q, k))) {
+                        if (rank == 0) barrier_expect(&s_full[stage], 2 * bytes);
+                        copy(std::true_type{}, address_in_first(&s_full[stage]));
+                    } else {
+                        uint64_t *barrier = PAIR ? &s_own[stage] : &s_full[stage];
+                        barrier_expect(barrier, bytes);
+                        copy(std::false_type{}, smem_address(barrier));
+                    }
                 }
                 __syncwarp();
                 if (++stage == s.stages) stage = 0, phase ^= 1;
             }
         }
+    } else if (w == 1) {
+        int stage = 0, count = 0;
+        unsigned full_phases = 0, own_phases = 0;  // a bit for each stage: the phase that comes next
+        bool good = true;
+        for (int t = worker; good && t < tiles; t += workers) {
+            const MmTile q = mm_tile<FORM, PAIR>(s, s_first, t);
+            if (q.steps == 0) continue;
+            const int slot = count & 1;
+            if (rank == 0 && !(good = warp_wait(&s_acc_empty[slot], ((count >> 1) & 1) ^ 1, s_stop))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            count++;
+            const int length = FORM == kGradient ? q.length : s.reduced;
+            const unsigned instruction = s.instruction | (unsigned)(q.n >> 3) << 17;
+            for (int k = 0; k < q.steps; k++) {
+                char *a = ring + (size_t)stage * s.stage_bytes;
+                const int left = length - k * kMmK, parts = min(4, (left + 15) / 16);
+                if (FORM == kGradient && ragged(q, k)) {
+                    uint64_t *barrier = PAIR ? &s_own[stage] : &s_full[stage];
+                    if (!(good = warp_wait(barrier, (PAIR ? own_phases : full_phases) >> stage & 1, s_stop))) break;
+                    // rows of the next expert (or behind the last) came along: zeros in both operands up to the next
+                    // multiple of 16, so that nothing that stands there, NaN included, gets into the sum
+                    const int end = (parts * 16 - left) * 8, boxes = 2 + (((PAIR ? q.n >> 1 : q.n) + 63) >> 6);
+                    for (int box = 0; box < boxes; box++)
+                        for (int i = lane; i < end; i += 32)
+                            *reinterpret_cast<uint4 *>(a + (size_t)box * 8192 + left * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (PAIR) {
+                        if (rank == 1) {
+                            if (lane == 0) arrive_at_first<true>(&s_ready[stage]);
+                        } else if (!(good = warp_wait<true>(&s_ready[stage], own_phases >> stage & 1, s_stop))) break;
+                        own_phases ^= 1u << stage;
+                    } else full_phases ^= 1u << stage;
+                } else {
+                    if (rank == 0 && !(good = warp_wait(&s_full[stage], full_phases >> stage & 1, s_stop))) break;
+                    full_phases ^= 1u << stage;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (rank == 0 && elect_one()) {
+                    const uint64_t da = operand_descriptor(smem_address(a), a_k), db = operand_descriptor(smem_address(a + a_bytes), b_k);
+                    for (int i = 0; i < parts; i++)
+                        multiply<PAIR>(tmem + slot * s.acc_stride, da + (uint64_t)(i * (a_k ? 32 : 2048) >> 4),
+                                       db + (uint64_t)(i * (b_k ? 32 : 2048) >> 4), instruction, k > 0 || i > 0);
+                    commit<PAIR>(&s_empty[stage]);
+                    if (k == q.steps - 1) commit<PAIR>(&s_acc_full[slot]);
+                }
+                __syncwarp();
+                if (++stage == s.stages) stage = 0;
+            }
+        }
     } else {
         const int part = w & 3;  // the quarter of the accumulators' lanes that this warp may read
         int count = 0;
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-            const MmTile q = mm_tile<FORM>(s, s_first, t);
-            const int slot = count & 1;
+        for (int t = worker; t < tiles; t += workers) {
+            const MmTile q = mm_tile<FORM, PAIR>(s, s_first, t);
+            const int slot = count & 1, m0 = q.m0 + rank * kMmM;
             if (q.steps > 0) {
                 if (!warp_wait(&s_acc_full[slot], (count >> 1) & 1, s_stop)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 count++;
             }
             const unsigned from = tmem + slot * s.acc_stride + ((unsigned)(part * 32) << 16);
-            if (FORM == kRowsLast) {
+            if (FORM == kRows) {
                 // a lane is a feature, a column a row of the output: 32 consecutive features of a row at a time
-                const int f = q.m0 + part * 32 + lane, n = min(s.n, q.hi - q.lo);
-                for (int c = 0; c < n; c += 32) {
+                const int f = m0 + part * 32 + lane;
+                for (int c = 0; c < q.length; c += 32) {
                     float v[32];
                     load_accumulators(from + c, v);
+                    TO *dst = out + (int64_t)(q.n0 + c) * ldo + f;
 #pragma unroll
                     for (int i = 0; i < 32; i++)
-                        if (c + i < n && f < s.features) out[(int64_t)(q.lo + c + i) * ldo + f] = from_float<TO>(v[i]);
+                        if (c + i < q.length && f < s.features) dst[i * ldo] = from_float<TO>(v[i]);
                 }
             } else {
                 // a lane is a row of the output; 32 columns at a time pass through shared memory, so that rows are written
                 // in whole sectors by neighbouring lanes
                 float4 *mine = staging + part * 256;
-                TO *base = out + (FORM == kGradient ? q.expert * stride_o + (int64_t)q.m0 * ldo : (int64_t)q.m0 * ldo);
-                const int m_end = FORM == kGradient ? s.features - q.m0 : q.hi - q.lo;
-                const int n_end = min(s.n, (FORM == kGradient ? s.columns : s.features) - q.n0);
+                TO *base = out + q.expert * stride_o + (int64_t)m0 * ldo;
+                const int m_end = s.features - m0, n_end = min(q.n, s.columns - q.n0);
                 constexpr int E = 16 / sizeof(TO), across = 32 / E, down = 32 / across;
-                for (int c = 0; c < n_end; c += 32) {
+                for (int c = 0; c < n_end && m_end > 0; c += 32) {
                     float v[32];
                     if (q.steps > 0) load_accumulators(from + c, v);
                     else {
@@ -442,7 +542,10 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             if (q.steps > 0) {
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) barrier_arrive(&s_acc_empty[slot]);
+                if (lane == 0) {
+                    if (PAIR) arrive_at_first<false>(&s_acc_empty[slot]);
+                    else barrier_arrive(&s_acc_empty[slot]);
+                }
             }
         }
     }
@@ -458,9 +561,11 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         }
         __syncthreads();
     }
+    if constexpr (PAIR) pair_barrier();  // nothing reaches into the other block's memory after this
     if (w == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(s.tmem));
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
     }
 }
 
@@ -505,29 +610,37 @@ static cudaError_t multiprocessors(int *n) {
 }
 
 // Fills what follows from the tile, and launches.
-template <int FORM, bool W_K, typename T, typename TO>
-static cudaError_t launch_mm(alphasparse_cuda_type_t type, MmShape s, int64_t most_tiles, const CUtensorMap &a, const CUtensorMap &b, TO *out,
+template <int FORM, bool PAIR, bool W_K, typename T, typename TO>
+static cudaError_t launch_mm(alphasparse_cuda_type_t type, MmShape s, int64_t most_tiles, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &c,
+                             TO *out,
                              int64_t ldo, int64_t stride_o, cudaStream_t st) {
-    constexpr bool a_k = FORM == kRowsFirst || (FORM == kRowsLast && W_K), b_k = FORM == kRowsLast || (FORM == kRowsFirst && W_K);
-    constexpr int most_smem = 232448 - 8192, staging = 16384;  // the tables and barriers are in what is left
-    s.b_bytes = (unsigned)(b_k ? s.n * kMmK : (s.n + 63) / 64 * 64 * kMmK) * 2;
-    const unsigned stage = kMmM * kMmK * 2 + s.b_bytes;
-    s.stages = std::min<int>(kMmMostStages, (most_smem - 1024 - staging) / (int)stage);
+    constexpr bool a_k = FORM == kRows && W_K, b_k = FORM == kRows;
+    constexpr int most_smem = 232448 - 8192, staging = FORM == kGradient ? 16384 : 0;  // tables and barriers are in what is left
+    const int half = PAIR ? s.n / 2 : s.n;
+    s.stage_bytes = (unsigned)(kMmM * kMmK + (b_k ? half : (half + 63) / 64 * 64) * kMmK) * 2;
+    s.stages = std::min<int>(kMmMostStages, (most_smem - 1024 - staging) / (int)s.stage_bytes);
     const unsigned format = type == ALPHA_SPARSE_CUDA_TYPE_BF16 ? 1 : 0;
-    s.instruction = 1u << 4 | format << 7 | format << 10 | (a_k ? 0u : 1u << 15) | (b_k ? 0u : 1u << 16) | (unsigned)(s.n >> 3) << 17 |
-                    (unsigned)(kMmM >> 4) << 24;
-    s.acc_stride = 32;
-    while ((int)s.acc_stride < s.n) s.acc_stride *= 2;
-    s.tmem = 2 * s.acc_stride;
+    s.instruction = 1u << 4 | format << 7 | format << 10 | (a_k ? 0u : 1u << 15) | (b_k ? 0u : 1u << 16) |
+                    (unsigned)((PAIR ? 2 * kMmM : kMmM) >> 4) << 24;
+    s.acc_stride = 256;
     s.vectors = address(out) % 16 == 0 && ldo * (int64_t)sizeof(TO) % 16 == 0 && (FORM != kGradient || stride_o * (int64_t)sizeof(TO) % 16 == 0);
-    const auto kernel = expert_mm_kernel<FORM, W_K, T, TO>;
-    const int smem = 1024 + s.stages * (int)stage + staging;
+    const auto kernel = expert_mm_kernel<FORM, PAIR, W_K, T, TO>;
+    const int smem = 1024 + s.stages * (int)s.stage_bytes + staging;
     int sms = 0;
     cudaError_t e = multiprocessors(&sms);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    kernel<<<(unsigned)std::min<int64_t>(sms, most_tiles), kMmThreads, smem, st>>>(a, b, s, out, ldo, stride_o);
-    return cudaGetLastError();
+    cudaLaunchAttribute cluster[1];
+    cluster[0].id = cudaLaunchAttributeClusterDimension;
+    cluster[0].val.clusterDim.x = 2, cluster[0].val.clusterDim.y = 1, cluster[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(PAIR ? 2 * std::min<int64_t>(sms / 2, most_tiles) : std::min<int64_t>(sms, most_tiles)));
+    config.blockDim = dim3(kMmThreads);
+    config.dynamicSmemBytes = (size_t)smem;
+    config.stream = st;
+    config.attrs = cluster;
+    config.numAttrs = PAIR ? 1 : 0;
+    return cudaLaunchKernelEx(&config, kernel, a, b, c, s, out, ldo, stride_o);
 }
 
 static int64_t up_to(int64_t v, int64_t unit) { return (v + unit - 1) / unit * unit; }
@@ -577,33 +690,27 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_mm(alphasparse_operation
     if (eb == 2 && reduced > 0 && takes_tma(x, ldx, rows, 0, 1) && takes_tma(w, ldw, out, stride_w, experts)) {
         MmShape s{};
         s.offsets = offsets, s.experts = (int)experts, s.rows = rows, s.features = (int)features, s.reduced = (int)reduced;
-        // Few rows an expert: they make the narrow side of the tile.
+        // Many rows an expert: two SMs on a tile.  Few: the weights are what has to be read, by as many SMs as there are; narrow
+        // tiles leave room for more of them on their way.
         const int64_t mean = (rows + experts - 1) / experts;
-        const bool last = mean <= 64;
-        CUtensorMap mx, mw;
-        bool made;
-        if (last) {
-            s.n = mean <= 16 ? 32 : mean <= 32 ? 64 : 128;
-            s.feature_tiles = (int)((features + kMmM - 1) / kMmM);
-            made = make_map(&mx, type, x, reduced, rows, ldx, 1, 0, s.n) && make_map(&mw, type, w, in, out, ldw, experts, stride_w, trans ? kMmM : kMmK);
-        } else {
-            // equal tiles of at most 256 features
-            s.feature_tiles = (int)((features + 255) / 256);
-            s.n = (int)up_to((features + s.feature_tiles - 1) / s.feature_tiles, 16);
-            made = make_map(&mx, type, x, reduced, rows, ldx, 1, 0, kMmM) && make_map(&mw, type, w, in, out, ldw, experts, stride_w, trans ? s.n : kMmK);
-        }
-        if (!made) {
+        const bool pair = mean > 64;
+        s.n = pair ? 256 : mean <= 16 ? 32 : mean <= 32 ? 64 : 128;
+        const int m = pair ? 2 * kMmM : kMmM;
+        s.feature_tiles = (int)((features + m - 1) / m);
+        CUtensorMap mx, mx16, mw;
+        if (!make_map(&mx, type, x, reduced, rows, ldx, 1, 0, 64) || !make_map(&mx16, type, x, reduced, rows, ldx, 1, 0, 16) ||
+             !make_map(&mw, type, w, in, out, ldw, experts, stride_w, trans ? kMmM : kMmK)) {
             record_error("alphasparse_cuda_expert_mm: no tensor map");
             return ALPHA_SPARSE_STATUS_EXECUTION_FAILED;
         }
-        const int64_t row_tiles = rows / (last ? s.n : kMmM) + std::min(experts, rows), tiles = row_tiles * s.feature_tiles;
+        const int64_t row_tiles = rows / s.n + std::min(experts, rows), tiles = row_tiles * s.feature_tiles;
         if (tiles > 0x7fffffff - 4096) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
         const auto go = [&](auto t) {
             using T = decltype(t);
-            if (last && trans) e = launch_mm<kRowsLast, true, T, T>(type, s, tiles, mw, mx, (T *)y, ldy, 0, st);
-            else if (last) e = launch_mm<kRowsLast, false, T, T>(type, s, tiles, mw, mx, (T *)y, ldy, 0, st);
-            else if (trans) e = launch_mm<kRowsFirst, true, T, T>(type, s, tiles, mx, mw, (T *)y, ldy, 0, st);
-            else e = launch_mm<kRowsFirst, false, T, T>(type, s, tiles, mx, mw, (T *)y, ldy, 0, st);
+            if (pair && trans) e = launch_mm<kRows, true, true, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
+            else if (pair) e = launch_mm<kRows, true, false, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
+            else if (trans) e = launch_mm<kRows, false, true, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
+            else e = launch_mm<kRows, false, false, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
         };
         if (type == ALPHA_SPARSE_CUDA_TYPE_F16) go(__half());
         else go(__nv_bfloat16());
@@ -645,9 +752,9 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_mm_grad(alphasparse_cuda
     if (eb == 2 && rows > 0 && takes_tma(dy, lddy, rows, 0, 1) && takes_tma(x, ldx, rows, 0, 1)) {
         MmShape s{};
         s.offsets = offsets, s.experts = (int)experts, s.rows = rows, s.features = (int)out, s.columns = (int)in, s.beta = beta;
-        s.feature_tiles = (int)((out + kMmM - 1) / kMmM);
+        s.feature_tiles = (int)((out + 2 * kMmM - 1) / (2 * kMmM));
         s.column_tiles = (int)((in + 255) / 256);
-        s.n = (int)up_to((in + s.column_tiles - 1) / s.column_tiles, 16);
+        s.n = (int)up_to((in + s.column_tiles - 1) / s.column_tiles, 32);  // equal tiles of at most 256 columns
         CUtensorMap my, mx;
         if (!make_map(&my, type, dy, out, rows, lddy, 1, 0, kMmK) || !make_map(&mx, type, x, in, rows, ldx, 1, 0, kMmK)) {
             record_error("alphasparse_cuda_expert_mm_grad: no tensor map");
@@ -657,8 +764,8 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_mm_grad(alphasparse_cuda
         if (tiles > 0x7fffffff - 4096) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
         const auto go = [&](auto t) {
             using T = decltype(t);
-            if (weight_type == ALPHA_SPARSE_CUDA_TYPE_F32) e = launch_mm<kGradient, false, T, float>(type, s, tiles, my, mx, (float *)dw, ldw, stride_w, st);
-            else e = launch_mm<kGradient, false, T, T>(type, s, tiles, my, mx, (T *)dw, ldw, stride_w, st);
+            if (weight_type == ALPHA_SPARSE_CUDA_TYPE_F32) e = launch_mm<kGradient, true, false, T, float>(type, s, tiles, my, mx, mx, (float *)dw, ldw, stride_w, st);
+            else e = launch_mm<kGradient, true, false, T, T>(type, s, tiles, my, mx, mx, (T *)dw, ldw, stride_w, st);
         };
         if (type == ALPHA_SPARSE_CUDA_TYPE_F16) go(__half());
         else go(__nv_bfloat16());
