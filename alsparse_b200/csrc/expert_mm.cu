@@ -23,7 +23,7 @@ static __device__ int g_expert_mm_status;
 // D[m, n] = sum over k of A[m, k] B[n, k].  What the three dimensions are:
 enum MmForm {
     kRows,     // m: output features, n: rows of an expert, k: input features
-    kGradient  // m: columns of dy, n: columns of x, k: rows of an expert   (dW = dy^T x)
+    kGradient  // m: columns of x, n: columns of dy, k: rows of an expert   (dW^T = x^T dy)
 };
 
 // First and last row of an expert, whatever the offsets hold
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(256)
 
 // ---- tensor cores --------------------------------------------------------------------------------
 
-constexpr int kMmThreads = 192;  // copies, products, four warps for the accumulators
+constexpr int kMmThreads = 352;  // copies, products, eight warps for the accumulators, one for the ends of ragged experts
 constexpr int kMmM = 128, kMmK = 64;
 constexpr int kMmMostStages = 8;
 constexpr unsigned long long kMmLimitNs = 2000000000ull;
@@ -262,60 +262,131 @@ __device__ __forceinline__ void arrive_at_first(uint64_t *b) {
 __device__ __forceinline__ void pair_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void load_accumulators(unsigned address, float (&v)[32]) {
-    unsigned r[32];
+// Requests 32 columns of this warp's 32 lanes; they are there after wait_accumulators.
+__device__ __forceinline__ void request_accumulators(unsigned address, unsigned (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
-        "tcgen05.wait::ld.sync.aligned;"
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
           "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
           "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(address)
         : "memory");
+}
+// The registers are named so that no use of them is moved before the wait.
+__device__ __forceinline__ void wait_accumulators(unsigned (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                   "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                   "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+
+template <typename T> __device__ __forceinline__ unsigned pack_two(float a, float b);
+template <> __device__ __forceinline__ unsigned pack_two<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned *>(&v);
+}
+template <> __device__ __forceinline__ unsigned pack_two<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const unsigned *>(&v);
+}
+
+// A warp writes a block of 32 rows x 32 columns of the output: a lane has one column, its register i row i.  dst: row 0, the
+// warp's first column; `rows` and `cols` of them exist.  32-bit elements: a row is a line, as it is.  16-bit ones are
+// exchanged among eight lanes in three steps, until a lane has eight columns of four rows and writes 16 bytes at a time (a
+// store of two bytes a lane and row took 923 us where this takes MM_DX us: 32,768 rows of 8 experts, 4096 x 4096,
+// operation N).
+template <typename TO>
+__device__ __forceinline__ void write_block(const unsigned (&r)[32], TO *dst, int64_t ldo, int rows, int cols, bool vectors, float beta) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (sizeof(TO) == 2) {
+        if (vectors && beta == 0.f) {
+            unsigned p[16];
 #pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+            for (int i = 0; i < 16; i++) {
+                const unsigned own = pack_two<TO>(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+                const unsigned other = __shfl_xor_sync(0xffffffffu, own, 1);
+                p[i] = lane & 1 ? __byte_perm(other, own, 0x7632) : __byte_perm(own, other, 0x5410);
+            }
+            uint2 h[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const unsigned other = __shfl_xor_sync(0xffffffffu, lane & 2 ? p[2 * i] : p[2 * i + 1], 2);
+                h[i] = lane & 2 ? make_uint2(other, p[2 * i + 1]) : make_uint2(p[2 * i], other);
+            }
+            const int first = lane & ~7;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint2 give = lane & 4 ? h[2 * i] : h[2 * i + 1], keep = lane & 4 ? h[2 * i + 1] : h[2 * i];
+                const uint2 other = make_uint2(__shfl_xor_sync(0xffffffffu, give.x, 4), __shfl_xor_sync(0xffffffffu, give.y, 4));
+                const uint4 o = lane & 4 ? make_uint4(other.x, other.y, keep.x, keep.y) : make_uint4(keep.x, keep.y, other.x, other.y);
+                const int row = 8 * i + (lane & 7);
+                TO *to = dst + row * ldo + first;
+                if (row < rows) {
+                    if (first + 8 <= cols) *reinterpret_cast<uint4 *>(to) = o;
+                    else {
+                        const TO *e = reinterpret_cast<const TO *>(&o);
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (first + j < cols) to[j] = e[j];
+                    }
+                }
+            }
+            return;
+        }
+    }
+    if (lane >= cols) return;
+#pragma unroll
+    for (int i = 0; i < 32; i++)
+        if (i < rows) {
+            TO *to = dst + i * ldo + lane;
+            const float v = __uint_as_float(r[i]);
+            *to = from_float<TO>(beta != 0.f ? fmaf(beta, to_float(*to), v) : v);
+        }
 }
 
 struct MmShape {
     const int *offsets;
     int experts;
     int64_t rows;
-    int features;      // kRows: columns of the output; kGradient: columns of dy
-    int columns;       // kGradient: columns of x
+    int m_size;        // kRows: columns of the output (features); kGradient: columns of x
+    int n_size;        // kGradient: columns of dy
     int reduced;       // kRows: length of the sum
     int n, stages;     // widest tile, depth of the ring
-    int feature_tiles, column_tiles;
+    int m_tiles, n_tiles;
     unsigned stage_bytes, instruction, acc_stride;
     bool vectors;      // rows of the output begin on 16-byte boundaries
     float beta;
 };
 
 struct MmTile {
-    int expert, m0, n0, n;  // n0: first row (kRows) or column; n: width of the product, a multiple of 16 (two blocks: 32)
+    int expert, m0, n0, n;  // n0: first row (kRows) or column of dy; n: width of the product, a multiple of 16 (two blocks: 32)
     int lo, length;         // kGradient: the expert's first row, its rows; kRows: length = rows of the tile
     int steps;
 };
 
 template <int FORM, bool PAIR>
-__device__ __forceinline__ MmTile mm_tile(const MmShape &s, const int *s_first, int t) {
+__device__ __forceinline__ MmTile mm_tile(const MmShape &s, const int *s_first, const int *s_begin, int t) {
     constexpr int M = PAIR ? 2 * kMmM : kMmM, unit = PAIR ? 32 : 16;
     MmTile q;
     int hi;
     if (FORM == kGradient) {
-        const int per = s.feature_tiles * s.column_tiles;
+        const int per = s.m_tiles * s.n_tiles;
         q.expert = t / per;
-        const int i = t - q.expert * per, f = i / s.column_tiles;
-        rows_of(s.offsets, q.expert, s.rows, &q.lo, &hi);
-        q.m0 = f * M, q.n0 = (i - f * s.column_tiles) * s.n;
-        q.n = min(s.n, (s.columns - q.n0 + unit - 1) / unit * unit);
+        const int i = t - q.expert * per, f = i / s.n_tiles;
+        q.lo = s_begin[q.expert], hi = max(q.lo, s_begin[q.expert + 1]);
+        q.m0 = f * M, q.n0 = (i - f * s.n_tiles) * s.n;
+        q.n = min(s.n, (s.n_size - q.n0 + unit - 1) / unit * unit);
         q.length = hi - q.lo;
         q.steps = (q.length + kMmK - 1) / kMmK;
     } else {
-        const int r = t / s.feature_tiles, f = t - r * s.feature_tiles;
+        const int r = t / s.m_tiles, f = t - r * s.m_tiles;
         q.expert = expert_of(s_first, s.experts, r);
-        rows_of(s.offsets, q.expert, s.rows, &q.lo, &hi);
+        q.lo = s_begin[q.expert], hi = max(q.lo, s_begin[q.expert + 1]);
         // equal shares of the expert's rows
         const int tiles = s_first[q.expert + 1] - s_first[q.expert], share = ((hi - q.lo + tiles - 1) / tiles + unit - 1) / unit * unit;
         q.n0 = q.lo + (r - s_first[q.expert]) * share;
@@ -333,8 +404,8 @@ __device__ __forceinline__ bool ragged(const MmTile &q, int k) { return q.length
 // W_K: consecutive terms of the sums are consecutive in memory (K-major weights), else consecutive features.  PAIR: two blocks
 // of a cluster on one tile: each fetches its 128 of the 256 m and its half of n, the first issues the products of both, the
 // accumulators of a block's 128 m are its own.  The copies of both report to the first block's barrier, but for the
-// last rows of an expert in kGradient: each block waits for its own and clears what does not belong to the expert, and the
-// second tells the first.
+// last rows of an expert in kGradient: each block waits for its own and clears what does not belong to the expert (its last
+// warp), and tells the first.
 template <int FORM, bool PAIR, bool W_K, typename T, typename TO>
 __global__ void __launch_bounds__(kMmThreads, 1)
     expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -343,13 +414,12 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     constexpr bool a_k = FORM == kRows && W_K, b_k = FORM == kRows;
     constexpr unsigned a_bytes = kMmM * kMmK * sizeof(T);
     extern __shared__ __align__(16) char s_raw[];
-    __shared__ int s_first[kMostExperts + 1];
+    __shared__ int s_first[kMostExperts + 1], s_begin[kMostExperts + 1];  // row tiles before an expert; the offsets, clamped
     __shared__ uint64_t s_full[kMmMostStages], s_empty[kMmMostStages], s_own[kMmMostStages], s_ready[kMmMostStages], s_acc_full[2], s_acc_empty[2];
     __shared__ unsigned s_tmem;
     __shared__ int s_stop_word;
     volatile int *s_stop = &s_stop_word;
     char *ring = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
-    float4 *staging = reinterpret_cast<float4 *>(ring + (size_t)s.stages * s.stage_bytes);  // kGradient: 4 KB for each of four warps
     const int w = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;  // clusters of two along x
     const int worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
@@ -357,8 +427,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
 
     if (w == 0) {
         if (lane == 0) {
-            for (int i = 0; i < s.stages; i++) barrier_init(&s_full[i], 1), barrier_init(&s_empty[i], 1), barrier_init(&s_own[i], 1), barrier_init(&s_ready[i], 1);
-            for (int i = 0; i < 2; i++) barrier_init(&s_acc_full[i], 1), barrier_init(&s_acc_empty[i], PAIR ? 8 : 4);
+            for (int i = 0; i < s.stages; i++) barrier_init(&s_full[i], 1), barrier_init(&s_empty[i], 1), barrier_init(&s_own[i], 1), barrier_init(&s_ready[i], PAIR ? 2 : 1);
+            for (int i = 0; i < 2; i++) barrier_init(&s_acc_full[i], 1), barrier_init(&s_acc_empty[i], PAIR ? 16 : 8);
             s_stop_word = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
@@ -372,6 +442,9 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         }
     } else if (w == 2 && FORM == kRows) {
         count_row_tiles(s.offsets, s.experts, s.rows, s.n, s_first);
+    } else if (w > 2) {
+        for (int e = threadIdx.x - 96; e <= s.experts; e += kMmThreads - 96)
+            s_begin[e] = (int)min(max((int64_t)__ldg(s.offsets + e), (int64_t)0), s.rows);
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -379,14 +452,14 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     if constexpr (PAIR) pair_barrier();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = s_tmem;
-    const int tiles = FORM == kGradient ? s.experts * s.feature_tiles * s.column_tiles : s_first[s.experts] * s.feature_tiles;
+    const int tiles = FORM == kGradient ? s.experts * s.m_tiles * s.n_tiles : s_first[s.experts] * s.m_tiles;
 
     if (w == 0) {
         int stage = 0;
         unsigned phase = 0;
         bool good = true;
         for (int t = worker; good && t < tiles; t += workers) {
-            const MmTile q = mm_tile<FORM, PAIR>(s, s_first, t);
+            const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
             const int half = PAIR ? q.n >> 1 : q.n, m0 = q.m0 + rank * kMmM, n0 = q.n0 + rank * half;
             // kRows: boxes of 64 rows, then of 16; kGradient: boxes of 64 columns
             const int wide = b_k ? half >> 6 : (half + 63) >> 6, narrow = b_k ? (half & 63) >> 4 : 0;
@@ -408,13 +481,15 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                     for (int g = 0; g < narrow; g++) copy_tile<B>(b + wide * 8192 + g * 2048, &map_c, k0, n0 + wide * 64 + g * 16, 0, barrier);
                 };
                 if (elect_one()) {
-                    if (PAIR && !(FORM == kGradient && ragged(q, k))) {
+                    if (FORM == kGradient && ragged(q, k)) {
+                        barrier_expect(&s_own[stage], bytes);
+                        copy(std::false_type{}, smem_address(&s_own[stage]));
+                    } else if (PAIR) {
                         if (rank == 0) barrier_expect(&s_full[stage], 2 * bytes);
                         copy(std::true_type{}, address_in_first(&s_full[stage]));
                     } else {
-                        uint64_t *barrier = PAIR ? &s_own[stage] : &s_full[stage];
-                        barrier_expect(barrier, bytes);
-                        copy(std::false_type{}, smem_address(barrier));
+                        barrier_expect(&s_full[stage], bytes);
+                        copy(std::false_type{}, smem_address(&s_full[stage]));
                     }
                 }
                 __syncwarp();
@@ -423,13 +498,13 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         }
     } else if (w == 1) {
         int stage = 0, count = 0;
-        unsigned full_phases = 0, own_phases = 0;  // a bit for each stage: the phase that comes next
+        unsigned full_phases = 0, ready_phases = 0;  // a bit for each stage: the phase that comes next
         bool good = true;
-        for (int t = worker; good && t < tiles; t += workers) {
-            const MmTile q = mm_tile<FORM, PAIR>(s, s_first, t);
+        for (int t = worker; rank == 0 && good && t < tiles; t += workers) {
+            const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
             if (q.steps == 0) continue;
             const int slot = count & 1;
-            if (rank == 0 && !(good = warp_wait(&s_acc_empty[slot], ((count >> 1) & 1) ^ 1, s_stop))) break;
+            if (!(good = warp_wait(&s_acc_empty[slot], ((count >> 1) & 1) ^ 1, s_stop))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             count++;
             const int length = FORM == kGradient ? q.length : s.reduced;
@@ -438,28 +513,14 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                 char *a = ring + (size_t)stage * s.stage_bytes;
                 const int left = length - k * kMmK, parts = min(4, (left + 15) / 16);
                 if (FORM == kGradient && ragged(q, k)) {
-                    uint64_t *barrier = PAIR ? &s_own[stage] : &s_full[stage];
-                    if (!(good = warp_wait(barrier, (PAIR ? own_phases : full_phases) >> stage & 1, s_stop))) break;
-                    // rows of the next expert (or behind the last) came along: zeros in both operands up to the next
-                    // multiple of 16, so that nothing that stands there, NaN included, gets into the sum
-                    const int end = (parts * 16 - left) * 8, boxes = 2 + (((PAIR ? q.n >> 1 : q.n) + 63) >> 6);
-                    for (int box = 0; box < boxes; box++)
-                        for (int i = lane; i < end; i += 32)
-                            *reinterpret_cast<uint4 *>(a + (size_t)box * 8192 + left * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (PAIR) {
-                        if (rank == 1) {
-                            if (lane == 0) arrive_at_first<true>(&s_ready[stage]);
-                        } else if (!(good = warp_wait<true>(&s_ready[stage], own_phases >> stage & 1, s_stop))) break;
-                        own_phases ^= 1u << stage;
-                    } else full_phases ^= 1u << stage;
+                    if (!(good = warp_wait<true>(&s_ready[stage], ready_phases >> stage & 1, s_stop))) break;
+                    ready_phases ^= 1u << stage;
                 } else {
-                    if (rank == 0 && !(good = warp_wait(&s_full[stage], full_phases >> stage & 1, s_stop))) break;
+                    if (!(good = warp_wait(&s_full[stage], full_phases >> stage & 1, s_stop))) break;
                     full_phases ^= 1u << stage;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (rank == 0 && elect_one()) {
+                if (elect_one()) {
                     const uint64_t da = operand_descriptor(smem_address(a), a_k), db = operand_descriptor(smem_address(a + a_bytes), b_k);
                     for (int i = 0; i < parts; i++)
                         multiply<PAIR>(tmem + slot * s.acc_stride, da + (uint64_t)(i * (a_k ? 32 : 2048) >> 4),
@@ -471,72 +532,33 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                 if (++stage == s.stages) stage = 0;
             }
         }
-    } else {
-        const int part = w & 3;  // the quarter of the accumulators' lanes that this warp may read
+    } else if (w < 10) {
+        // the quarter of the accumulators' lanes that this warp may read, and whether it takes the even or the odd blocks of 32
+        // columns (four warps alone take longer for a tile than the products of a few hundred rows)
+        const int part = w & 3, odd = (w - 2) >> 2;
         int count = 0;
         for (int t = worker; t < tiles; t += workers) {
-            const MmTile q = mm_tile<FORM, PAIR>(s, s_first, t);
-            const int slot = count & 1, m0 = q.m0 + rank * kMmM;
+            const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
+            const int slot = count & 1, m = q.m0 + rank * kMmM + part * 32;
             if (q.steps > 0) {
                 if (!warp_wait(&s_acc_full[slot], (count >> 1) & 1, s_stop)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 count++;
             }
             const unsigned from = tmem + slot * s.acc_stride + ((unsigned)(part * 32) << 16);
-            if (FORM == kRows) {
-                // a lane is a feature, a column a row of the output: 32 consecutive features of a row at a time
-                const int f = m0 + part * 32 + lane;
-                for (int c = 0; c < q.length; c += 32) {
-                    float v[32];
-                    load_accumulators(from + c, v);
-                    TO *dst = out + (int64_t)(q.n0 + c) * ldo + f;
+            const int rows = FORM == kGradient ? min(q.n, s.n_size - q.n0) : q.length;
+            TO *dst = out + (FORM == kGradient ? q.expert * stride_o : 0) + (int64_t)q.n0 * ldo + m;
+            if (m < s.m_size) {
+                for (int c = odd * 32; c < rows; c += 64) {
+                    unsigned v[32];
+                    if (q.steps > 0) {
+                        request_accumulators(from + c, v);
+                        wait_accumulators(v);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (c + i < q.length && f < s.features) dst[i * ldo] = from_float<TO>(v[i]);
-                }
-            } else {
-                // a lane is a row of the output; 32 columns at a time pass through shared memory, so that rows are written
-                // in whole sectors by neighbouring lanes
-                float4 *mine = staging + part * 256;
-                TO *base = out + q.expert * stride_o + (int64_t)m0 * ldo;
-                const int m_end = s.features - m0, n_end = min(q.n, s.columns - q.n0);
-                constexpr int E = 16 / sizeof(TO), across = 32 / E, down = 32 / across;
-                for (int c = 0; c < n_end && m_end > 0; c += 32) {
-                    float v[32];
-                    if (q.steps > 0) load_accumulators(from + c, v);
-                    else {
-#pragma unroll
-                        for (int i = 0; i < 32; i++) v[i] = 0.f;
+                        for (int i = 0; i < 32; i++) v[i] = 0;
                     }
-#pragma unroll
-                    for (int i = 0; i < 8; i++) mine[lane * 8 + (i ^ (lane & 7))] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                    __syncwarp();
-                    const int column = lane % across;
-#pragma unroll
-                    for (int i = 0; i < 32 / down; i++) {
-                        const int r = i * down + lane / across, m = part * 32 + r, n = c + column * E;
-                        if (m >= m_end || n >= n_end) continue;
-                        float x[E];
-#pragma unroll
-                        for (int j = 0; j < E / 4; j++) {
-                            const float4 p = mine[r * 8 + ((column * (E / 4) + j) ^ (r & 7))];
-                            x[4 * j] = p.x, x[4 * j + 1] = p.y, x[4 * j + 2] = p.z, x[4 * j + 3] = p.w;
-                        }
-                        TO *dst = base + (int64_t)m * ldo + q.n0 + n;
-                        if (s.vectors && n + E <= n_end) {
-                            Pack<TO, E> o;
-                            if (s.beta != 0.f) o = *reinterpret_cast<const Pack<TO, E> *>(dst);
-#pragma unroll
-                            for (int j = 0; j < E; j++)
-                                o.v[j] = from_float<TO>(s.beta != 0.f ? fmaf(s.beta, to_float(o.v[j]), x[j]) : x[j]);
-                            store_pack<TO, E>(dst, o);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < E; j++)
-                                if (n + j < n_end) dst[j] = from_float<TO>(s.beta != 0.f ? fmaf(s.beta, to_float(dst[j]), x[j]) : x[j]);
-                        }
-                    }
-                    __syncwarp();
+                    write_block<TO>(v, dst + c * ldo, ldo, rows - c, s.m_size - m, s.vectors, s.beta);
                 }
             }
             if (q.steps > 0) {
@@ -547,6 +569,31 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                     else barrier_arrive(&s_acc_empty[slot]);
                 }
             }
+        }
+    } else if (FORM == kGradient) {
+        // the ends of experts whose rows are no multiple of 16: rows of the next expert (or behind the last) came along with
+        // the copy.  Zeros in both operands up to the next multiple, so that nothing that stands there, NaN included, gets
+        // into the sum; then the first block's products may go on.
+        int stage = 0;
+        unsigned own_phases = 0;  // a bit for each stage: the phase that comes next
+        bool good = true;
+        for (int t = worker; good && t < tiles; t += workers) {
+            const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
+            const int last = q.steps - 1, left = q.length - last * kMmK;
+            if (q.steps > 0 && ragged(q, last)) {
+                const int at = (stage + last) % s.stages;
+                if (!(good = warp_wait(&s_own[at], own_phases >> at & 1, s_stop))) break;
+                own_phases ^= 1u << at;
+                char *a = ring + (size_t)at * s.stage_bytes;
+                const int end = ((left + 15) / 16 * 16 - left) * 8, boxes = 2 + (((PAIR ? q.n >> 1 : q.n) + 63) >> 6);
+                for (int box = 0; box < boxes; box++)
+                    for (int i = lane; i < end; i += 32)
+                        *reinterpret_cast<uint4 *>(a + (size_t)box * 8192 + left * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) arrive_at_first<true>(&s_ready[at]);
+            }
+            stage = (stage + q.steps) % s.stages;
         }
     }
     __syncwarp();
@@ -615,17 +662,17 @@ static cudaError_t launch_mm(alphasparse_cuda_type_t type, MmShape s, int64_t mo
                              TO *out,
                              int64_t ldo, int64_t stride_o, cudaStream_t st) {
     constexpr bool a_k = FORM == kRows && W_K, b_k = FORM == kRows;
-    constexpr int most_smem = 232448 - 8192, staging = FORM == kGradient ? 16384 : 0;  // tables and barriers are in what is left
+    constexpr int most_smem = 232448 - 12288;  // tables and barriers are in what is left
     const int half = PAIR ? s.n / 2 : s.n;
     s.stage_bytes = (unsigned)(kMmM * kMmK + (b_k ? half : (half + 63) / 64 * 64) * kMmK) * 2;
-    s.stages = std::min<int>(kMmMostStages, (most_smem - 1024 - staging) / (int)s.stage_bytes);
+    s.stages = std::min<int>(kMmMostStages, (most_smem - 1024) / (int)s.stage_bytes);
     const unsigned format = type == ALPHA_SPARSE_CUDA_TYPE_BF16 ? 1 : 0;
     s.instruction = 1u << 4 | format << 7 | format << 10 | (a_k ? 0u : 1u << 15) | (b_k ? 0u : 1u << 16) |
                     (unsigned)((PAIR ? 2 * kMmM : kMmM) >> 4) << 24;
     s.acc_stride = 256;
     s.vectors = address(out) % 16 == 0 && ldo * (int64_t)sizeof(TO) % 16 == 0 && (FORM != kGradient || stride_o * (int64_t)sizeof(TO) % 16 == 0);
     const auto kernel = expert_mm_kernel<FORM, PAIR, W_K, T, TO>;
-    const int smem = 1024 + s.stages * (int)s.stage_bytes + staging;
+    const int smem = 1024 + s.stages * (int)s.stage_bytes;
     int sms = 0;
     cudaError_t e = multiprocessors(&sms);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -689,21 +736,21 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_mm(alphasparse_operation
     cudaError_t e = cudaSuccess;
     if (eb == 2 && reduced > 0 && takes_tma(x, ldx, rows, 0, 1) && takes_tma(w, ldw, out, stride_w, experts)) {
         MmShape s{};
-        s.offsets = offsets, s.experts = (int)experts, s.rows = rows, s.features = (int)features, s.reduced = (int)reduced;
+        s.offsets = offsets, s.experts = (int)experts, s.rows = rows, s.m_size = (int)features, s.reduced = (int)reduced;
         // Many rows an expert: two SMs on a tile.  Few: the weights are what has to be read, by as many SMs as there are; narrow
         // tiles leave room for more of them on their way.
         const int64_t mean = (rows + experts - 1) / experts;
         const bool pair = mean > 64;
         s.n = pair ? 256 : mean <= 16 ? 32 : mean <= 32 ? 64 : 128;
         const int m = pair ? 2 * kMmM : kMmM;
-        s.feature_tiles = (int)((features + m - 1) / m);
+        s.m_tiles = (int)((features + m - 1) / m);
         CUtensorMap mx, mx16, mw;
         if (!make_map(&mx, type, x, reduced, rows, ldx, 1, 0, 64) || !make_map(&mx16, type, x, reduced, rows, ldx, 1, 0, 16) ||
              !make_map(&mw, type, w, in, out, ldw, experts, stride_w, trans ? kMmM : kMmK)) {
             record_error("alphasparse_cuda_expert_mm: no tensor map");
             return ALPHA_SPARSE_STATUS_EXECUTION_FAILED;
         }
-        const int64_t row_tiles = rows / s.n + std::min(experts, rows), tiles = row_tiles * s.feature_tiles;
+        const int64_t row_tiles = rows / s.n + std::min(experts, rows), tiles = row_tiles * s.m_tiles;
         if (tiles > 0x7fffffff - 4096) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
         const auto go = [&](auto t) {
             using T = decltype(t);
@@ -751,21 +798,21 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_mm_grad(alphasparse_cuda
     cudaError_t e = cudaSuccess;
     if (eb == 2 && rows > 0 && takes_tma(dy, lddy, rows, 0, 1) && takes_tma(x, ldx, rows, 0, 1)) {
         MmShape s{};
-        s.offsets = offsets, s.experts = (int)experts, s.rows = rows, s.features = (int)out, s.columns = (int)in, s.beta = beta;
-        s.feature_tiles = (int)((out + 2 * kMmM - 1) / (2 * kMmM));
-        s.column_tiles = (int)((in + 255) / 256);
-        s.n = (int)up_to((in + s.column_tiles - 1) / s.column_tiles, 32);  // equal tiles of at most 256 columns
+        s.offsets = offsets, s.experts = (int)experts, s.rows = rows, s.m_size = (int)in, s.n_size = (int)out, s.beta = beta;
+        s.m_tiles = (int)((in + 2 * kMmM - 1) / (2 * kMmM));
+        s.n_tiles = (int)((out + 255) / 256);
+        s.n = (int)up_to((out + s.n_tiles - 1) / s.n_tiles, 32);  // equal tiles of at most 256 columns of dy
         CUtensorMap my, mx;
         if (!make_map(&my, type, dy, out, rows, lddy, 1, 0, kMmK) || !make_map(&mx, type, x, in, rows, ldx, 1, 0, kMmK)) {
             record_error("alphasparse_cuda_expert_mm_grad: no tensor map");
             return ALPHA_SPARSE_STATUS_EXECUTION_FAILED;
         }
-        const int64_t tiles = experts * s.feature_tiles * s.column_tiles;
+        const int64_t tiles = experts * s.m_tiles * s.n_tiles;
         if (tiles > 0x7fffffff - 4096) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
         const auto go = [&](auto t) {
             using T = decltype(t);
-            if (weight_type == ALPHA_SPARSE_CUDA_TYPE_F32) e = launch_mm<kGradient, true, false, T, float>(type, s, tiles, my, mx, mx, (float *)dw, ldw, stride_w, st);
-            else e = launch_mm<kGradient, true, false, T, T>(type, s, tiles, my, mx, mx, (T *)dw, ldw, stride_w, st);
+            if (weight_type == ALPHA_SPARSE_CUDA_TYPE_F32) e = launch_mm<kGradient, true, false, T, float>(type, s, tiles, mx, my, my, (float *)dw, ldw, stride_w, st);
+            else e = launch_mm<kGradient, true, false, T, T>(type, s, tiles, mx, my, my, (T *)dw, ldw, stride_w, st);
         };
         if (type == ALPHA_SPARSE_CUDA_TYPE_F16) go(__half());
         else go(__nv_bfloat16());
