@@ -1,6 +1,7 @@
 // Embedding lookup and the gradient of its table: Y = scale S E and dE = alpha S^T dY + beta dE, S the one-hot matrix of
 // the tokens.  S is never stored: the lookup reads the tokens, the gradient sorts their positions by token (the transpose
 // of S in CSR form, made for one product) and sums the rows of dY run by run.  No counterpart in the reference.
+#include <limits.h>
 #include <stdio.h>
 
 #include <algorithm>
@@ -74,8 +75,11 @@ __global__ void __launch_bounds__(kRowThreads)
     for (int u = 0; u < U; u++) {
         const int v = v0 + (u << log);
         if (inside && scale != 1.f) {
+            float f[N];
+            unpack<T, N>(p[u], f);
 #pragma unroll
-            for (int i = 0; i < N; i++) p[u].v[i] = from_float<T>(to_float(p[u].v[i]) * scale);
+            for (int i = 0; i < N; i++) f[i] *= scale;
+            p[u] = pack<T, N>(f);
         }
         if (v < nv) store_pack<T, N>(dst + (int64_t)v * N, p[u]);
     }
@@ -83,55 +87,69 @@ __global__ void __launch_bounds__(kRowThreads)
 
 // ---- gradient ------------------------------------------------------------------------------------
 
-constexpr int kGradRows = 512;     // table rows whose tokens one block of the sort collects
+constexpr int kGradMostRows = 1024;  // table rows whose tokens one block of the sort collects, at most
 constexpr int kGradSortWarps = 32;
-constexpr int kGradPiece = 32;     // sorted positions one block of the sum walks
+constexpr int kGradAhead = 16;       // tokens a lane of the sort requests at a time
+constexpr int kGradPiece = 32;       // sorted positions one block of the sum walks
 constexpr int kGradThreads = 128;
 
-// Positions sorted by token, stable, in one launch.  A block owns kGradRows rows of the table and reads every token:
-// a warp takes one contiguous share of them, counts those of each of the block's rows, and after the prefix over warps
-// and rows reads its share again and writes the positions to where they belong.  Tokens below the block's rows are
-// counted on the way, so that no block waits for another.
+// Positions sorted by token, stable, in one launch.  A block owns `own` rows of the table and reads every token: a warp
+// takes one contiguous share of them, counts those of each of the block's rows, and after the prefix over warps and rows
+// goes through its share again and writes the positions to where they belong.  Tokens below the block's rows are
+// counted on the way, so that no block waits for another.  Bound by the latency of a few dependent steps up to some
+// 16,384 tokens, whose shares stay in registers between the two passes; beyond, by instructions.
 template <typename I>
 __global__ void __launch_bounds__(kGradSortWarps * 32)
-    tokens_by_row_kernel(int tokens, const I *__restrict__ token, int64_t inctoken, int vocab, int *__restrict__ ptr,
-                         int *__restrict__ pos, int *__restrict__ row) {
+    tokens_by_row_kernel(int tokens, const I *__restrict__ token, int64_t inctoken, int vocab, int own, int *__restrict__ ptr,
+                         int *__restrict__ pos, int *__restrict__ row, int *__restrict__ joins) {
     extern __shared__ int s_count[];  // [warp][row]
     __shared__ int s_sum[kGradSortWarps], s_below[kGradSortWarps];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int base = blockIdx.x * kGradRows;
-    const int mine = min(kGradRows, vocab - base);
-    for (int i = threadIdx.x; i < kGradSortWarps * kGradRows; i += blockDim.x) s_count[i] = 0;
-    __syncthreads();
+    const int base = blockIdx.x * own;
+    const int mine = min(own, vocab - base);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *joins = 0;  // the list of the sum begins empty
     const int share = (int)(((int64_t)tokens + kGradSortWarps * 32 - 1) / (kGradSortWarps * 32)) * 32;
     const int64_t begin = min((int64_t)tokens, (int64_t)w * share), end = min((int64_t)tokens, begin + share);
-    int *count = s_count + w * kGradRows;
+    int *count = s_count + w * own;
     int below = 0;
-    for (int64_t i0 = begin; i0 < end; i0 += 128) {
-        int64_t t[4];
+    // the block's row of each token of this lane, -1 for none
+    int r[kGradAhead];
+    const auto request = [&](int64_t i0) {
+        I t[kGradAhead];
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < kGradAhead; u++) {
             const int64_t i = i0 + u * 32 + lane;
-            t[u] = i < end ? (int64_t)token[i * inctoken] : -1;
+            t[u] = i < end ? token[i * inctoken] : (I)-1;
         }
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            if (t[u] >= 0 && t[u] < base) below++;
-            else if (t[u] >= base && t[u] < base + mine) atomicAdd(&count[t[u] - base], 1);
+        for (int u = 0; u < kGradAhead; u++) r[u] = t[u] >= 0 && t[u] < (I)vocab ? (int)t[u] - base : INT_MIN;
+    };
+    request(begin);
+    for (int i = threadIdx.x; i < kGradSortWarps * own; i += blockDim.x) s_count[i] = 0;
+    __syncthreads();
+    for (int64_t i0 = begin; i0 < end; i0 += kGradAhead * 32) {
+        if (i0 != begin) request(i0);
+#pragma unroll
+        for (int u = 0; u < kGradAhead; u++) {
+            if (r[u] < 0) below += r[u] != INT_MIN;
+            else if (r[u] < mine) atomicAdd(&count[r[u]], 1);
         }
     }
     below = __reduce_add_sync(0xffffffffu, below);
     if (lane == 0) s_below[w] = below;
     __syncthreads();
     int start = 0;
+#pragma unroll
     for (int v = 0; v < kGradSortWarps; v++) start += s_below[v];
     int total = 0;
-    if (threadIdx.x < kGradRows)
+    if ((int)threadIdx.x < own) {
+#pragma unroll 8
         for (int v = 0; v < kGradSortWarps; v++) {
-            const int c = s_count[v * kGradRows + threadIdx.x];
-            s_count[v * kGradRows + threadIdx.x] = total;
+            const int c = s_count[v * own + threadIdx.x];
+            s_count[v * own + threadIdx.x] = total;
             total += c;
         }
+    }
     int inc = total;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -142,32 +160,27 @@ __global__ void __launch_bounds__(kGradSortWarps * 32)
     __syncthreads();
     for (int v = 0; v < w; v++) start += s_sum[v];
     start += inc - total;
-    if ((int)threadIdx.x < kGradRows) {
-        for (int v = 0; v < kGradSortWarps; v++) s_count[v * kGradRows + threadIdx.x] += start;
+    if ((int)threadIdx.x < own) {
+#pragma unroll 8
+        for (int v = 0; v < kGradSortWarps; v++) s_count[v * own + threadIdx.x] += start;
         if ((int)threadIdx.x < mine) ptr[base + threadIdx.x] = start;
         if (base + (int)threadIdx.x == vocab - 1) ptr[vocab] = start + total;
     }
     __syncthreads();
-    for (int64_t i0 = begin; i0 < end; i0 += 128) {
-        int64_t t[4];
+    for (int64_t i0 = begin; i0 < end; i0 += kGradAhead * 32) {
+        if (share > kGradAhead * 32) request(i0);
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int64_t i = i0 + u * 32 + lane;
-            t[u] = i < end ? (int64_t)token[i * inctoken] : -1;
-        }
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const bool in = t[u] >= base && t[u] < base + mine;
+        for (int u = 0; u < kGradAhead; u++) {
+            const bool in = r[u] >= 0 && r[u] < mine;
             if (!__any_sync(0xffffffffu, in)) continue;
-            const int r = in ? (int)(t[u] - base) : -1;
-            const unsigned same = __match_any_sync(0xffffffffu, r);
+            const unsigned same = __match_any_sync(0xffffffffu, in ? r[u] : -1);
             const int lower = __popc(same & ((1u << lane) - 1u));
-            const int at = in ? count[r] + lower : 0;
+            const int at = in ? count[r[u]] + lower : 0;
             __syncwarp();
             if (in) {
                 pos[at] = (int)(i0 + u * 32 + lane);
-                row[at] = base + r;
-                if (lower == 0) count[r] += __popc(same);
+                row[at] = base + r[u];
+                if (lower == 0) count[r[u]] += __popc(same);
             }
             __syncwarp();
         }
@@ -176,23 +189,34 @@ __global__ void __launch_bounds__(kGradSortWarps * 32)
 
 template <typename T, int N>
 __device__ __forceinline__ void finish_row(T *p, const float (&acc)[N], float alpha, float beta) {
-    Pack<T, N> out;
-    if (beta != 0.f) out = *reinterpret_cast<const Pack<T, N> *>(p);
+    float f[N];
+    if (beta != 0.f) unpack<T, N>(load_pack<T, N, true>(p), f);
 #pragma unroll
-    for (int i = 0; i < N; i++)
-        out.v[i] = from_float<T>(beta != 0.f ? fmaf(alpha, acc[i], beta * to_float(out.v[i])) : alpha * acc[i]);
-    store_pack<T, N>(p, out);
+    for (int i = 0; i < N; i++) f[i] = beta != 0.f ? fmaf(alpha, acc[i], beta * f[i]) : alpha * acc[i];
+    store_pack<T, N>(p, pack<T, N>(f));
 }
 
-// Block (piece, column tile): walks kGradPiece sorted positions, eight rows of dY requested at a time, and adds up runs of
-// one token in 32 bits, in the order of the tokens.  A run that begins and ends in the piece is finished here; what
-// the piece holds of others goes to the partial sums (first slot: of the run that came in, second: of the one that goes on).
-// The blocks behind take the table's rows that no token names: zeros for beta = 0, beta times what is there else.
-template <typename T, typename TO, int N>
+// A run of one token that goes over from piece to piece: block `piece` begins it, `pieces` behind go on.  The columns from
+// `column` up to `end`: at most kJoinWarps tiles of 128, a warp each, for few pieces; one tile, shared by the warps, for many.
+struct Join {
+    int row, piece, pieces, column, end;
+};
+constexpr int kJoinWarps = 8;
+constexpr int kJoinFew = 8;
+constexpr int kJoinTile = 128;
+
+// Block (piece, column tile): walks kGradPiece sorted positions, several rows of dY requested at a time (and the old values of
+// table rows that end among them), and adds up runs of one token in 32 bits, in the order of the tokens.  A run that
+// begins and ends in the piece is finished here; what the piece holds of others goes to the partial sums (first slot: of the run
+// that came in, second: of the one that goes on), and the run to the list of the join.  The list's order is not fixed, the
+// order of every sum is.  The blocks behind take the table's rows that no token names: zeros for beta = 0, beta times
+// what is there else.
+template <typename T, typename TO, int N, bool BETA>
 __global__ void __launch_bounds__(kGradThreads)
     embedding_grad_kernel(int pieces, int tiles, int nv, int vocab, const int *__restrict__ ptr, const int *__restrict__ pos,
                           const int *__restrict__ row, const T *__restrict__ dy, int64_t lddy, float alpha, float beta,
-                          TO *__restrict__ dtable, int64_t ldt, float *__restrict__ partial, int64_t ldp) {
+                          TO *__restrict__ dtable, int64_t ldt, float *__restrict__ partial, int64_t ldp, int *__restrict__ joins,
+                          Join *__restrict__ join) {
     const int64_t sums = (int64_t)pieces * tiles;
     if (blockIdx.x >= sums) {
         const int first = (int)(blockIdx.x - sums) * 8;
@@ -214,27 +238,49 @@ __global__ void __launch_bounds__(kGradThreads)
         if (lane < n) s_pos[lane] = pos[begin + lane];
     }
     __syncthreads();
+    if (lane == 0 && s_row[n] == s_row[n + 1]) {
+        const int r = s_row[n];
+        if (ptr[r] >= begin) {  // the run begins here
+            const int behind = (ptr[r + 1] - 1) / kGradPiece - piece, width = nv * N;
+            const int step = behind <= kJoinFew ? kJoinTile * kJoinWarps : kJoinTile;
+            const int c0 = tile * kGradThreads * N, c1 = min(width, c0 + kGradThreads * N);
+            int at = atomicAdd(joins, (c1 - c0 + step - 1) / step);
+            for (int c = c0; c < c1; c += step) join[at++] = Join{r, piece, behind, c, min(c + step, c1)};
+        }
+    }
     const int v = tile * kGradThreads + lane;
     if (v >= nv) return;
     const T *src = dy + (int64_t)v * N;
+    TO *dst = dtable + (int64_t)v * N;
     float acc[N] = {};
     bool came_in = s_row[0] == s_row[1];
-    constexpr int kAhead = 8;
+    constexpr int kAhead = BETA ? 4 : 8;
     for (int i0 = 0; i0 < n; i0 += kAhead) {
         Pack<T, N> p[kAhead];
+        Pack<TO, N> old[BETA ? kAhead : 1];
 #pragma unroll
         for (int u = 0; u < kAhead; u++)
             if (i0 + u < n) p[u] = load_pack<T, N>(src + s_pos[i0 + u] * lddy);
+        if (BETA) {
+#pragma unroll
+            for (int u = 0; u < kAhead; u++)
+                if (i0 + u < n && s_row[i0 + u + 1] != s_row[i0 + u + 2]) old[u] = load_pack<TO, N, true>(dst + (int64_t)s_row[i0 + u + 1] * ldt);
+        }
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
             const int i = i0 + u;
             if (i >= n) break;
+            float f[N];
+            unpack<T, N>(p[u], f);
 #pragma unroll
-            for (int k = 0; k < N; k++) acc[k] += to_float(p[u].v[k]);
+            for (int k = 0; k < N; k++) acc[k] += f[k];
             const bool ends = s_row[i + 1] != s_row[i + 2];
             if (!ends && i + 1 < n) continue;
             if (ends && !came_in) {
-                finish_row<TO, N>(dtable + (int64_t)s_row[i + 1] * ldt + (int64_t)v * N, acc, alpha, beta);
+                if (BETA) unpack<TO, N>(old[BETA ? u : 0], f);
+#pragma unroll
+                for (int k = 0; k < N; k++) f[k] = BETA ? fmaf(alpha, acc[k], beta * f[k]) : alpha * acc[k];
+                store_pack<TO, N>(dst + (int64_t)s_row[i + 1] * ldt, pack<TO, N>(f));
             } else {
                 float *to = partial + ((int64_t)piece * 2 + (came_in ? 0 : 1)) * ldp + (int64_t)v * N;
 #pragma unroll
@@ -247,38 +293,44 @@ __global__ void __launch_bounds__(kGradThreads)
     }
 }
 
-// Runs that cross pieces: the block of the piece in which such a run begins adds its partial sums, a share of the pieces
-// per warp, the warps' sums in their order.  The order is fixed, so the result does not change from call to call.
-constexpr int kJoinWarps = 8;
+// Runs that cross pieces, one entry of the list at a time: the partial sums of the run, few by one warp, many in equal shares by
+// all, whose sums are added in their order.
 template <typename TO>
 __global__ void __launch_bounds__(kJoinWarps * 32)
-    embedding_grad_join_kernel(int width, int vocab, const int *__restrict__ ptr, const int *__restrict__ row, float alpha,
-                               float beta, TO *__restrict__ dtable, int64_t ldt, const float *__restrict__ partial, int64_t ldp) {
+    embedding_grad_join_kernel(float alpha, float beta, TO *__restrict__ dtable, int64_t ldt,
+                               const float *__restrict__ partial, int64_t ldp, const int *__restrict__ joins, const Join *__restrict__ join) {
     __shared__ float4 s_sum[kJoinWarps][32];
-    const int piece = blockIdx.x, last = (piece + 1) * kGradPiece - 1;
-    if (last + 1 >= ptr[vocab]) return;
-    const int r = row[last];
-    if (row[last + 1] != r || ptr[r] < piece * kGradPiece) return;
-    const int first = piece + 1, pieces = (ptr[r + 1] - 1) / kGradPiece - piece;  // pieces behind this one
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int share = (pieces + kJoinWarps - 1) / kJoinWarps, begin = min(pieces, w * share), end = min(pieces, begin + share);
-    for (int c0 = blockIdx.y * 128; c0 < width; c0 += gridDim.y * 128) {
-        const int c = c0 + lane * 4;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, count = *joins;
+    for (int i = blockIdx.x; i < count; i += gridDim.x) {
+        const Join j = join[i];
+        const bool few = j.pieces <= kJoinFew;
+        const int share = few ? j.pieces : (j.pieces + kJoinWarps - 1) / kJoinWarps;
+        const int begin = few ? 0 : min(j.pieces, w * share), end = min(j.pieces, begin + share);
+        const int c0 = j.column + (few ? w * kJoinTile : 0), c = c0 + lane * 4;
+        const float *from = partial + c;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < width) {
-            if (w == 0) acc = *reinterpret_cast<const float4 *>(partial + ((int64_t)piece * 2 + 1) * ldp + c);
-#pragma unroll 4
-            for (int i = begin; i < end; i++) {
-                const float4 p = *reinterpret_cast<const float4 *>(partial + (int64_t)(first + i) * 2 * ldp + c);
-                acc.x += p.x, acc.y += p.y, acc.z += p.z, acc.w += p.w;
+        if (c < j.end) {
+            if (few || w == 0) acc = *reinterpret_cast<const float4 *>(from + ((int64_t)j.piece * 2 + 1) * ldp);
+#pragma unroll 8
+            for (int p = begin; p < end; p++) {
+                const float4 v = *reinterpret_cast<const float4 *>(from + (int64_t)(j.piece + 1 + p) * 2 * ldp);
+                acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
             }
         }
+        TO *dst = dtable + (int64_t)j.row * ldt;
         s_sum[w][lane] = acc;
-        __syncthreads();
-        if (threadIdx.x < 128 && c0 + (int)threadIdx.x < width) {
-            float sum[1] = {0.f};
-            for (int v = 0; v < min(kJoinWarps, pieces); v++) sum[0] += reinterpret_cast<const float *>(s_sum[v])[threadIdx.x];
-            finish_row<TO, 1>(dtable + (int64_t)r * ldt + c0 + threadIdx.x, sum, alpha, beta);
+        if (few) __syncwarp();
+        else __syncthreads();
+        if (few || w == 0) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {  // neighbouring lanes, neighbouring columns
+                const int at = q * 32 + lane;
+                float sum[1] = {0.f};
+                if (few) sum[0] = reinterpret_cast<const float *>(s_sum[w])[at];
+                else
+                    for (int v = 0; v < kJoinWarps; v++) sum[0] += reinterpret_cast<const float *>(s_sum[v])[at];
+                if (c0 + at < j.end) finish_row<TO, 1>(dst + c0 + at, sum, alpha, beta);
+            }
         }
         __syncthreads();
     }
@@ -286,7 +338,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
 
 // The pieces of the workspace, each on a 256-byte boundary
 struct GradSpace {
-    size_t ptr, pos, row, partial, bytes;
+    size_t ptr, pos, row, joins, join, partial, bytes;
     int64_t pieces, ldp;
     GradSpace(int64_t tokens, int64_t vocab, int64_t width) {
         const auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
@@ -295,7 +347,10 @@ struct GradSpace {
         ptr = 0;
         pos = up(sizeof(int) * ((size_t)vocab + 1));
         row = pos + up(sizeof(int) * (size_t)tokens);
-        partial = row + up(sizeof(int) * (size_t)tokens);
+        joins = row + up(sizeof(int) * (size_t)tokens);
+        join = joins + up(sizeof(int));
+        // one entry per piece and tile of 128 columns at most
+        partial = join + up(sizeof(Join) * (size_t)pieces * (size_t)((width + kJoinTile - 1) / kJoinTile));
         bytes = partial + up(sizeof(float) * 2 * (size_t)pieces * (size_t)ldp);
     }
 };
@@ -308,7 +363,8 @@ template <typename T, typename TO>
 static cudaError_t launch_grad_sums(const GradSpace &sp, char *buffer, int64_t tokens, int64_t vocab, int64_t width, float alpha,
                                     const T *dy, int64_t lddy, float beta, TO *dtable, int64_t ldt, cudaStream_t st) {
     int *ptr = reinterpret_cast<int *>(buffer + sp.ptr), *pos = reinterpret_cast<int *>(buffer + sp.pos),
-        *row = reinterpret_cast<int *>(buffer + sp.row);
+        *row = reinterpret_cast<int *>(buffer + sp.row), *joins = reinterpret_cast<int *>(buffer + sp.joins);
+    Join *join = reinterpret_cast<Join *>(buffer + sp.join);
     float *partial = reinterpret_cast<float *>(buffer + sp.partial);
     const int vb = vector_bytes(sizeof(T), {address(dy), (uint64_t)lddy * sizeof(T), (uint64_t)width * sizeof(T)});
     const int vo = vector_bytes(sizeof(TO), {address(dtable), (uint64_t)ldt * sizeof(TO), (uint64_t)width * sizeof(TO)});
@@ -318,8 +374,9 @@ static cudaError_t launch_grad_sums(const GradSpace &sp, char *buffer, int64_t t
         const int64_t blocks = sp.pieces * tiles + (beta == 1.f ? 0 : (vocab + 7) / 8);
         if (blocks <= 0) return cudaSuccess;
         if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-        embedding_grad_kernel<T, TO, N><<<(unsigned)blocks, kGradThreads, 0, st>>>(
-            (int)sp.pieces, tiles, nv, (int)vocab, ptr, pos, row, dy, lddy, alpha, beta, dtable, ldt, partial, sp.ldp);
+        const auto kernel = beta != 0.f ? embedding_grad_kernel<T, TO, N, true> : embedding_grad_kernel<T, TO, N, false>;
+        kernel<<<(unsigned)blocks, kGradThreads, 0, st>>>((int)sp.pieces, tiles, nv, (int)vocab, ptr, pos, row, dy, lddy, alpha, beta, dtable,
+                                                          ldt, partial, sp.ldp, joins, join);
         return cudaGetLastError();
     };
     cudaError_t e;
@@ -331,9 +388,9 @@ static cudaError_t launch_grad_sums(const GradSpace &sp, char *buffer, int64_t t
     if (e != cudaSuccess) return e;
     count_launch();
     if (sp.pieces > 1) {
-        const unsigned tiles = (unsigned)std::min<int64_t>(8, (width + 127) / 128);
-        embedding_grad_join_kernel<TO><<<dim3((unsigned)sp.pieces - 1, tiles), kJoinWarps * 32, 0, st>>>(
-            (int)width, (int)vocab, ptr, row, alpha, beta, dtable, ldt, partial, sp.ldp);
+        const int64_t most = (sp.pieces - 1) * ((width + kJoinTile - 1) / kJoinTile);
+        embedding_grad_join_kernel<TO><<<(unsigned)std::min<int64_t>(148 * 4, most), kJoinWarps * 32, 0, st>>>(alpha, beta, dtable, ldt,
+                                                                                                         partial, sp.ldp, joins, join);
         count_launch();
     }
     return cudaGetLastError();
@@ -411,13 +468,17 @@ extern "C" alphasparse_status_t alphasparse_cuda_embedding_grad(alphasparse_cuda
     char *space = static_cast<char *>(buffer);
     int *ptr = reinterpret_cast<int *>(space + sp.ptr), *pos = reinterpret_cast<int *>(space + sp.pos),
         *row = reinterpret_cast<int *>(space + sp.row);
-    const unsigned blocks = (unsigned)((vocab + kGradRows - 1) / kGradRows);
-    const size_t smem = sizeof(int) * kGradSortWarps * kGradRows;
+    // as many blocks as there are SMs, while their counts fit shared memory
+    const int own = (int)std::min<int64_t>(kGradMostRows, ((vocab + 147) / 148 + 31) / 32 * 32);
+    const unsigned blocks = (unsigned)((vocab + own - 1) / own);
+    const size_t smem = sizeof(int) * kGradSortWarps * (size_t)own;
     const auto sort = [&](auto i) {
         using I = decltype(i);
-        cudaError_t e = cudaFuncSetAttribute(tokens_by_row_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        cudaError_t e = cudaFuncSetAttribute(tokens_by_row_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)(sizeof(int) * kGradSortWarps * kGradMostRows));
         if (e != cudaSuccess) return e;
-        tokens_by_row_kernel<I><<<blocks, kGradSortWarps * 32, smem, st>>>((int)tokens, (const I *)token, inctoken, (int)vocab, ptr, pos, row);
+        tokens_by_row_kernel<I><<<blocks, kGradSortWarps * 32, smem, st>>>((int)tokens, (const I *)token, inctoken, (int)vocab, own, ptr, pos, row,
+                                                                          reinterpret_cast<int *>(space + sp.joins));
         return cudaGetLastError();
     };
     ASB_CUDA_OR(index_type == ALPHA_SPARSE_CUDA_INDEX_I32 ? sort((int32_t)0) : sort((int64_t)0), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);

@@ -285,16 +285,6 @@ __device__ __forceinline__ void wait_accumulators(unsigned (&r)[32]) {
                  : "memory");
 }
 
-template <typename T> __device__ __forceinline__ unsigned pack_two(float a, float b);
-template <> __device__ __forceinline__ unsigned pack_two<__half>(float a, float b) {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const unsigned *>(&v);
-}
-template <> __device__ __forceinline__ unsigned pack_two<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const unsigned *>(&v);
-}
-
 // A warp writes a block of 32 rows x 32 columns of the output: a lane has one column, its register i row i.  dst: row 0, the
 // warp's first column; `rows` and `cols` of them exist.  32-bit elements: a row is a line, as it is.  16-bit ones are
 // exchanged among eight lanes in three steps, until a lane has eight columns of four rows and writes 16 bytes at a time (a

@@ -14,8 +14,10 @@ namespace asb {
 // ---- plan ----------------------------------------------------------------------------------------
 
 constexpr int kPlanThreads = 512, kPlanWarps = kPlanThreads / 32;
-constexpr int kPlanKeys = 4096;    // pairs a block takes at least
+constexpr int kPlanOne = 4096;     // up to so many pairs in one block
+constexpr int kPlanKeys = 2048;    // else pairs a block takes at least
 constexpr int kPlanMostBlocks = 256;
+constexpr int kPlanAhead = 8;      // pairs a lane requests at a time
 
 // Exclusive prefix over the threads of the block; s_sum: one int per warp
 __device__ __forceinline__ int plan_scan(int v, int *s_sum) {
@@ -35,59 +37,79 @@ __device__ __forceinline__ int plan_scan(int v, int *s_sum) {
 }
 
 // A block takes a contiguous share of the pairs and each of its warps a contiguous share of that, counts the pairs of each
-// expert per warp, and (PLACE) after the prefix over experts, blocks and warps reads them again and places them.  With more
-// than one block a first launch writes the blocks' counts for the second to read.
+// expert per warp, and (PLACE) after the prefix over experts, blocks and warps goes through them again and places them.  With
+// more than one block a first launch writes the blocks' counts for the second to read.  Bound by the latency of its steps: a
+// lane's pairs are requested eight at a time and stay in registers between the passes where they are no more.
 template <bool PLACE>
 __global__ void __launch_bounds__(kPlanThreads)
     plan_kernel(int64_t pairs, int64_t share, int experts, int k, const int *__restrict__ index, int64_t ldi,
                 int *__restrict__ counts, int *__restrict__ offsets, int *__restrict__ slot, int64_t lds) {
     extern __shared__ int s_count[];  // [warp][expert]
     __shared__ int s_sum[kPlanWarps];
+    __shared__ int s_total[kPlanThreads], s_before[kPlanThreads];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    for (int i = threadIdx.x; i < kPlanWarps * experts; i += kPlanThreads) s_count[i] = 0;
-    __syncthreads();
     const int64_t first = blockIdx.x * share, last = min(pairs, first + share);
     const int64_t part = (share / kPlanWarps + 31) / 32 * 32;
     const int64_t begin = min(last, first + w * part), end = w == kPlanWarps - 1 ? last : min(last, begin + part);
     int *count = s_count + w * experts;
-    const auto key_at = [&](int64_t i) {
-        if (i >= end) return -1;
-        const int64_t t = (int64_t)((unsigned)i / (unsigned)k);
-        const int e = index[t * ldi + (i - t * k)];
-        return e >= 0 && e < experts ? e : -1;
+    int e[kPlanAhead];
+    const auto request = [&](int64_t i0) {
+#pragma unroll
+        for (int u = 0; u < kPlanAhead; u++) {
+            const int64_t i = i0 + u * 32 + lane, t = (int64_t)((unsigned)i / (unsigned)k);
+            e[u] = i < end ? index[t * ldi + (i - t * k)] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < kPlanAhead; u++)
+            if (e[u] < 0 || e[u] >= experts) e[u] = -1;
     };
-    for (int64_t i0 = begin; i0 < end; i0 += 128) {
-        int e[4];
+    request(begin);
+    for (int i = threadIdx.x; i < kPlanWarps * experts; i += kPlanThreads) s_count[i] = 0;
+    __syncthreads();
+    for (int64_t i0 = begin; i0 < end; i0 += kPlanAhead * 32) {
+        if (i0 != begin) request(i0);
 #pragma unroll
-        for (int u = 0; u < 4; u++) e[u] = key_at(i0 + u * 32 + lane);
-#pragma unroll
-        for (int u = 0; u < 4; u++)
+        for (int u = 0; u < kPlanAhead; u++)
             if (e[u] >= 0) atomicAdd(&count[e[u]], 1);
     }
     __syncthreads();
     const int blocks = gridDim.x, b = blockIdx.x;
+    // threads side by side have neighbouring experts; where experts are few, groups of threads share the blocks' counts
+    const int across = min(kPlanThreads, (experts + 31) / 32 * 32), parts = kPlanThreads / across;
+    const int my_part = threadIdx.x / across, column = threadIdx.x - my_part * across;
     int carry = 0;
-    for (int e0 = 0; e0 < experts; e0 += kPlanThreads) {
-        const int e = e0 + threadIdx.x;
+    for (int e0 = 0; e0 < experts; e0 += across) {
+        const int x = e0 + column;
         int mine = 0;
-        if (e < experts)
+        if (my_part == 0 && x < experts) {
+#pragma unroll
             for (int v = 0; v < kPlanWarps; v++) {
-                const int c = s_count[v * experts + e];
-                s_count[v * experts + e] = mine;
+                const int c = s_count[v * experts + x];
+                s_count[v * experts + x] = mine;
                 mine += c;
             }
+        }
         if (!PLACE) {
-            if (e < experts) counts[(int64_t)b * experts + e] = mine;
+            if (my_part == 0 && x < experts) counts[(int64_t)b * experts + x] = mine;
             continue;
         }
         int total = mine, before = 0;
-        if (blocks > 1 && e < experts) {
+        if (blocks > 1) {
             total = 0;
+            if (my_part < parts && x < experts) {
 #pragma unroll 8
-            for (int v = 0; v < blocks; v++) {
-                const int c = counts[(int64_t)v * experts + e];
-                before += v < b ? c : 0;
-                total += c;
+                for (int v = my_part; v < blocks; v += parts) {
+                    const int c = counts[(int64_t)v * experts + x];
+                    before += v < b ? c : 0;
+                    total += c;
+                }
+            }
+            s_total[threadIdx.x] = total, s_before[threadIdx.x] = before;
+            __syncthreads();
+            if (my_part == 0) {
+                for (int v = 1; v < parts; v++) total += s_total[v * across + column], before += s_before[v * across + column];
+            } else {
+                total = 0;
             }
         }
         const int start = carry + plan_scan(total, s_sum);
@@ -95,22 +117,22 @@ __global__ void __launch_bounds__(kPlanThreads)
         __syncthreads();
         carry = s_sum[0];
         __syncthreads();
-        if (e < experts) {
-            for (int v = 0; v < kPlanWarps; v++) s_count[v * experts + e] += start + before;
+        if (my_part == 0 && x < experts) {
+#pragma unroll
+            for (int v = 0; v < kPlanWarps; v++) s_count[v * experts + x] += start + before;
             if (b == 0) {
-                offsets[e] = start;
-                if (e == experts - 1) offsets[experts] = start + total;
+                offsets[x] = start;
+                if (x == experts - 1) offsets[experts] = start + total;
             }
         }
     }
     if (!PLACE) return;
     __syncthreads();
-    for (int64_t i0 = begin; i0 < end; i0 += 128) {
-        int e[4];
+    for (int64_t i0 = begin; i0 < end; i0 += kPlanAhead * 32) {
+        if (part > kPlanAhead * 32 || i0 != begin) request(i0);
 #pragma unroll
-        for (int u = 0; u < 4; u++) e[u] = key_at(i0 + u * 32 + lane);
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < kPlanAhead; u++) {
+            if (i0 + u * 32 >= end) break;
             const int64_t i = i0 + u * 32 + lane;
             const unsigned same = __match_any_sync(0xffffffffu, e[u]);
             const int lower = __popc(same & ((1u << lane) - 1u));
@@ -133,7 +155,7 @@ struct PlanShape {
     size_t bytes;
     PlanShape(int64_t tokens, int64_t k, int64_t experts) {
         pairs = tokens * k;
-        const int64_t want = std::min<int64_t>(kPlanMostBlocks, std::max<int64_t>(1, (pairs + kPlanKeys - 1) / kPlanKeys));
+        const int64_t want = pairs <= kPlanOne ? 1 : std::min<int64_t>(kPlanMostBlocks, (pairs + kPlanKeys - 1) / kPlanKeys);
         const int64_t unit = 32 * kPlanWarps;  // whole steps of every warp
         share = ((pairs + want - 1) / want + unit - 1) / unit * unit;
         if (share == 0) share = unit;
@@ -175,11 +197,11 @@ __global__ void __launch_bounds__(kRowThreads)
 // out[t] = sum over j of weight[t, j] y[slot[t, j]] + beta out[t], in 32 bits in the order of j, rounded once.  Eight rows of y
 // are requested at a time, 16 bytes of each by a thread: 128 bytes in flight at 64 registers.  (12,001 tokens of 6 rows of 2048
 // fp16: four rows of 64 bytes at 138 registers, one block per SM, 94 us; so COMBINE_US us.)
-constexpr __host__ __device__ int combine_unroll(int bytes) { return bytes >= 16 ? 1 : bytes >= 8 ? 2 : bytes >= 4 ? 4 : 8; }
+constexpr __host__ __device__ int combine_unroll(int bytes) { return bytes >= 16 ? 1 : bytes >= 8 ? 2 : 4; }
 constexpr int kCombineAhead = 8;
 
 template <typename T, int N, int U>
-__global__ void __launch_bounds__(kRowThreads, 4)
+__global__ void __launch_bounds__(kRowThreads, N * sizeof(T) == 16 ? 4 : 3)
     combine_kernel(int tokens, int k, int nv, const T *__restrict__ y, int64_t ldy, int64_t rows, const int *__restrict__ slot,
                    int64_t lds, const float *__restrict__ weight, int64_t ldw, float beta, T *__restrict__ out, int64_t ldo,
                    int log) {
@@ -207,9 +229,12 @@ __global__ void __launch_bounds__(kRowThreads, 4)
             if (at[j] < 0) continue;
             const float w = weight ? __ldg(weight + t * ldw + j0 + j) : 1.f;
 #pragma unroll
-            for (int u = 0; u < U; u++)
+            for (int u = 0; u < U; u++) {
+                float f[N];
+                unpack<T, N>(p[j][u], f);
 #pragma unroll
-                for (int i = 0; i < N; i++) acc[u][i] = fmaf(w, to_float(p[j][u].v[i]), acc[u][i]);
+                for (int i = 0; i < N; i++) acc[u][i] = fmaf(w, f[i], acc[u][i]);
+            }
         }
     }
 #pragma unroll
@@ -217,11 +242,13 @@ __global__ void __launch_bounds__(kRowThreads, 4)
         const int v = v0 + (u << log);
         if (v >= nv) continue;
         T *dst = out + t * ldo + (int64_t)v * N;
-        Pack<T, N> r;
-        if (beta != 0.f) r = *reinterpret_cast<const Pack<T, N> *>(dst);
+        if (beta != 0.f) {
+            float f[N];
+            unpack<T, N>(load_pack<T, N, true>(dst), f);
 #pragma unroll
-        for (int i = 0; i < N; i++) r.v[i] = from_float<T>(beta != 0.f ? fmaf(beta, to_float(r.v[i]), acc[u][i]) : acc[u][i]);
-        store_pack<T, N>(dst, r);
+            for (int i = 0; i < N; i++) acc[u][i] = fmaf(beta, f[i], acc[u][i]);
+        }
+        store_pack<T, N>(dst, pack<T, N>(acc[u]));
     }
 }
 
@@ -229,7 +256,7 @@ __global__ void __launch_bounds__(kRowThreads, 4)
 // whole row of a token, so that the inner products end in it: lanes, then warps, in a fixed order.  Eight rows at a time,
 // as above; their eight inner products are added up over a warp together, each step halving what a lane holds.
 template <typename T, int N>
-__global__ void __launch_bounds__(kRowThreads, 3)
+__global__ void __launch_bounds__(kRowThreads, N * sizeof(T) == 16 ? 3 : 2)
     combine_grad_kernel(int tokens, int k, int nv, const T *__restrict__ dout, int64_t ldo, const T *__restrict__ y, int64_t ldy,
                         int64_t rows, const int *__restrict__ slot, int64_t lds, const float *__restrict__ weight, int64_t ldw,
                         T *__restrict__ dy, int64_t lddy, float *__restrict__ dweight, int64_t lddw, int log) {
@@ -263,14 +290,15 @@ __global__ void __launch_bounds__(kRowThreads, 3)
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     if (v0 + u * group >= nv) continue;
-                    Pack<T, N> o;
+                    float f[N], g[N];
+                    unpack<T, N>(d[u], f);
+                    unpack<T, N>(p[j][u], g);
 #pragma unroll
                     for (int i = 0; i < N; i++) {
-                        const float f = to_float(d[u].v[i]);
-                        dot[j] = fmaf(f, to_float(p[j][u].v[i]), dot[j]);
-                        o.v[i] = from_float<T>(w * f);
+                        dot[j] = fmaf(f[i], g[i], dot[j]);
+                        f[i] *= w;
                     }
-                    store_pack<T, N>(dy + at[j] * lddy + (int64_t)(v0 + u * group) * N, o);
+                    store_pack<T, N>(dy + at[j] * lddy + (int64_t)(v0 + u * group) * N, pack<T, N>(f));
                 }
             }
         }

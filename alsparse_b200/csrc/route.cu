@@ -88,9 +88,10 @@ __device__ __forceinline__ void load_logits(const T *row, int experts, bool pack
     if (packs && first + I <= experts) {
 #pragma unroll
         for (int i = 0; i < I; i += P) {
-            const Pack<T, P> p = load_pack<T, P>(row + first + i);
+            float f[P];
+            unpack<T, P>(load_pack<T, P>(row + first + i), f);
 #pragma unroll
-            for (int j = 0; j < P; j++) x[i + j] = to_float(p.v[j]);
+            for (int j = 0; j < P; j++) x[i + j] = f[j];
         }
     } else {
 #pragma unroll

@@ -22,50 +22,97 @@ template <> __device__ __forceinline__ float from_float(float v) { return v; }
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 
-// N consecutive elements, moved in accesses of at most 16 bytes
+template <typename T> __device__ __forceinline__ unsigned pack_two(float a, float b);  // 16-bit types, a in the low half
+template <> __device__ __forceinline__ unsigned pack_two<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned *>(&v);
+}
+template <> __device__ __forceinline__ unsigned pack_two<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const unsigned *>(&v);
+}
+
+// N consecutive elements as words, moved in accesses of at most 16 bytes.  (Kept as words and taken apart by shifts: arrays of
+// 16-bit elements cost the compiler registers and stack.)
 template <typename T, int N>
-struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
-    T v[N];
+struct Pack {
+    static constexpr int bytes = sizeof(T) * N, words = bytes < 4 ? 1 : bytes / 4;
+    unsigned w[words];
 };
 
-template <typename T, int N>
+// PLAIN: memory that the kernel writes too
+template <typename T, int N, bool PLAIN = false>
 __device__ __forceinline__ Pack<T, N> load_pack(const T *p) {
     Pack<T, N> r;
-    constexpr int bytes = sizeof(T) * N;
+    constexpr int bytes = Pack<T, N>::bytes;
+    const auto get = [](const auto *q) { return PLAIN ? *q : __ldg(q); };
     if constexpr (bytes >= 16) {
 #pragma unroll
-        for (int i = 0; i < bytes / 16; i++)
-            reinterpret_cast<uint4 *>(&r)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+        for (int i = 0; i < bytes / 16; i++) {
+            const uint4 v = get(reinterpret_cast<const uint4 *>(p) + i);
+            r.w[4 * i] = v.x, r.w[4 * i + 1] = v.y, r.w[4 * i + 2] = v.z, r.w[4 * i + 3] = v.w;
+        }
     } else if constexpr (bytes == 8) {
-        *reinterpret_cast<uint2 *>(&r) = __ldg(reinterpret_cast<const uint2 *>(p));
+        const uint2 v = get(reinterpret_cast<const uint2 *>(p));
+        r.w[0] = v.x, r.w[1] = v.y;
     } else if constexpr (bytes == 4) {
-        *reinterpret_cast<unsigned *>(&r) = __ldg(reinterpret_cast<const unsigned *>(p));
+        r.w[0] = get(reinterpret_cast<const unsigned *>(p));
     } else {
-        *reinterpret_cast<unsigned short *>(&r) = __ldg(reinterpret_cast<const unsigned short *>(p));
+        r.w[0] = get(reinterpret_cast<const unsigned short *>(p));
     }
     return r;
 }
 
 template <typename T, int N>
 __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r) {
-    constexpr int bytes = sizeof(T) * N;
+    constexpr int bytes = Pack<T, N>::bytes;
     if constexpr (bytes >= 16) {
 #pragma unroll
-        for (int i = 0; i < bytes / 16; i++) reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(&r)[i];
+        for (int i = 0; i < bytes / 16; i++)
+            reinterpret_cast<uint4 *>(p)[i] = make_uint4(r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]);
     } else if constexpr (bytes == 8) {
-        *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(&r);
+        *reinterpret_cast<uint2 *>(p) = make_uint2(r.w[0], r.w[1]);
     } else if constexpr (bytes == 4) {
-        *reinterpret_cast<unsigned *>(p) = *reinterpret_cast<const unsigned *>(&r);
+        *reinterpret_cast<unsigned *>(p) = r.w[0];
     } else {
-        *reinterpret_cast<unsigned short *>(p) = *reinterpret_cast<const unsigned short *>(&r);
+        *reinterpret_cast<unsigned short *>(p) = (unsigned short)r.w[0];
     }
 }
 
+// All bits zero: zeros of every type
 template <typename T, int N>
 __device__ __forceinline__ Pack<T, N> zero_pack() {
     Pack<T, N> r;
 #pragma unroll
-    for (int i = 0; i < N; i++) r.v[i] = from_float<T>(0.f);
+    for (int i = 0; i < Pack<T, N>::words; i++) r.w[i] = 0;
+    return r;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void unpack(const Pack<T, N> &p, float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if constexpr (std::is_same<T, float>::value) {
+            f[i] = __uint_as_float(p.w[i]);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            f[i] = __uint_as_float(i & 1 ? p.w[i / 2] & 0xffff0000u : p.w[i / 2] << 16);
+        } else {
+            f[i] = __half2float(__ushort_as_half((unsigned short)(i & 1 ? p.w[i / 2] >> 16 : p.w[i / 2] & 0xffffu)));
+        }
+    }
+}
+
+// Rounds to nearest, ties to even: the only rounding to the type
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> pack(const float (&f)[N]) {
+    Pack<T, N> r;
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+        for (int i = 0; i < N; i++) r.w[i] = __float_as_uint(f[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < (N + 1) / 2; i++) r.w[i] = pack_two<T>(f[2 * i], 2 * i + 1 < N ? f[2 * i + 1] : 0.f);
+    }
     return r;
 }
 
