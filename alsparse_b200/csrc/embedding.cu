@@ -104,6 +104,7 @@ __global__ void __launch_bounds__(kGradSortWarps * 32)
                          int *__restrict__ pos, int *__restrict__ row, int *__restrict__ joins) {
     extern __shared__ int s_count[];  // [warp][row]
     __shared__ int s_sum[kGradSortWarps], s_below[kGradSortWarps];
+    let_next_begin();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int base = blockIdx.x * own;
     const int mine = min(own, vocab - base);
@@ -217,6 +218,8 @@ __global__ void __launch_bounds__(kGradThreads)
                           const int *__restrict__ row, const T *__restrict__ dy, int64_t lddy, float alpha, float beta,
                           TO *__restrict__ dtable, int64_t ldt, float *__restrict__ partial, int64_t ldp, int *__restrict__ joins,
                           Join *__restrict__ join) {
+    after_previous();
+    let_next_begin();
     const int64_t sums = (int64_t)pieces * tiles;
     if (blockIdx.x >= sums) {
         const int first = (int)(blockIdx.x - sums) * 8;
@@ -300,6 +303,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
     embedding_grad_join_kernel(float alpha, float beta, TO *__restrict__ dtable, int64_t ldt,
                                const float *__restrict__ partial, int64_t ldp, const int *__restrict__ joins, const Join *__restrict__ join) {
     __shared__ float4 s_sum[kJoinWarps][32];
+    after_previous();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, count = *joins;
     for (int i = blockIdx.x; i < count; i += gridDim.x) {
         const Join j = join[i];
@@ -375,9 +379,8 @@ static cudaError_t launch_grad_sums(const GradSpace &sp, char *buffer, int64_t t
         if (blocks <= 0) return cudaSuccess;
         if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
         const auto kernel = beta != 0.f ? embedding_grad_kernel<T, TO, N, true> : embedding_grad_kernel<T, TO, N, false>;
-        kernel<<<(unsigned)blocks, kGradThreads, 0, st>>>((int)sp.pieces, tiles, nv, (int)vocab, ptr, pos, row, dy, lddy, alpha, beta, dtable,
-                                                          ldt, partial, sp.ldp, joins, join);
-        return cudaGetLastError();
+        return launch_behind(kernel, dim3((unsigned)blocks), kGradThreads, 0, st, (int)sp.pieces, tiles, nv, (int)vocab, ptr, pos, row, dy, lddy,
+                             alpha, beta, dtable, ldt, partial, sp.ldp, joins, join);
     };
     cudaError_t e;
     constexpr int full = 16 / sizeof(T);
@@ -389,8 +392,9 @@ static cudaError_t launch_grad_sums(const GradSpace &sp, char *buffer, int64_t t
     count_launch();
     if (sp.pieces > 1) {
         const int64_t most = (sp.pieces - 1) * ((width + kJoinTile - 1) / kJoinTile);
-        embedding_grad_join_kernel<TO><<<(unsigned)std::min<int64_t>(148 * 4, most), kJoinWarps * 32, 0, st>>>(alpha, beta, dtable, ldt,
-                                                                                                         partial, sp.ldp, joins, join);
+        e = launch_behind(embedding_grad_join_kernel<TO>, dim3((unsigned)std::min<int64_t>(148 * 4, most)), kJoinWarps * 32, 0, st, alpha, beta,
+                          dtable, ldt, partial, sp.ldp, joins, join);
+        if (e != cudaSuccess) return e;
         count_launch();
     }
     return cudaGetLastError();

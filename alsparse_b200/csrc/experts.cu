@@ -47,6 +47,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     extern __shared__ int s_count[];  // [warp][expert]
     __shared__ int s_sum[kPlanWarps];
     __shared__ int s_total[kPlanThreads], s_before[kPlanThreads];
+    if (!PLACE) let_next_begin();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t first = blockIdx.x * share, last = min(pairs, first + share);
     const int64_t part = (share / kPlanWarps + 31) / 32 * 32;
@@ -95,6 +96,7 @@ __global__ void __launch_bounds__(kPlanThreads)
         }
         int total = mine, before = 0;
         if (blocks > 1) {
+            if (e0 == 0) after_previous();  // the counts, and with them whatever came before the first launch
             total = 0;
             if (my_part < parts && x < experts) {
 #pragma unroll 8
@@ -383,7 +385,12 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_plan(int64_t tokens, int
     }
     ASB_CUDA_OR(cudaFuncSetAttribute(plan_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(int) * kPlanWarps * kMostExperts)),
                 ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
-    plan_kernel<true><<<sh.blocks, kPlanThreads, smem, st>>>(sh.pairs, sh.share, (int)experts, (int)k, index, ldi, counts, offsets, slot, lds);
+    if (sh.blocks > 1)
+        ASB_CUDA_OR(launch_behind(plan_kernel<true>, dim3(sh.blocks), kPlanThreads, smem, st, sh.pairs, sh.share, (int)experts, (int)k, index, ldi,
+                                  counts, offsets, slot, lds),
+                    ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    else
+        plan_kernel<true><<<1, kPlanThreads, smem, st>>>(sh.pairs, sh.share, (int)experts, (int)k, index, ldi, counts, offsets, slot, lds);
     count_launch();
     ASB_CUDA_OR(cudaGetLastError(), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
     return ALPHA_SPARSE_STATUS_SUCCESS;

@@ -116,6 +116,24 @@ __device__ __forceinline__ Pack<T, N> pack(const float (&f)[N]) {
     return r;
 }
 
+// ---- launches ----------------------------------------------------------------------------------
+
+// A kernel that begins with after_previous(): its blocks may be made resident while the kernel before it on the stream ends
+// (as soon as that one has called let_next_begin or its blocks are done), and wait there until its writes are complete.
+// Saves about two microseconds between the kernels of one call.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... P, typename... A>
+cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchAttribute behind[1];
+    behind[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    behind[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid, config.blockDim = dim3(threads), config.dynamicSmemBytes = smem, config.stream = st;
+    config.attrs = behind, config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, P(args)...);
+}
+
 // ---- arguments -------------------------------------------------------------------------------
 
 // 0 for a value that names no type
