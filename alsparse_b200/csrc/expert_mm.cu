@@ -33,33 +33,33 @@ __device__ __forceinline__ void rows_of(const int *__restrict__ offsets, int e, 
     *hi = (int)min(max((int64_t)__ldg(offsets + e + 1), a), rows);
 }
 
-// first[e] = row tiles of the experts before e, e = 0 .. experts; by one warp.  Offsets that name more rows than there are
-// (they do not ascend) give no tiles at all.
-__device__ __forceinline__ void count_row_tiles(const int *__restrict__ offsets, int experts, int64_t rows, int tile, int *first) {
+// begin[e] = offsets[e] within [0, rows] and not before begin[e - 1] as it stands there, for the whole block to read after a barrier
+__device__ __forceinline__ void load_offsets(const int *__restrict__ offsets, int experts, int64_t rows, int *begin) {
+    for (int e = threadIdx.x; e <= experts; e += blockDim.x) begin[e] = (int)min(max((int64_t)__ldg(offsets + e), (int64_t)0), rows);
+}
+
+// first[e] = row tiles of the experts before e, e = 0 .. experts; by one warp, from begin.  Offsets that name more rows than
+// there are (they do not ascend) give no tiles at all.
+__device__ __forceinline__ void count_row_tiles(const int *begin, int experts, int64_t rows, int tile, int *first) {
     const int lane = threadIdx.x & 31;
     int carry = 0;
     int64_t named = 0;
     for (int e0 = 0; e0 < experts; e0 += 32) {
-        int n = 0, lo = 0, hi = 0;
-        if (e0 + lane < experts) {
-            rows_of(offsets, e0 + lane, rows, &lo, &hi);
-            n = (hi - lo + tile - 1) / tile;
-        }
-        int64_t here = hi - lo;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) here += __shfl_xor_sync(0xffffffffu, here, o);
-        named += here;
-        if (named > rows) {
-            carry = 0;
-            break;
-        }
+        const int e = e0 + lane, here = e < experts ? max(0, begin[e + 1] - begin[e]) : 0;
+        const int n = (here + tile - 1) / tile;
         int inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
-        if (e0 + lane < experts) first[e0 + lane] = carry + inc - n;
+        // the sum of 32 counts may pass an int
+        named += (int64_t)__reduce_add_sync(0xffffffffu, (unsigned)here >> 16) * 65536 + __reduce_add_sync(0xffffffffu, (unsigned)here & 0xffffu);
+        if (named > rows) {
+            carry = 0;
+            break;
+        }
+        if (e < experts) first[e] = carry + inc - n;
         carry += __shfl_sync(0xffffffffu, inc, 31);
     }
     if (lane == 0) first[experts] = carry;
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(256)
     expert_mm_plain_kernel(const int *__restrict__ offsets, int experts, int64_t rows, int m_size, int n_size, int k_size,
                            const T *__restrict__ a, int64_t lda, int64_t stride_a, const T *__restrict__ b, int64_t ldb,
                            int64_t stride_b, float beta, TO *__restrict__ c, int64_t ldc, int64_t stride_c) {
-    __shared__ int s_first[kMostExperts + 1];
+    __shared__ int s_first[kMostExperts + 1], s_begin[kMostExperts + 1];
     __shared__ __align__(16) float s_a[kPlainStep][kPlainTile + 4], s_b[kPlainStep][kPlainTile + 4];  // read four at a time
     int e, lo, hi, m0, m_end, k_end;
     const int n0 = blockIdx.x * kPlainTile;
@@ -95,7 +95,9 @@ __global__ void __launch_bounds__(256)
         rows_of(offsets, e, rows, &lo, &hi);
         m0 = blockIdx.y * kPlainTile, m_end = m_size, k_end = hi - lo;
     } else {
-        if (threadIdx.x < 32) count_row_tiles(offsets, experts, rows, kPlainTile, s_first);
+        load_offsets(offsets, experts, rows, s_begin);
+        __syncthreads();
+        if (threadIdx.x < 32) count_row_tiles(s_begin, experts, rows, kPlainTile, s_first);
         __syncthreads();
         const int r = (int)(blockIdx.y + blockIdx.z * gridDim.y);
         if (r >= s_first[experts]) return;
@@ -143,7 +145,7 @@ __global__ void __launch_bounds__(256)
 
 // ---- tensor cores --------------------------------------------------------------------------------
 
-constexpr int kMmThreads = 352;  // copies, products, eight warps for the accumulators, one for the ends of ragged experts
+constexpr int kMmThreads = 384;  // copies, products, eight warps for the accumulators, two for the ends of ragged experts
 constexpr int kMmM = 128, kMmK = 64;
 constexpr int kMmMostStages = 8;
 constexpr unsigned long long kMmLimitNs = 2000000000ull;
@@ -296,34 +298,34 @@ __device__ __forceinline__ void write_block(const unsigned (&r)[32], TO *dst, in
     if constexpr (sizeof(TO) == 2) {
         if (vectors && beta == 0.f) {
             unsigned p[16];
+            const unsigned halves = lane & 1 ? 0x3276 : 0x5410;  // the odd rows of both lanes, or the even ones
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const unsigned own = pack_two<TO>(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-                const unsigned other = __shfl_xor_sync(0xffffffffu, own, 1);
-                p[i] = lane & 1 ? __byte_perm(other, own, 0x7632) : __byte_perm(own, other, 0x5410);
+                p[i] = __byte_perm(own, __shfl_xor_sync(0xffffffffu, own, 1), halves);
             }
+            const bool second = lane & 2, upper = lane & 4;
             uint2 h[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const unsigned other = __shfl_xor_sync(0xffffffffu, lane & 2 ? p[2 * i] : p[2 * i + 1], 2);
-                h[i] = lane & 2 ? make_uint2(other, p[2 * i + 1]) : make_uint2(p[2 * i], other);
+                const unsigned other = __shfl_xor_sync(0xffffffffu, second ? p[2 * i] : p[2 * i + 1], 2);
+                h[i] = make_uint2(second ? other : p[2 * i], second ? p[2 * i + 1] : other);
             }
             const int first = lane & ~7;
+            TO *to = dst + (lane & 7) * ldo + first;
+            const bool whole = rows >= 32 && cols >= 32;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint2 give = lane & 4 ? h[2 * i] : h[2 * i + 1], keep = lane & 4 ? h[2 * i + 1] : h[2 * i];
-                const uint2 other = make_uint2(__shfl_xor_sync(0xffffffffu, give.x, 4), __shfl_xor_sync(0xffffffffu, give.y, 4));
-                const uint4 o = lane & 4 ? make_uint4(other.x, other.y, keep.x, keep.y) : make_uint4(keep.x, keep.y, other.x, other.y);
-                const int row = 8 * i + (lane & 7);
-                TO *to = dst + row * ldo + first;
-                if (row < rows) {
-                    if (first + 8 <= cols) *reinterpret_cast<uint4 *>(to) = o;
-                    else {
-                        const TO *e = reinterpret_cast<const TO *>(&o);
+            for (int i = 0; i < 4; i++, to += 8 * ldo) {
+                const unsigned ox = __shfl_xor_sync(0xffffffffu, upper ? h[2 * i].x : h[2 * i + 1].x, 4);
+                const unsigned oy = __shfl_xor_sync(0xffffffffu, upper ? h[2 * i].y : h[2 * i + 1].y, 4);
+                const uint4 o = make_uint4(upper ? ox : h[2 * i].x, upper ? oy : h[2 * i].y, upper ? h[2 * i + 1].x : ox, upper ? h[2 * i + 1].y : oy);
+                if (whole || (8 * i + (lane & 7) < rows && first + 8 <= cols)) {
+                    *reinterpret_cast<uint4 *>(to) = o;
+                } else if (8 * i + (lane & 7) < rows) {
+                    const unsigned e[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            if (first + j < cols) to[j] = e[j];
-                    }
+                    for (int j = 0; j < 8; j++)
+                        if (first + j < cols) reinterpret_cast<unsigned short *>(to)[j] = (unsigned short)(e[j / 2] >> 16 * (j & 1));
                 }
             }
             return;
@@ -415,8 +417,12 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     const int worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
     constexpr unsigned columns = 512;  // all of TMEM: one block per SM
 
+    load_offsets(s.offsets, s.experts, s.rows, s_begin);
     if (w == 0) {
         if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+            if (b_k) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_c) : "memory");
             for (int i = 0; i < s.stages; i++) barrier_init(&s_full[i], 1), barrier_init(&s_empty[i], 1), barrier_init(&s_own[i], 1), barrier_init(&s_ready[i], PAIR ? 2 : 1);
             for (int i = 0; i < 2; i++) barrier_init(&s_acc_full[i], 1), barrier_init(&s_acc_empty[i], PAIR ? 16 : 8);
             s_stop_word = 0;
@@ -430,15 +436,14 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(&s_tmem)), "r"(columns) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         }
-    } else if (w == 2 && FORM == kRows) {
-        count_row_tiles(s.offsets, s.experts, s.rows, s.n, s_first);
-    } else if (w > 2) {
-        for (int e = threadIdx.x - 96; e <= s.experts; e += kMmThreads - 96)
-            s_begin[e] = (int)min(max((int64_t)__ldg(s.offsets + e), (int64_t)0), s.rows);
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (FORM == kRows) {
+        if (w == 2) count_row_tiles(s_begin, s.experts, s.rows, s.n, s_first);
+        __syncthreads();
+    }
     if constexpr (PAIR) pair_barrier();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = s_tmem;
@@ -538,16 +543,23 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             const unsigned from = tmem + slot * s.acc_stride + ((unsigned)(part * 32) << 16);
             const int rows = FORM == kGradient ? min(q.n, s.n_size - q.n0) : q.length;
             TO *dst = out + (FORM == kGradient ? q.expert * stride_o : 0) + (int64_t)q.n0 * ldo + m;
-            if (m < s.m_size) {
+            if (q.steps == 0) {
+                // an expert without rows: beta times what is there, a row of the block's 128 columns per warp and step
+                TO *all = dst - part * 32;
+                const int cols = min(kMmM, s.m_size - q.m0 - rank * kMmM);
+                for (int r = w - 2; r < rows; r += 8) {
+                    TO *to = all + r * ldo;
+                    if (s.vectors && s.beta == 0.f && cols == kMmM) {
+                        if (lane * 16 < kMmM * (int)sizeof(TO)) reinterpret_cast<uint4 *>(to)[lane] = make_uint4(0, 0, 0, 0);
+                    } else {
+                        for (int c = lane; c < cols; c += 32) to[c] = from_float<TO>(s.beta != 0.f ? s.beta * to_float(to[c]) : 0.f);
+                    }
+                }
+            } else if (m < s.m_size) {
                 for (int c = odd * 32; c < rows; c += 64) {
                     unsigned v[32];
-                    if (q.steps > 0) {
-                        request_accumulators(from + c, v);
-                        wait_accumulators(v);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; i++) v[i] = 0;
-                    }
+                    request_accumulators(from + c, v);
+                    wait_accumulators(v);
                     write_block<TO>(v, dst + c * ldo, ldo, rows - c, s.m_size - m, s.vectors, s.beta);
                 }
             }
@@ -563,8 +575,9 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     } else if (FORM == kGradient) {
         // the ends of experts whose rows are no multiple of 16: rows of the next expert (or behind the last) came along with
         // the copy.  Zeros in both operands up to the next multiple, so that nothing that stands there, NaN included, gets
-        // into the sum; then the first block's products may go on.
-        int stage = 0;
+        // into the sum; then the first block's products may go on.  Two warps in turn: one alone takes 1.7 us a tile, of which its
+        // fence and arrival are most, and the rest of a short tile 1.0.
+        int stage = 0, turn = w & 1;
         unsigned own_phases = 0;  // a bit for each stage: the phase that comes next
         bool good = true;
         for (int t = worker; good && t < tiles; t += workers) {
@@ -572,16 +585,20 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             const int last = q.steps - 1, left = q.length - last * kMmK;
             if (q.steps > 0 && ragged(q, last)) {
                 const int at = (stage + last) % s.stages;
+                // both wait for every one: a phase that is not waited for would be taken for the one after the next
                 if (!(good = warp_wait(&s_own[at], own_phases >> at & 1, s_stop))) break;
                 own_phases ^= 1u << at;
-                char *a = ring + (size_t)at * s.stage_bytes;
-                const int end = ((left + 15) / 16 * 16 - left) * 8, boxes = 2 + (((PAIR ? q.n >> 1 : q.n) + 63) >> 6);
-                for (int box = 0; box < boxes; box++)
-                    for (int i = lane; i < end; i += 32)
-                        *reinterpret_cast<uint4 *>(a + (size_t)box * 8192 + left * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) arrive_at_first<true>(&s_ready[at]);
+                turn ^= 1;
+                if (turn) {
+                    char *a = ring + (size_t)at * s.stage_bytes;
+                    const int end = ((left + 15) / 16 * 16 - left) * 8, boxes = 2 + (((PAIR ? q.n >> 1 : q.n) + 63) >> 6);
+                    for (int box = 0; box < boxes; box++)
+                        for (int i = lane; i < end; i += 32)
+                            *reinterpret_cast<uint4 *>(a + (size_t)box * 8192 + left * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) arrive_at_first<true>(&s_ready[at]);
+                }
             }
             stage = (stage + q.steps) % s.stages;
         }
