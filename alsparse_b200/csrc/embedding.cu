@@ -54,10 +54,14 @@ alphasparse_status_t check_operands(const char *call, std::initializer_list<Oper
 
 // ---- lookup --------------------------------------------------------------------------------------
 
-template <typename T, typename I, int N, int U>
+// ANY: rows that begin on no 16-byte boundary.  A row of y is cut at the boundaries of its memory and read at whatever shift the
+// table's row has to it.  (16,000 rows of 3283 fp16: 2 bytes an access, 16 of
+// them in flight, 79 us, so 42 us.)
+template <typename T, typename I, int U, bool ANY>
 __global__ void __launch_bounds__(kRowThreads)
-    embedding_kernel(int rows, const I *__restrict__ token, int64_t inctoken, int64_t vocab, int nv, float scale,
-                     const T *__restrict__ table, int64_t ldt, T *__restrict__ y, int64_t ldy, int log) {
+    embedding_kernel(int rows, const I *__restrict__ token, int64_t inctoken, int64_t vocab, int width, float scale,
+                     const T *__restrict__ table, int64_t ldt, Window all, T *__restrict__ y, int64_t ldy, int log) {
+    constexpr int E = 16 / sizeof(T);
     const int64_t r = (int64_t)blockIdx.x * (kRowThreads >> log) + (threadIdx.x >> log);
     if (r >= rows) return;
     const int64_t t = (int64_t)token[r * inctoken];
@@ -65,23 +69,36 @@ __global__ void __launch_bounds__(kRowThreads)
     const T *src = table + (inside ? t : 0) * ldt;
     T *dst = y + r * ldy;
     const int v0 = (int)(blockIdx.y * (U << log) + (threadIdx.x & ((1 << log) - 1)));
-    Pack<T, N> p[U];
+    const Cut<T> cut(dst, width);
+    Pack<T, E> p[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int v = v0 + (u << log);
-        p[u] = inside && v < nv ? load_pack<T, N>(src + (int64_t)v * N) : zero_pack<T, N>();
+        p[u] = zero_pack<T, E>();
+        if (ANY) {
+            if (inside && cut.is_whole(v)) p[u] = load_any<T>(src + cut.begin(v), all);
+        } else if (inside && v * E < width) {
+            p[u] = load_pack<T, E>(src + v * E);
+        }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int v = v0 + (u << log);
         if (inside && scale != 1.f) {
-            float f[N];
-            unpack<T, N>(p[u], f);
+            float f[E];
+            unpack<T, E>(p[u], f);
 #pragma unroll
-            for (int i = 0; i < N; i++) f[i] *= scale;
-            p[u] = pack<T, N>(f);
+            for (int i = 0; i < E; i++) f[i] *= scale;
+            p[u] = pack<T, E>(f);
         }
-        if (v < nv) store_pack<T, N>(dst + (int64_t)v * N, p[u]);
+        if (ANY) {
+            if (cut.is_whole(v)) store_pack<T, E>(dst + cut.begin(v), p[u]);
+            else
+                for (int i = cut.begin(v); i < cut.end(v); i++)
+                    dst[i] = !inside ? from_float<T>(0.f) : scale != 1.f ? from_float<T>(to_float(__ldg(src + i)) * scale) : __ldg(src + i);
+        } else if (v * E < width) {
+            store_pack<T, E>(dst + v * E, p[u]);
+        }
     }
 }
 
@@ -416,19 +433,18 @@ extern "C" alphasparse_status_t alphasparse_cuda_embedding(alphasparse_cuda_inde
                                                                                {y, tokens, width, ldy, eb, true}});
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     const int vb = vector_bytes(eb, {address(table), (uint64_t)ldt * eb, address(y), (uint64_t)ldy * eb, (uint64_t)width * eb});
-    const int64_t nv = width * (int64_t)eb / vb;
-    const RowShape shape = row_shape(tokens, nv, in_flight(vb));
+    const bool any = vb < 16;
+    const RowShape shape = row_shape(tokens, any ? most_pieces(width, eb) : width * (int64_t)eb / 16, 4);
+    const Window all = window(table, vocab, width, ldt, eb);
     cudaStream_t st = current_stream();
     const auto run = [&](auto t) {
         using T = decltype(t);
         const auto with_index = [&](auto i) {
             using I = decltype(i);
-            with_pack<T>(vb, [&](auto n) {
-                constexpr int N = decltype(n)::value;
-                const auto kernel = shape.unroll == 1 ? embedding_kernel<T, I, N, 1> : embedding_kernel<T, I, N, in_flight(N * sizeof(T))>;
-                kernel<<<shape.grid, kRowThreads, 0, st>>>((int)tokens, (const I *)token, inctoken, vocab, (int)nv, scale,
-                                                         (const T *)table, ldt, (T *)y, ldy, shape.log);
-            });
+            const auto kernel = any ? (shape.unroll == 1 ? embedding_kernel<T, I, 1, true> : embedding_kernel<T, I, 4, true>)
+                                    : (shape.unroll == 1 ? embedding_kernel<T, I, 1, false> : embedding_kernel<T, I, 4, false>);
+            kernel<<<shape.grid, kRowThreads, 0, st>>>((int)tokens, (const I *)token, inctoken, vocab, (int)width, scale, (const T *)table, ldt, all,
+                                                     (T *)y, ldy, shape.log);
         };
         if (index_type == ALPHA_SPARSE_CUDA_INDEX_I32) with_index((int32_t)0);
         else with_index((int64_t)0);

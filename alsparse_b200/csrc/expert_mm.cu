@@ -290,7 +290,7 @@ __device__ __forceinline__ void wait_accumulators(unsigned (&r)[32]) {
 // A warp writes a block of 32 rows x 32 columns of the output: a lane has one column, its register i row i.  dst: row 0, the
 // warp's first column; `rows` and `cols` of them exist.  32-bit elements: a row is a line, as it is.  16-bit ones are
 // exchanged among eight lanes in three steps, until a lane has eight columns of four rows and writes 16 bytes at a time (a
-// store of two bytes a lane and row took 923 us where this takes MM_DX us: 32,768 rows of 8 experts, 4096 x 4096,
+// store of two bytes a lane and row took 923 us where this takes 705 us: 32,768 rows of 8 experts, 4096 x 4096,
 // operation N).
 template <typename TO>
 __device__ __forceinline__ void write_block(const unsigned (&r)[32], TO *dst, int64_t ldo, int rows, int cols, bool vectors, float beta) {

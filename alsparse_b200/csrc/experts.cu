@@ -168,28 +168,50 @@ struct PlanShape {
 
 // ---- dispatch --------------------------------------------------------------------------------------
 
-// Threads along a token's row as row_shape lays them out: the row is read once and written to every place of the token.
-template <typename T, int N, int U>
+// Threads along a token's row as row_shape lays them out: the row is read once and written to every place of the token.  ANY:
+// rows that begin on no 16-byte boundary; each place is cut at the boundaries of its memory, and the row read again at the
+// shift that it has to it, out of L1.
+template <typename T, int U, bool ANY>
 __global__ void __launch_bounds__(kRowThreads)
-    dispatch_kernel(int tokens, int k, int nv, const T *__restrict__ x, int64_t ldx, const int *__restrict__ slot, int64_t lds,
-                    int64_t rows, T *__restrict__ xs, int64_t ldxs, int log) {
+    dispatch_kernel(int tokens, int k, int width, const T *__restrict__ x, int64_t ldx, Window all, const int *__restrict__ slot,
+                    int64_t lds, int64_t rows, T *__restrict__ xs, int64_t ldxs, int log) {
+    constexpr int E = 16 / sizeof(T);
     const int64_t t = (int64_t)blockIdx.x * (kRowThreads >> log) + (threadIdx.x >> log);
     if (t >= tokens) return;
     const int v0 = (int)(blockIdx.y * (U << log) + (threadIdx.x & ((1 << log) - 1)));
-    Pack<T, N> p[U];
+    const T *src = x + t * ldx;
+    Pack<T, E> p[U];
+    if (!ANY) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int v = v0 + (u << log);
-        if (v < nv) p[u] = load_pack<T, N>(x + t * ldx + (int64_t)v * N);
+        for (int u = 0; u < U; u++) {
+            const int v = v0 + (u << log);
+            if (v * E < width) p[u] = load_pack<T, E>(src + v * E);
+        }
     }
     for (int j = 0; j < k; j++) {
         const int at = __ldg(slot + t * lds + j);
         if (at < 0 || at >= rows) continue;
         T *dst = xs + at * ldxs;
+        if (ANY) {
+            const Cut<T> cut(dst, width);
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int v = v0 + (u << log);
-            if (v < nv) store_pack<T, N>(dst + (int64_t)v * N, p[u]);
+            for (int u = 0; u < U; u++) {
+                const int v = v0 + (u << log);
+                if (cut.is_whole(v)) p[u] = load_any<T>(src + cut.begin(v), all);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int v = v0 + (u << log);
+                if (cut.is_whole(v)) store_pack<T, E>(dst + cut.begin(v), p[u]);
+                else
+                    for (int i = cut.begin(v); i < cut.end(v); i++) dst[i] = __ldg(src + i);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int v = v0 + (u << log);
+                if (v * E < width) store_pack<T, E>(dst + v * E, p[u]);
+            }
         }
     }
 }
@@ -198,75 +220,84 @@ __global__ void __launch_bounds__(kRowThreads)
 
 // out[t] = sum over j of weight[t, j] y[slot[t, j]] + beta out[t], in 32 bits in the order of j, rounded once.  Eight rows of y
 // are requested at a time, 16 bytes of each by a thread: 128 bytes in flight at 64 registers.  (12,001 tokens of 6 rows of 2048
-// fp16: four rows of 64 bytes at 138 registers, one block per SM, 94 us; so COMBINE_US us.)
-constexpr __host__ __device__ int combine_unroll(int bytes) { return bytes >= 16 ? 1 : bytes >= 8 ? 2 : 4; }
-constexpr int kCombineAhead = 8;
+// fp16: four rows of 64 bytes at 138 registers, one block per SM, 94 us; so 65 us.)  ANY, rows that begin on no 16-byte
+// boundary: four rows at a time, since each takes two loads.
+constexpr int kCombineAhead = 8, kCombineAheadAny = 4;
 
-template <typename T, int N, int U>
-__global__ void __launch_bounds__(kRowThreads, N * sizeof(T) == 16 ? 4 : 3)
-    combine_kernel(int tokens, int k, int nv, const T *__restrict__ y, int64_t ldy, int64_t rows, const int *__restrict__ slot,
-                   int64_t lds, const float *__restrict__ weight, int64_t ldw, float beta, T *__restrict__ out, int64_t ldo,
-                   int log) {
+template <typename T, bool ANY>
+__global__ void __launch_bounds__(kRowThreads, 4)
+    combine_kernel(int tokens, int k, int width, const T *__restrict__ y, int64_t ldy, Window all, int64_t rows,
+                   const int *__restrict__ slot, int64_t lds, const float *__restrict__ weight, int64_t ldw, float beta,
+                   T *__restrict__ out, int64_t ldo, int log) {
+    constexpr int E = 16 / sizeof(T), A = ANY ? kCombineAheadAny : kCombineAhead;
     const int64_t t = (int64_t)blockIdx.x * (kRowThreads >> log) + (threadIdx.x >> log);
     if (t >= tokens) return;
-    const int v0 = (int)(blockIdx.y * (U << log) + (threadIdx.x & ((1 << log) - 1)));
-    float acc[U][N] = {};
-    for (int j0 = 0; j0 < k; j0 += kCombineAhead) {
-        Pack<T, N> p[kCombineAhead][U];
-        int at[kCombineAhead];
+    const int v = (int)((blockIdx.y << log) + (threadIdx.x & ((1 << log) - 1)));
+    T *dst = out + t * ldo;
+    const Cut<T> cut(dst, width);
+    const int *places = slot + t * lds;
+    if (ANY && !cut.is_whole(v)) {
+        for (int i = cut.begin(v); i < cut.end(v); i++) {
+            float acc = 0.f;
+            for (int j = 0; j < k; j++) {
+                const int at = __ldg(places + j);
+                if (at >= 0 && at < rows) acc = fmaf(weight ? __ldg(weight + t * ldw + j) : 1.f, to_float(__ldg(y + at * ldy + i)), acc);
+            }
+            dst[i] = from_float<T>(beta != 0.f ? fmaf(beta, to_float(dst[i]), acc) : acc);
+        }
+        return;
+    }
+    const int from = ANY ? cut.begin(v) : v * E;
+    if (from >= width) return;
+    float acc[E] = {};
+    for (int j0 = 0; j0 < k; j0 += A) {
+        Pack<T, E> p[A];
+        int at[A];
 #pragma unroll
-        for (int j = 0; j < kCombineAhead; j++) {
-            at[j] = j0 + j < k ? __ldg(slot + t * lds + j0 + j) : -1;
+        for (int j = 0; j < A; j++) {
+            at[j] = j0 + j < k ? __ldg(places + j0 + j) : -1;
             if (at[j] >= rows) at[j] = -1;
         }
 #pragma unroll
-        for (int j = 0; j < kCombineAhead; j++)
+        for (int j = 0; j < A; j++)
+            if (at[j] >= 0) p[j] = ANY ? load_any<T>(y + at[j] * ldy + from, all) : load_pack<T, E>(y + at[j] * ldy + from);
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int v = v0 + (u << log);
-                if (at[j] >= 0 && v < nv) p[j][u] = load_pack<T, N>(y + at[j] * ldy + (int64_t)v * N);
-            }
-#pragma unroll
-        for (int j = 0; j < kCombineAhead; j++) {
+        for (int j = 0; j < A; j++) {
             if (at[j] < 0) continue;
             const float w = weight ? __ldg(weight + t * ldw + j0 + j) : 1.f;
+            float f[E];
+            unpack<T, E>(p[j], f);
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                float f[N];
-                unpack<T, N>(p[j][u], f);
-#pragma unroll
-                for (int i = 0; i < N; i++) acc[u][i] = fmaf(w, f[i], acc[u][i]);
-            }
+            for (int i = 0; i < E; i++) acc[i] = fmaf(w, f[i], acc[i]);
         }
     }
+    dst += from;
+    if (beta != 0.f) {
+        float f[E];
+        unpack<T, E>(load_pack<T, E, true>(dst), f);
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int v = v0 + (u << log);
-        if (v >= nv) continue;
-        T *dst = out + t * ldo + (int64_t)v * N;
-        if (beta != 0.f) {
-            float f[N];
-            unpack<T, N>(load_pack<T, N, true>(dst), f);
-#pragma unroll
-            for (int i = 0; i < N; i++) acc[u][i] = fmaf(beta, f[i], acc[u][i]);
-        }
-        store_pack<T, N>(dst, pack<T, N>(acc[u]));
+        for (int i = 0; i < E; i++) acc[i] = fmaf(beta, f[i], acc[i]);
     }
+    store_pack<T, E>(dst, pack<T, E>(acc));
 }
 
 // dy[slot[t, j]] = weight[t, j] dout[t] and dweight[t, j] = <dout[t], y[slot[t, j]]>.  A group of threads of one block has the
 // whole row of a token, so that the inner products end in it: lanes, then warps, in a fixed order.  Eight rows at a time,
-// as above; their eight inner products are added up over a warp together, each step halving what a lane holds.
-template <typename T, int N>
-__global__ void __launch_bounds__(kRowThreads, N * sizeof(T) == 16 ? 3 : 2)
-    combine_grad_kernel(int tokens, int k, int nv, const T *__restrict__ dout, int64_t ldo, const T *__restrict__ y, int64_t ldy,
-                        int64_t rows, const int *__restrict__ slot, int64_t lds, const float *__restrict__ weight, int64_t ldw,
-                        T *__restrict__ dy, int64_t lddy, float *__restrict__ dweight, int64_t lddw, int log) {
+// as above; their eight inner products are added up over a warp together, each step halving what a lane holds.  (12,001
+// tokens of 6 rows of 2048 fp16: four rows at a time 143 us, so 119 us; two blocks per SM instead of three 151 us.)  ANY: each
+// row of dy is cut at the boundaries of its memory, and the rows of dout and y read at the shifts that they have to it.
+template <typename T, bool ANY>
+__global__ void __launch_bounds__(kRowThreads, 3)
+    combine_grad_kernel(int tokens, int k, int width, const T *__restrict__ dout, int64_t ldo, Window all_dout,
+                        const T *__restrict__ y, int64_t ldy, Window all_y, int64_t rows, const int *__restrict__ slot, int64_t lds,
+                        const float *__restrict__ weight, int64_t ldw, T *__restrict__ dy, int64_t lddy,
+                        float *__restrict__ dweight, int64_t lddw, int pieces, int log) {
     __shared__ float s_dot[kRowThreads / 32][kCombineAhead];
+    constexpr int E = 16 / sizeof(T);
     const int64_t t = (int64_t)blockIdx.x * (kRowThreads >> log) + (threadIdx.x >> log);
     const bool mine = t < tokens;  // a block's threads stay together for the barriers
     const int group = 1 << log, me = threadIdx.x & (group - 1), lane = threadIdx.x & 31;
-    constexpr int U = combine_unroll(N * sizeof(T));
+    const T *d_row = dout + t * ldo;
     for (int j0 = 0; j0 < k; j0 += kCombineAhead) {
         int at[kCombineAhead];
         float dot[kCombineAhead] = {};
@@ -275,32 +306,54 @@ __global__ void __launch_bounds__(kRowThreads, N * sizeof(T) == 16 ? 3 : 2)
             at[j] = mine && j0 + j < k ? __ldg(slot + t * lds + j0 + j) : -1;
             if (at[j] >= rows) at[j] = -1;
         }
-        for (int v0 = me; mine && v0 < nv; v0 += group * U) {
-            Pack<T, N> d[U], p[kCombineAhead][U];
+        for (int v = me; mine && v < pieces; v += group) {
+            if (ANY) {
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (v0 + u * group < nv) d[u] = load_pack<T, N>(dout + t * ldo + (int64_t)(v0 + u * group) * N);
+                for (int j = 0; j < kCombineAhead; j++) {
+                    if (at[j] < 0) continue;
+                    const float w = weight ? __ldg(weight + t * ldw + j0 + j) : 1.f;
+                    const T *y_row = y + at[j] * ldy;
+                    T *dst = dy + at[j] * lddy;
+                    const Cut<T> cut(dst, width);
+                    const int from = cut.begin(v);
+                    if (cut.is_whole(v)) {
+                        float f[E], g[E];
+                        unpack<T, E>(load_any<T>(d_row + from, all_dout), f);
+                        unpack<T, E>(load_any<T>(y_row + from, all_y), g);
 #pragma unroll
-            for (int j = 0; j < kCombineAhead; j++)
+                        for (int i = 0; i < E; i++) {
+                            dot[j] = fmaf(f[i], g[i], dot[j]);
+                            f[i] *= w;
+                        }
+                        store_pack<T, E>(dst + from, pack<T, E>(f));
+                    } else {
+                        for (int i = from; i < cut.end(v); i++) {
+                            const float f = to_float(__ldg(d_row + i));
+                            dot[j] = fmaf(f, to_float(__ldg(y_row + i)), dot[j]);
+                            dst[i] = from_float<T>(w * f);
+                        }
+                    }
+                }
+            } else {
+                const int from = v * E;
+                const Pack<T, E> d = load_pack<T, E>(d_row + from);
+                Pack<T, E> p[kCombineAhead];
 #pragma unroll
-                for (int u = 0; u < U; u++)
-                    if (at[j] >= 0 && v0 + u * group < nv) p[j][u] = load_pack<T, N>(y + at[j] * ldy + (int64_t)(v0 + u * group) * N);
+                for (int j = 0; j < kCombineAhead; j++)
+                    if (at[j] >= 0) p[j] = load_pack<T, E>(y + at[j] * ldy + from);
 #pragma unroll
-            for (int j = 0; j < kCombineAhead; j++) {
-                if (at[j] < 0) continue;
-                const float w = weight ? __ldg(weight + t * ldw + j0 + j) : 1.f;
+                for (int j = 0; j < kCombineAhead; j++) {
+                    if (at[j] < 0) continue;
+                    const float w = weight ? __ldg(weight + t * ldw + j0 + j) : 1.f;
+                    float f[E], g[E];
+                    unpack<T, E>(d, f);
+                    unpack<T, E>(p[j], g);
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    if (v0 + u * group >= nv) continue;
-                    float f[N], g[N];
-                    unpack<T, N>(d[u], f);
-                    unpack<T, N>(p[j][u], g);
-#pragma unroll
-                    for (int i = 0; i < N; i++) {
+                    for (int i = 0; i < E; i++) {
                         dot[j] = fmaf(f[i], g[i], dot[j]);
                         f[i] *= w;
                     }
-                    store_pack<T, N>(dy + at[j] * lddy + (int64_t)(v0 + u * group) * N, pack<T, N>(f));
+                    store_pack<T, E>(dy + at[j] * lddy + from, pack<T, E>(f));
                 }
             }
         }
@@ -407,16 +460,15 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_dispatch(alphasparse_cud
                                                                                       {xs, rows, width, ldxs, eb, true}});
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     const int vb = vector_bytes(eb, {address(x), (uint64_t)ldx * eb, address(xs), (uint64_t)ldxs * eb, (uint64_t)width * eb});
-    const int64_t nv = width * (int64_t)eb / vb;
-    const RowShape shape = row_shape(tokens, nv, in_flight(vb));
+    const bool any = vb < 16;
+    const RowShape shape = row_shape(tokens, any ? most_pieces(width, eb) : width * (int64_t)eb / 16, 4);
+    const Window all = window(x, tokens, width, ldx, eb);
     cudaStream_t st = current_stream();
     const auto run = [&](auto t) {
         using T = decltype(t);
-        with_pack<T>(vb, [&](auto n) {
-            constexpr int N = decltype(n)::value;
-            const auto kernel = shape.unroll == 1 ? dispatch_kernel<T, N, 1> : dispatch_kernel<T, N, in_flight(N * sizeof(T))>;
-            kernel<<<shape.grid, kRowThreads, 0, st>>>((int)tokens, (int)k, (int)nv, (const T *)x, ldx, slot, lds, rows, (T *)xs, ldxs, shape.log);
-        });
+        const auto kernel = any ? (shape.unroll == 1 ? dispatch_kernel<T, 1, true> : dispatch_kernel<T, 4, true>)
+                                : (shape.unroll == 1 ? dispatch_kernel<T, 1, false> : dispatch_kernel<T, 4, false>);
+        kernel<<<shape.grid, kRowThreads, 0, st>>>((int)tokens, (int)k, (int)width, (const T *)x, ldx, all, slot, lds, rows, (T *)xs, ldxs, shape.log);
     };
     ASB_BY_TYPE(type, run)
     count_launch();
@@ -437,16 +489,15 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_combine(alphasparse_cuda
                                                                                      {out, tokens, width, ldo, eb, true}});
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     const int vb = vector_bytes(eb, {address(y), (uint64_t)ldy * eb, address(out), (uint64_t)ldo * eb, (uint64_t)width * eb});
-    const int64_t nv = width * (int64_t)eb / vb;
-    const RowShape shape = row_shape(tokens, nv, combine_unroll(vb));
+    const bool any = vb < 16;
+    const RowShape shape = row_shape(tokens, any ? most_pieces(width, eb) : width * (int64_t)eb / 16, 1);
+    const Window all = window(y, rows, width, ldy, eb);
     cudaStream_t st = current_stream();
     const auto run = [&](auto t) {
         using T = decltype(t);
-        with_pack<T>(vb, [&](auto n) {
-            constexpr int N = decltype(n)::value;
-            const auto kernel = shape.unroll == 1 ? combine_kernel<T, N, 1> : combine_kernel<T, N, combine_unroll(N * sizeof(T))>;
-            kernel<<<shape.grid, kRowThreads, 0, st>>>((int)tokens, (int)k, (int)nv, (const T *)y, ldy, rows, slot, lds, weight, ldw, beta, (T *)out, ldo, shape.log);
-        });
+        const auto kernel = any ? combine_kernel<T, true> : combine_kernel<T, false>;
+        kernel<<<shape.grid, kRowThreads, 0, st>>>((int)tokens, (int)k, (int)width, (const T *)y, ldy, all, rows, slot, lds, weight, ldw, beta, (T *)out, ldo,
+                                                 shape.log);
     };
     ASB_BY_TYPE(type, run)
     count_launch();
@@ -472,18 +523,18 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_combine_grad(alphasparse
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     const int vb = vector_bytes(eb, {address(dout), (uint64_t)ldo * eb, address(y), (uint64_t)ldy * eb, address(dy),
                                      (uint64_t)lddy * eb, (uint64_t)width * eb});
-    const int64_t nv = width * (int64_t)eb / vb;
+    const bool any = vb < 16;
+    const int64_t pieces = any ? most_pieces(width, eb) : width * (int64_t)eb / 16;
     int log = 0;
-    while ((1 << log) < kRowThreads && (int64_t)1 << log < nv) log++;
+    while ((1 << log) < kRowThreads && (int64_t)1 << log < pieces) log++;
     const unsigned blocks = (unsigned)((tokens + (kRowThreads >> log) - 1) / (kRowThreads >> log));
+    const Window all_dout = window(dout, tokens, width, ldo, eb), all_y = window(y, rows, width, ldy, eb);
     cudaStream_t st = current_stream();
     const auto run = [&](auto t) {
         using T = decltype(t);
-        with_pack<T>(vb, [&](auto n) {
-            constexpr int N = decltype(n)::value;
-            combine_grad_kernel<T, N><<<blocks, kRowThreads, 0, st>>>((int)tokens, (int)k, (int)nv, (const T *)dout, ldo, (const T *)y, ldy, rows,
-                                                                   slot, lds, weight, ldw, (T *)dy, lddy, dweight, lddw, log);
-        });
+        const auto kernel = any ? combine_grad_kernel<T, true> : combine_grad_kernel<T, false>;
+        kernel<<<blocks, kRowThreads, 0, st>>>((int)tokens, (int)k, (int)width, (const T *)dout, ldo, all_dout, (const T *)y, ldy, all_y, rows, slot, lds, weight,
+                                             ldw, (T *)dy, lddy, dweight, lddw, (int)pieces, log);
     };
     ASB_BY_TYPE(type, run)
     count_launch();

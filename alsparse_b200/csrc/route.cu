@@ -242,7 +242,7 @@ __device__ __forceinline__ void sort_keys(unsigned long long (&key)[I]) {
 // 32-bit keys, up to eight a lane: each lane sorts its own (order above, the complement of the index below, so that equal
 // keys go by index) and leaves them in shared memory; the highest head is taken k times, its lane reads its next.  Bound by
 // instructions.  (256 experts in 8 groups, 8 of them, 32,768 tokens: the plain way 104 us, sorted keys moved up in
-// registers 55 us, so ROUTE_US us.)
+// registers 55 us, so 47 us.)
 template <int I, bool BIAS>
 __device__ __forceinline__ bool choose_sorted(const RouteShape &sh, const float (&x)[I], const float *bias, float top, float sum,
                                               double *s_space, int *choice, float *logit) {

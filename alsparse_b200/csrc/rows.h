@@ -116,6 +116,58 @@ __device__ __forceinline__ Pack<T, N> pack(const float (&f)[N]) {
     return r;
 }
 
+// ---- rows that begin on no 16-byte boundary ------------------------------------------------------
+
+// The memory of an operand: aligned loads around one of its rows do not reach out of it.
+struct Window {
+    const char *lo, *hi;
+};
+
+// 16 bytes of elements from an address that is only aligned to the element: the two aligned vectors that hold them, shifted
+// together; element by element where those reach out of the operand.
+template <typename T>
+__device__ __forceinline__ Pack<T, 16 / sizeof(T)> load_any(const T *p, const Window &w) {
+    constexpr int E = 16 / sizeof(T);
+    const char *at = reinterpret_cast<const char *>(p);
+    const unsigned shift = (unsigned)(reinterpret_cast<uintptr_t>(at) & 15);
+    const char *a = at - shift;
+    if (shift == 0) return load_pack<T, E>(p);
+    Pack<T, E> r;
+    if (a >= w.lo && a + 32 <= w.hi) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(a)), y = __ldg(reinterpret_cast<const uint4 *>(a) + 1);
+        unsigned c[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 6; i++) c[i] = shift & 8 ? c[i + 2] : c[i];
+#pragma unroll
+        for (int i = 0; i < 5; i++) c[i] = shift & 4 ? c[i + 1] : c[i];
+#pragma unroll
+        for (int i = 0; i < 4; i++) r.w[i] = sizeof(T) == 4 ? c[i] : __funnelshift_r(c[i], c[i + 1], (shift & 2) * 8);
+    } else {
+        float f[E];
+#pragma unroll
+        for (int i = 0; i < E; i++) f[i] = to_float(__ldg(p + i));
+        r = pack<T, E>(f);
+    }
+    return r;
+}
+
+// A row of `width` elements cut at the 16-byte boundaries of memory: piece 0 up to the first, pieces 1 .. whole of 16 bytes,
+// piece whole + 1 behind the last.
+template <typename T>
+struct Cut {
+    static constexpr int E = 16 / sizeof(T);
+    int head, whole, width;
+    __device__ __forceinline__ Cut(const T *row, int width_) : width(width_) {
+        head = min(width, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T));
+        whole = (width - head) / E;
+    }
+    __device__ __forceinline__ bool is_whole(int v) const { return v >= 1 && v <= whole; }
+    __device__ __forceinline__ int begin(int v) const { return v == 0 ? 0 : min(width, head + (v - 1) * E); }
+    __device__ __forceinline__ int end(int v) const { return v == 0 ? head : min(width, head + v * E); }  // of pieces that are not whole
+};
+// Pieces of a row, whichever way it is cut
+inline int64_t most_pieces(int64_t width, size_t elem) { return width * (int64_t)elem / 16 + 2; }
+
 // ---- launches ----------------------------------------------------------------------------------
 
 // A kernel that begins with after_previous(): its blocks may be made resident while the kernel before it on the stream ends
@@ -174,20 +226,8 @@ inline int vector_bytes(size_t elem, std::initializer_list<uint64_t> all) {
     for (uint64_t v : all) any |= v;
     return any % 16 == 0 ? 16 : any % 8 == 0 ? 8 : any % 4 == 0 ? 4 : (int)elem;
 }
-// Calls f with the number of elements of T that make `vb` bytes, as a compile-time constant
-template <typename T, typename F>
-void with_pack(int vb, F f) {
-    if (vb == 16) f(std::integral_constant<int, 16 / sizeof(T)>{});
-    else if (vb == 8) f(std::integral_constant<int, 8 / sizeof(T)>{});
-    else if (vb == 4) f(std::integral_constant<int, 4 / sizeof(T)>{});
-    else f(std::integral_constant<int, 1>{});
-}
 
 inline uint64_t address(const void *p) { return (uint64_t)reinterpret_cast<uintptr_t>(p); }
-
-// Vectors of `bytes` bytes that a thread has in flight: 64 bytes of them.  (16,383 rows of 1001 floats, 4-byte vectors: four
-// take 28.6 us, sixteen LOOKUP_RAGGED us.)
-constexpr __host__ __device__ int in_flight(int bytes) { return bytes >= 16 ? 4 : bytes >= 8 ? 8 : 16; }
 
 // A row of `nv` vectors by a group of 2^log threads, `unroll` vectors a thread and piece of the row.  Few vectors in all:
 // one a thread, so that the call is done in one round trip to memory; many: `many`, so that enough are in flight.
@@ -204,6 +244,11 @@ inline RowShape row_shape(int64_t rows, int64_t nv, int many) {
     const int64_t per_block = kRowThreads >> s.log, piece = (int64_t)s.unroll << s.log;
     s.grid = dim3((unsigned)((rows + per_block - 1) / per_block), (unsigned)((nv + piece - 1) / piece));
     return s;
+}
+
+inline Window window(const void *p, int64_t rows, int64_t width, int64_t ld, size_t elem) {
+    const char *lo = static_cast<const char *>(p);
+    return Window{lo, lo + (rows > 0 ? ((size_t)(rows - 1) * (size_t)ld + (size_t)width) * elem : 0)};
 }
 
 }  // namespace asb
