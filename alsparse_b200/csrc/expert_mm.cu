@@ -7,7 +7,8 @@
 // of 16, so an expert's rows are cut into equal tiles of at most 256 and little is multiplied for nothing.  With many rows
 // an expert two SMs work on one tile of 256 (cta_group::2), which halves what each fetches of the narrow operand.  The offsets
 // stay on the device: every block forms the same table of row tiles.
-// expert_mm_plain_kernel: 32-bit operands, and addresses or strides that TMA does not take (no multiple of 16 bytes).
+// Addresses or strides that TMA does not take (no multiple of 16 bytes) are brought by eight warps of their own instead.
+// expert_mm_plain_kernel: 32-bit operands, on the ordinary units.
 #include <cuda.h>
 #include <stdio.h>
 
@@ -146,6 +147,8 @@ __global__ void __launch_bounds__(256)
 // ---- tensor cores --------------------------------------------------------------------------------
 
 constexpr int kMmThreads = 384;  // copies, products, eight warps for the accumulators, two for the ends of ragged experts
+constexpr int kMmCopyWarps = 8;  // ANY: after the others, instead of the two for ragged ends
+constexpr int kMmThreadsAny = 320 + 32 * kMmCopyWarps;
 constexpr int kMmM = 128, kMmK = 64;
 constexpr int kMmMostStages = 8;
 constexpr unsigned long long kMmLimitNs = 2000000000ull;
@@ -353,7 +356,44 @@ struct MmShape {
     unsigned stage_bytes, instruction, acc_stride;
     bool vectors;      // rows of the output begin on 16-byte boundaries
     float beta;
+    // ANY: the operands themselves (a: the weights of all experts, or x; b: x, or dy)
+    const void *a, *b;
+    int64_t lda, ldb, stride_a;
+    Window all_a, all_b;
 };
+
+// ANY: a thread's share of an operand's part of a stage: boxes of `rows` rows of 64 elements side by side, in the order that the
+// copies of TMA leave them in (16 bytes c of row r at c ^ (r & 7)).  Only `rows_there` rows and `cols_there` columns exist; the
+// rest becomes zeros.
+template <typename T>
+__device__ __forceinline__ void copy_boxes(char *dst, const T *src, int64_t ld, const Window &all, int rows, int boxes, int rows_there,
+                                           int cols_there, int thread) {
+    constexpr int E = 16 / sizeof(T), ahead = 4;
+    const int chunks = rows * boxes * 8;
+    for (int i0 = thread; i0 < chunks; i0 += ahead * 32 * kMmCopyWarps) {
+        Pack<T, E> p[ahead];
+#pragma unroll
+        for (int u = 0; u < ahead; u++) {
+            const int i = i0 + u * 32 * kMmCopyWarps, c = i & 7, row = (i >> 3) % rows, col = (i >> 3) / rows * 64 + c * E;
+            p[u] = zero_pack<T, E>();
+            if (i < chunks && row < rows_there && col < cols_there) {
+                const T *from = src + row * ld + col;
+                if (col + E <= cols_there) p[u] = load_any<T>(from, all);
+                else {
+                    float f[E];
+#pragma unroll
+                    for (int j = 0; j < E; j++) f[j] = col + j < cols_there ? to_float(__ldg(from + j)) : 0.f;
+                    p[u] = pack<T, E>(f);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < ahead; u++) {
+            const int i = i0 + u * 32 * kMmCopyWarps, c = i & 7, row = (i >> 3) % rows, box = (i >> 3) / rows;
+            if (i < chunks) store_pack<T, E>(reinterpret_cast<T *>(dst + (box * rows + row) * 128 + ((c ^ (row & 7)) << 4)), p[u]);
+        }
+    }
+}
 
 struct MmTile {
     int expert, m0, n0, n;  // n0: first row (kRows) or column of dy; n: width of the product, a multiple of 16 (two blocks: 32)
@@ -398,8 +438,8 @@ __device__ __forceinline__ bool ragged(const MmTile &q, int k) { return q.length
 // accumulators of a block's 128 m are its own.  The copies of both report to the first block's barrier, but for the
 // last rows of an expert in kGradient: each block waits for its own and clears what does not belong to the expert (its last
 // warp), and tells the first.
-template <int FORM, bool PAIR, bool W_K, typename T, typename TO>
-__global__ void __launch_bounds__(kMmThreads, 1)
+template <int FORM, bool PAIR, bool W_K, bool ANY, typename T, typename TO>
+__global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
     expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                      const __grid_constant__ CUtensorMap map_c, const MmShape s,
                      TO *__restrict__ out, int64_t ldo, int64_t stride_o) {
@@ -420,10 +460,12 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     load_offsets(s.offsets, s.experts, s.rows, s_begin);
     if (w == 0) {
         if (lane == 0) {
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
-            if (b_k) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_c) : "memory");
-            for (int i = 0; i < s.stages; i++) barrier_init(&s_full[i], 1), barrier_init(&s_empty[i], 1), barrier_init(&s_own[i], 1), barrier_init(&s_ready[i], PAIR ? 2 : 1);
+            if (!ANY) {
+                asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+                asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+                if (b_k) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_c) : "memory");
+            }
+            for (int i = 0; i < s.stages; i++) barrier_init(&s_full[i], ANY ? kMmCopyWarps : 1), barrier_init(&s_empty[i], 1), barrier_init(&s_own[i], 1), barrier_init(&s_ready[i], PAIR ? 2 : 1);
             for (int i = 0; i < 2; i++) barrier_init(&s_acc_full[i], 1), barrier_init(&s_acc_empty[i], PAIR ? 16 : 8);
             s_stop_word = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -452,7 +494,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     if (w == 0) {
         int stage = 0;
         unsigned phase = 0;
-        bool good = true;
+        bool good = !ANY;
         for (int t = worker; good && t < tiles; t += workers) {
             const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
             const int half = PAIR ? q.n >> 1 : q.n, m0 = q.m0 + rank * kMmM, n0 = q.n0 + rank * half;
@@ -476,7 +518,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                     for (int g = 0; g < narrow; g++) copy_tile<B>(b + wide * 8192 + g * 2048, &map_c, k0, n0 + wide * 64 + g * 16, 0, barrier);
                 };
                 if (elect_one()) {
-                    if (FORM == kGradient && ragged(q, k)) {
+                    if (!ANY && FORM == kGradient && ragged(q, k)) {
                         barrier_expect(&s_own[stage], bytes);
                         copy(std::false_type{}, smem_address(&s_own[stage]));
                     } else if (PAIR) {
@@ -507,7 +549,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             for (int k = 0; k < q.steps; k++) {
                 char *a = ring + (size_t)stage * s.stage_bytes;
                 const int left = length - k * kMmK, parts = min(4, (left + 15) / 16);
-                if (FORM == kGradient && ragged(q, k)) {
+                if (!ANY && FORM == kGradient && ragged(q, k)) {
                     if (!(good = warp_wait<true>(&s_ready[stage], ready_phases >> stage & 1, s_stop))) break;
                     ready_phases ^= 1u << stage;
                 } else {
@@ -570,6 +612,35 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                     if (PAIR) arrive_at_first<false>(&s_acc_empty[slot]);
                     else barrier_arrive(&s_acc_empty[slot]);
                 }
+            }
+        }
+    } else if (ANY) {
+        const int thread = threadIdx.x - 320;
+        int stage = 0;
+        unsigned phase = 0;
+        bool good = true;
+        for (int t = worker; good && t < tiles; t += workers) {
+            const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
+            for (int k = 0; k < q.steps; k++) {
+                if (!(good = warp_wait(&s_empty[stage], phase ^ 1, s_stop))) break;
+                char *a = ring + (size_t)stage * s.stage_bytes, *b = a + a_bytes;
+                const int k0 = k * kMmK, m_there = s.m_size - q.m0;
+                const T *pa = static_cast<const T *>(s.a), *pb = static_cast<const T *>(s.b);
+                if (FORM == kGradient) {
+                    const int there = q.length - k0;
+                    copy_boxes<T>(a, pa + (int64_t)(q.lo + k0) * s.lda + q.m0, s.lda, s.all_a, kMmK, 2, there, m_there, thread);
+                    copy_boxes<T>(b, pb + (int64_t)(q.lo + k0) * s.ldb + q.n0, s.ldb, s.all_b, kMmK, (q.n + 63) >> 6, there, s.n_size - q.n0, thread);
+                } else {
+                    const int there = s.reduced - k0;
+                    pa += q.expert * s.stride_a;
+                    if (W_K) copy_boxes<T>(a, pa + (int64_t)q.m0 * s.lda + k0, s.lda, s.all_a, kMmM, 1, m_there, there, thread);
+                    else copy_boxes<T>(a, pa + (int64_t)k0 * s.lda + q.m0, s.lda, s.all_a, kMmK, 2, there, m_there, thread);
+                    copy_boxes<T>(b, pb + (int64_t)q.n0 * s.ldb + k0, s.ldb, s.all_b, q.n, 1, q.length, there, thread);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) barrier_arrive(&s_full[stage]);
+                if (++stage == s.stages) stage = 0, phase ^= 1;
             }
         }
     } else if (FORM == kGradient) {
@@ -664,7 +735,7 @@ static cudaError_t multiprocessors(int *n) {
 }
 
 // Fills what follows from the tile, and launches.
-template <int FORM, bool PAIR, bool W_K, typename T, typename TO>
+template <int FORM, bool PAIR, bool W_K, bool ANY, typename T, typename TO>
 static cudaError_t launch_mm(alphasparse_cuda_type_t type, MmShape s, int64_t most_tiles, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &c,
                              TO *out,
                              int64_t ldo, int64_t stride_o, cudaStream_t st) {
@@ -678,7 +749,7 @@ static cudaError_t launch_mm(alphasparse_cuda_type_t type, MmShape s, int64_t mo
                     (unsigned)((PAIR ? 2 * kMmM : kMmM) >> 4) << 24;
     s.acc_stride = 256;
     s.vectors = address(out) % 16 == 0 && ldo * (int64_t)sizeof(TO) % 16 == 0 && (FORM != kGradient || stride_o * (int64_t)sizeof(TO) % 16 == 0);
-    const auto kernel = expert_mm_kernel<FORM, PAIR, W_K, T, TO>;
+    const auto kernel = expert_mm_kernel<FORM, PAIR, W_K, ANY, T, TO>;
     const int smem = 1024 + s.stages * (int)s.stage_bytes;
     int sms = 0;
     cudaError_t e = multiprocessors(&sms);
@@ -689,7 +760,7 @@ static cudaError_t launch_mm(alphasparse_cuda_type_t type, MmShape s, int64_t mo
     cluster[0].val.clusterDim.x = 2, cluster[0].val.clusterDim.y = 1, cluster[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)(PAIR ? 2 * std::min<int64_t>(sms / 2, most_tiles) : std::min<int64_t>(sms, most_tiles)));
-    config.blockDim = dim3(kMmThreads);
+    config.blockDim = dim3(ANY ? kMmThreadsAny : kMmThreads);
     config.dynamicSmemBytes = (size_t)smem;
     config.stream = st;
     config.attrs = cluster;
@@ -741,30 +812,37 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_mm(alphasparse_operation
     if (status != ALPHA_SPARSE_STATUS_SUCCESS) return status;
     cudaStream_t st = current_stream();
     cudaError_t e = cudaSuccess;
-    if (eb == 2 && reduced > 0 && takes_tma(x, ldx, rows, 0, 1) && takes_tma(w, ldw, out, stride_w, experts)) {
+    if (eb == 2 && reduced > 0) {
         MmShape s{};
         s.offsets = offsets, s.experts = (int)experts, s.rows = rows, s.m_size = (int)features, s.reduced = (int)reduced;
+        const bool any = !takes_tma(x, ldx, rows, 0, 1) || !takes_tma(w, ldw, out, stride_w, experts);
         // Many rows an expert: two SMs on a tile.  Few: the weights are what has to be read, by as many SMs as there are; narrow
         // tiles leave room for more of them on their way.
         const int64_t mean = (rows + experts - 1) / experts;
-        const bool pair = mean > 64;
+        const bool pair = mean > 64 && !any;
         s.n = pair ? 256 : mean <= 16 ? 32 : mean <= 32 ? 64 : 128;
         const int m = pair ? 2 * kMmM : kMmM;
         s.m_tiles = (int)((features + m - 1) / m);
-        CUtensorMap mx, mx16, mw;
-        if (!make_map(&mx, type, x, reduced, rows, ldx, 1, 0, 64) || !make_map(&mx16, type, x, reduced, rows, ldx, 1, 0, 16) ||
-             !make_map(&mw, type, w, in, out, ldw, experts, stride_w, trans ? kMmM : kMmK)) {
+        const int64_t row_tiles = rows / s.n + std::min(experts, rows), tiles = row_tiles * s.m_tiles;
+        if (tiles > 0x7fffffff - 4096) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+        CUtensorMap mx{}, mx16{}, mw{};
+        if (any) {
+            s.a = w, s.lda = ldw, s.stride_a = stride_w, s.b = x, s.ldb = ldx;
+            s.all_a = window(w, 1, (experts - 1) * stride_w + (out - 1) * ldw + in, 0, eb);
+            s.all_b = window(x, rows, reduced, ldx, eb);
+        } else if (!make_map(&mx, type, x, reduced, rows, ldx, 1, 0, 64) || !make_map(&mx16, type, x, reduced, rows, ldx, 1, 0, 16) ||
+                   !make_map(&mw, type, w, in, out, ldw, experts, stride_w, trans ? kMmM : kMmK)) {
             record_error("alphasparse_cuda_expert_mm: no tensor map");
             return ALPHA_SPARSE_STATUS_EXECUTION_FAILED;
         }
-        const int64_t row_tiles = rows / s.n + std::min(experts, rows), tiles = row_tiles * s.m_tiles;
-        if (tiles > 0x7fffffff - 4096) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
         const auto go = [&](auto t) {
             using T = decltype(t);
-            if (pair && trans) e = launch_mm<kRows, true, true, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
-            else if (pair) e = launch_mm<kRows, true, false, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
-            else if (trans) e = launch_mm<kRows, false, true, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
-            else e = launch_mm<kRows, false, false, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
+            if (any && trans) e = launch_mm<kRows, false, true, true, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
+            else if (any) e = launch_mm<kRows, false, false, true, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
+            else if (pair && trans) e = launch_mm<kRows, true, true, false, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
+            else if (pair) e = launch_mm<kRows, true, false, false, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
+            else if (trans) e = launch_mm<kRows, false, true, false, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
+            else e = launch_mm<kRows, false, false, false, T, T>(type, s, tiles, mw, mx, mx16, (T *)y, ldy, 0, st);
         };
         if (type == ALPHA_SPARSE_CUDA_TYPE_F16) go(__half());
         else go(__nv_bfloat16());
@@ -803,23 +881,33 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_mm_grad(alphasparse_cuda
     if (status != ALPHA_SPARSE_STATUS_SUCCESS) return status;
     cudaStream_t st = current_stream();
     cudaError_t e = cudaSuccess;
-    if (eb == 2 && rows > 0 && takes_tma(dy, lddy, rows, 0, 1) && takes_tma(x, ldx, rows, 0, 1)) {
+    if (eb == 2 && rows > 0) {
         MmShape s{};
         s.offsets = offsets, s.experts = (int)experts, s.rows = rows, s.m_size = (int)in, s.n_size = (int)out, s.beta = beta;
-        s.m_tiles = (int)((in + 2 * kMmM - 1) / (2 * kMmM));
-        s.n_tiles = (int)((out + 255) / 256);
-        s.n = (int)up_to((out + s.n_tiles - 1) / s.n_tiles, 32);  // equal tiles of at most 256 columns of dy
-        CUtensorMap my, mx;
-        if (!make_map(&my, type, dy, out, rows, lddy, 1, 0, kMmK) || !make_map(&mx, type, x, in, rows, ldx, 1, 0, kMmK)) {
+        const bool any = !takes_tma(dy, lddy, rows, 0, 1) || !takes_tma(x, ldx, rows, 0, 1);
+        const int64_t m = any ? kMmM : 2 * kMmM, n = any ? 128 : 256;
+        s.m_tiles = (int)((in + m - 1) / m);
+        s.n_tiles = (int)((out + n - 1) / n);
+        s.n = (int)up_to((out + s.n_tiles - 1) / s.n_tiles, any ? 16 : 32);  // equal tiles of the columns of dy
+        const int64_t tiles = experts * s.m_tiles * s.n_tiles;
+        if (tiles > 0x7fffffff - 4096) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+        CUtensorMap my{}, mx{};
+        if (any) {
+            s.a = x, s.lda = ldx, s.b = dy, s.ldb = lddy;
+            s.all_a = window(x, rows, in, ldx, eb), s.all_b = window(dy, rows, out, lddy, eb);
+        } else if (!make_map(&my, type, dy, out, rows, lddy, 1, 0, kMmK) || !make_map(&mx, type, x, in, rows, ldx, 1, 0, kMmK)) {
             record_error("alphasparse_cuda_expert_mm_grad: no tensor map");
             return ALPHA_SPARSE_STATUS_EXECUTION_FAILED;
         }
-        const int64_t tiles = experts * s.m_tiles * s.n_tiles;
-        if (tiles > 0x7fffffff - 4096) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
         const auto go = [&](auto t) {
             using T = decltype(t);
-            if (weight_type == ALPHA_SPARSE_CUDA_TYPE_F32) e = launch_mm<kGradient, true, false, T, float>(type, s, tiles, mx, my, my, (float *)dw, ldw, stride_w, st);
-            else e = launch_mm<kGradient, true, false, T, T>(type, s, tiles, mx, my, my, (T *)dw, ldw, stride_w, st);
+            const auto with_output = [&](auto o) {
+                using TO = decltype(o);
+                if (any) e = launch_mm<kGradient, false, false, true, T, TO>(type, s, tiles, mx, my, my, (TO *)dw, ldw, stride_w, st);
+                else e = launch_mm<kGradient, true, false, false, T, TO>(type, s, tiles, mx, my, my, (TO *)dw, ldw, stride_w, st);
+            };
+            if (weight_type == ALPHA_SPARSE_CUDA_TYPE_F32) with_output((float)0);
+            else with_output(t);
         };
         if (type == ALPHA_SPARSE_CUDA_TYPE_F16) go(__half());
         else go(__nv_bfloat16());

@@ -84,9 +84,9 @@ def test_gradient(dtype, out_type, out, inner, counts, rows):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("op", [T, N])
-@pytest.mark.parametrize("out,inner", [(1, 1), (7, 33), (65, 130), (100, 63)])
+@pytest.mark.parametrize("out,inner", [(1, 1), (7, 33), (65, 130), (100, 63), (301, 1155)])
 def test_odd_sizes_and_32_bits(dtype, op, out, inner):
-    """Rows that begin on no 16-byte boundary, and 32-bit elements: without tensor cores."""
+    """Rows that begin on no 16-byte boundary, and 32-bit elements."""
     g = gen(out)
     counts = [70, 0, 3, 1, 130]
     w = normal(g, 5, out, inner, dtype=dtype)
