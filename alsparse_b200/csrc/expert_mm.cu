@@ -7,7 +7,7 @@
 // of 16, so an expert's rows are cut into equal tiles of at most 256 and little is multiplied for nothing.  With many rows
 // an expert two SMs work on one tile of 256 (cta_group::2), which halves what each fetches of the narrow operand.  The offsets
 // stay on the device: every block forms the same table of row tiles.
-// Addresses or strides that TMA does not take (no multiple of 16 bytes) are brought by eight warps of their own instead.
+// Addresses or strides that TMA does not take (no multiple of 16 bytes) are brought by fourteen warps of their own instead.
 // expert_mm_plain_kernel: 32-bit operands, on the ordinary units.
 #include <cuda.h>
 #include <stdio.h>
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(256)
 // ---- tensor cores --------------------------------------------------------------------------------
 
 constexpr int kMmThreads = 384;  // copies, products, eight warps for the accumulators, two for the ends of ragged experts
-constexpr int kMmCopyWarps = 8;  // ANY: after the others, instead of the two for ragged ends
+constexpr int kMmCopyWarps = 14;  // ANY: after the others, instead of the two for ragged ends
 constexpr int kMmThreadsAny = 320 + 32 * kMmCopyWarps;
 constexpr int kMmM = 128, kMmK = 64;
 constexpr int kMmMostStages = 8;
@@ -362,35 +362,81 @@ struct MmShape {
     Window all_a, all_b;
 };
 
-// ANY: a thread's share of an operand's part of a stage: boxes of `rows` rows of 64 elements side by side, in the order that the
-// copies of TMA leave them in (16 bytes c of row r at c ^ (r & 7)).  Only `rows_there` rows and `cols_there` columns exist; the
-// rest becomes zeros.
+__device__ __forceinline__ uint4 load_if(const char *p, bool there) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    asm("{\n.reg .pred p;\nsetp.ne.b32 p, %5, 0;\n@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n}"
+        : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+        : "l"(p), "r"((unsigned)there));
+    return v;
+}
+
+// load_any in two parts: the two aligned vectors are requested without a branch, so that several are on their way at once, and
+// shifted together when they are needed.  `there` false: zeros.  (32,768 x 1001 x 1439, 16 experts: 1346 us with load_any and eight warps, 876 us
+// so, 834 us with fourteen.  The kernels on rows, which have more blocks to hide latency, lose by the registers: lookup of odd rows 42 -> 61 us.)
 template <typename T>
-__device__ __forceinline__ void copy_boxes(char *dst, const T *src, int64_t ld, const Window &all, int rows, int boxes, int rows_there,
+struct AnyPack {
+    static constexpr int E = 16 / sizeof(T);
+    uint4 x, y;
+    const T *p;
+    bool apart;
+    __device__ __forceinline__ AnyPack() {}
+    __device__ __forceinline__ AnyPack(const T *p_, const Window &w, bool there) : p(p_) {
+        const char *at = reinterpret_cast<const char *>(p);
+        const unsigned shift = (unsigned)(reinterpret_cast<uintptr_t>(at) & 15);
+        const char *a = at - shift;
+        const bool inside = shift == 0 || (a >= w.lo && a + 32 <= w.hi);
+        x = load_if(a, there && inside);
+        y = load_if(a + 16, there && inside && shift != 0);
+        apart = there && !inside;
+    }
+    __device__ __forceinline__ Pack<T, E> get() const {
+        Pack<T, E> r;
+        if (apart) {
+            float f[E];
+#pragma unroll
+            for (int i = 0; i < E; i++) f[i] = to_float(__ldg(p + i));
+            return pack<T, E>(f);
+        }
+        const unsigned shift = (unsigned)(reinterpret_cast<uintptr_t>(p) & 15);
+        unsigned c[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 6; i++) c[i] = shift & 8 ? c[i + 2] : c[i];
+#pragma unroll
+        for (int i = 0; i < 5; i++) c[i] = shift & 4 ? c[i + 1] : c[i];
+#pragma unroll
+        for (int i = 0; i < 4; i++) r.w[i] = sizeof(T) == 4 ? c[i] : __funnelshift_r(c[i], c[i + 1], (shift & 2) * 8);
+        return r;
+    }
+};
+
+// ANY: a thread's share of an operand's part of a stage, in the order that the copies of TMA leave it in (16 bytes c of a row of
+// 128 bytes at c ^ (row & 7)).  K_MAJOR: one box of `extent` rows; else boxes of 64 rows side by side, `extent` columns wide.  Only
+// `rows_there` rows and `cols_there` columns exist; the rest becomes zeros.
+template <typename T, bool K_MAJOR>
+__device__ __forceinline__ void copy_boxes(char *dst, const T *src, int64_t ld, const Window &all, int extent, int rows_there,
                                            int cols_there, int thread) {
-    constexpr int E = 16 / sizeof(T), ahead = 4;
-    const int chunks = rows * boxes * 8;
+    constexpr int E = 16 / sizeof(T), ahead = 3;  // chunks a thread has on their way
+    const int chunks = K_MAJOR ? extent * 8 : (extent + 63) / 64 * 512;
     for (int i0 = thread; i0 < chunks; i0 += ahead * 32 * kMmCopyWarps) {
-        Pack<T, E> p[ahead];
+        AnyPack<T> p[ahead];
 #pragma unroll
         for (int u = 0; u < ahead; u++) {
-            const int i = i0 + u * 32 * kMmCopyWarps, c = i & 7, row = (i >> 3) % rows, col = (i >> 3) / rows * 64 + c * E;
-            p[u] = zero_pack<T, E>();
-            if (i < chunks && row < rows_there && col < cols_there) {
-                const T *from = src + row * ld + col;
-                if (col + E <= cols_there) p[u] = load_any<T>(from, all);
-                else {
-                    float f[E];
-#pragma unroll
-                    for (int j = 0; j < E; j++) f[j] = col + j < cols_there ? to_float(__ldg(from + j)) : 0.f;
-                    p[u] = pack<T, E>(f);
-                }
-            }
+            const int i = i0 + u * 32 * kMmCopyWarps, row = K_MAJOR ? i >> 3 : i >> 3 & 63, col = (K_MAJOR ? 0 : i >> 9) * 64 + (i & 7) * E;
+            p[u] = AnyPack<T>(src + row * ld + col, all, i < chunks && row < rows_there && col + E <= cols_there);
         }
 #pragma unroll
         for (int u = 0; u < ahead; u++) {
-            const int i = i0 + u * 32 * kMmCopyWarps, c = i & 7, row = (i >> 3) % rows, box = (i >> 3) / rows;
-            if (i < chunks) store_pack<T, E>(reinterpret_cast<T *>(dst + (box * rows + row) * 128 + ((c ^ (row & 7)) << 4)), p[u]);
+            const int i = i0 + u * 32 * kMmCopyWarps, row = K_MAJOR ? i >> 3 : i >> 3 & 63, col = (K_MAJOR ? 0 : i >> 9) * 64 + (i & 7) * E;
+            if (i >= chunks) break;
+            Pack<T, E> v = p[u].get();
+            if (row < rows_there && col < cols_there && col + E > cols_there) {
+                float f[E];
+#pragma unroll
+                for (int j = 0; j < E; j++) f[j] = col + j < cols_there ? to_float(__ldg(src + row * ld + col + j)) : 0.f;
+                v = pack<T, E>(f);
+            }
+            // rows of all boxes are 128 bytes apart
+            store_pack<T, E>(reinterpret_cast<T *>(dst + (i >> 3) * 128 + (((i & 7) ^ (i >> 3 & 7)) << 4)), v);
         }
     }
 }
@@ -628,14 +674,14 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
                 const T *pa = static_cast<const T *>(s.a), *pb = static_cast<const T *>(s.b);
                 if (FORM == kGradient) {
                     const int there = q.length - k0;
-                    copy_boxes<T>(a, pa + (int64_t)(q.lo + k0) * s.lda + q.m0, s.lda, s.all_a, kMmK, 2, there, m_there, thread);
-                    copy_boxes<T>(b, pb + (int64_t)(q.lo + k0) * s.ldb + q.n0, s.ldb, s.all_b, kMmK, (q.n + 63) >> 6, there, s.n_size - q.n0, thread);
+                    copy_boxes<T, false>(a, pa + (int64_t)(q.lo + k0) * s.lda + q.m0, s.lda, s.all_a, kMmM, there, m_there, thread);
+                    copy_boxes<T, false>(b, pb + (int64_t)(q.lo + k0) * s.ldb + q.n0, s.ldb, s.all_b, q.n, there, s.n_size - q.n0, thread);
                 } else {
                     const int there = s.reduced - k0;
                     pa += q.expert * s.stride_a;
-                    if (W_K) copy_boxes<T>(a, pa + (int64_t)q.m0 * s.lda + k0, s.lda, s.all_a, kMmM, 1, m_there, there, thread);
-                    else copy_boxes<T>(a, pa + (int64_t)k0 * s.lda + q.m0, s.lda, s.all_a, kMmK, 2, there, m_there, thread);
-                    copy_boxes<T>(b, pb + (int64_t)q.n0 * s.ldb + k0, s.ldb, s.all_b, q.n, 1, q.length, there, thread);
+                    if (W_K) copy_boxes<T, true>(a, pa + (int64_t)q.m0 * s.lda + k0, s.lda, s.all_a, kMmM, m_there, there, thread);
+                    else copy_boxes<T, false>(a, pa + (int64_t)k0 * s.lda + q.m0, s.lda, s.all_a, kMmM, there, m_there, thread);
+                    copy_boxes<T, true>(b, pb + (int64_t)q.n0 * s.ldb + k0, s.ldb, s.all_b, q.n, q.length, there, thread);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
