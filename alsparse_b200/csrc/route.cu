@@ -12,6 +12,7 @@
 namespace asb {
 
 constexpr int kRouteWarps = 4;
+constexpr int kSortedItems = 8;  // logits a lane that it sorts; more: the largest one by one (512 experts, 8 of them: sorted 87 us, so 59 us)
 constexpr unsigned kAll = 0xffffffffu;
 
 // Keys as unsigned numbers of the same order.  0 stands for an expert that cannot be chosen (a logit or key of minus
@@ -134,6 +135,14 @@ __device__ __forceinline__ unsigned best_groups(const RouteShape &sh, const F *s
 // some eight units of it in all) and of the sum with the bias: two that are further apart than this stand as they do in 64.
 __device__ __forceinline__ bool apart(float a, float b) { return a - b > 4e-6f * (1.f + fabsf(b)); }
 
+// The score of a key: in 32 bits by the fast functions, since what they may get wrong is decided again
+__device__ __forceinline__ float key_score(const RouteShape &sh, float x, float top, float sum) {
+    return sh.sigmoid ? __fdividef(1.f, 1.f + __expf(-x)) : __fdividef(__expf(x - top), sum);
+}
+__device__ __forceinline__ double key_score(const RouteShape &sh, double x, double top, double sum) {
+    return sh.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - top) / sum;
+}
+
 // Experts of one token by keys of type F, in a warp; lane j gets the j-th choice, -1 where nothing is left.  The plain way: the
 // largest key that is left, k times.  Returns false when 32-bit keys do not decide it.
 template <typename F, int I, bool BIAS>
@@ -150,7 +159,7 @@ __device__ __forceinline__ bool choose(const RouteShape &sh, const float (&x)[I]
         const int e = lane * I + i;
         F v = (F)x[i];
         if (BIAS && e < sh.experts && x[i] != -INFINITY)
-            v = (sh.sigmoid ? (F)1 / ((F)1 + exp_of(-v)) : exp_of(v - top) / sum) + (F)__ldg(bias + e);
+            v = key_score(sh, v, top, sum) + (F)__ldg(bias + e);
         key[i] = e < sh.experts ? order_of(v) : 0;
         // the values themselves go through shared memory to the lanes of the groups
         if (sh.groups > 1 && e < sh.experts) s_key[e + group] = v;
@@ -371,7 +380,7 @@ __device__ __forceinline__ float weight_of(const RouteShape &sh, float v, bool l
 // A warp per token.  (Four tokens a warp one after the other, their weights formed together and the next token's logits
 // requested ahead, was no faster: fewer warps to hide the chain of dependent steps of each.)
 template <typename T, int I, bool BIAS>
-__global__ void __launch_bounds__(kRouteWarps * 32, I <= 8 ? 8 : 1)
+__global__ void __launch_bounds__(kRouteWarps * 32, I <= 8 ? 8 : I <= 16 ? 6 : 1)
     route_kernel(RouteShape sh, int tokens, const T *__restrict__ logits, int64_t ldl, const float *__restrict__ bias,
                  int *__restrict__ index, int64_t ldi, float *__restrict__ weight, int64_t ldw) {
     extern __shared__ double s_space[];
@@ -387,7 +396,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, I <= 8 ? 8 : 1)
     int choice = -1;
     float v = 0.f;  // the logit of the choice
     bool decided;
-    if constexpr (I <= 8) decided = choose_sorted<I, BIAS>(sh, x, bias, top, sum, s_key, &choice, &v);
+    if constexpr (I <= kSortedItems) decided = choose_sorted<I, BIAS>(sh, x, bias, top, sum, s_key, &choice, &v);
     else decided = choose<float, I, BIAS>(sh, x, bias, top, sum, reinterpret_cast<float *>(s_key), &choice);
     if constexpr (BIAS) {
         if (!decided) {
@@ -396,7 +405,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, I <= 8 ? 8 : 1)
         }
     }
     const bool live = choice >= 0;
-    if ((BIAS || I > 8) && live) v = to_float(row[choice]);
+    if ((BIAS || I > kSortedItems) && live) v = to_float(row[choice]);
     const float s = weight_of(sh, v, live, top, sum);
     if (lane < sh.k) {
         index[t * ldi + lane] = choice;
@@ -521,7 +530,7 @@ extern "C" alphasparse_status_t alphasparse_cuda_route(alphasparse_cuda_score_t 
             sh.packs = address(logits) % pack == 0 && (uint64_t)ldl * sizeof(T) % pack == 0;
             const int across = sh.group_size / I;
             sh.group_lanes = sh.group_size % I == 0 && (across & (across - 1)) == 0 ? across : 0;
-            sh.space = std::max(limited ? sh.experts + sh.groups : 0, I <= 8 ? 32 * I : 0);
+            sh.space = std::max(limited ? sh.experts + sh.groups : 0, I <= kSortedItems ? 32 * I : 0);
             const size_t smem = sizeof(double) * kRouteWarps * (size_t)sh.space;
             const auto kernel = bias ? route_kernel<T, I, true> : route_kernel<T, I, false>;
             kernel<<<blocks, kRouteWarps * 32, smem, st>>>(sh, (int)tokens, (const T *)logits, ldl, bias, index, ldi, weight, ldw);
