@@ -23,6 +23,16 @@ static bool memory_of(const void *p, int dev) {
     return at.type == cudaMemoryTypeDevice && at.device == dev;
 }
 
+// Whether two operands share memory: their extents meet, and they are not different columns of rows of one length
+static bool meet(const Operand &a, const Operand &b) {
+    if (a.begin() >= b.end() || b.begin() >= a.end()) return false;
+    const uint64_t pitch = (uint64_t)a.ld * a.elem;
+    if (pitch == 0 || pitch != (uint64_t)b.ld * b.elem) return true;
+    const uint64_t wa = (uint64_t)a.width * a.elem, wb = (uint64_t)b.width * b.elem;
+    const uint64_t from = b.begin() >= a.begin() ? (b.begin() - a.begin()) % pitch : (pitch - (a.begin() - b.begin()) % pitch) % pitch;
+    return from < wa || from + wb > pitch;
+}
+
 alphasparse_status_t check_operands(const char *call, std::initializer_list<Operand> operands) {
     char msg[200];
     for (const Operand &o : operands) {
@@ -36,7 +46,7 @@ alphasparse_status_t check_operands(const char *call, std::initializer_list<Oper
     }
     for (const Operand *a = operands.begin(); a != operands.end(); a++)
         for (const Operand *b = operands.begin(); b != a; b++)
-            if ((a->written || b->written) && !a->empty() && !b->empty() && a->begin() < b->end() && b->begin() < a->end()) {
+            if ((a->written || b->written) && !a->empty() && !b->empty() && meet(*a, *b)) {
                 snprintf(msg, sizeof(msg), "%s: an output lies in the place of another operand", call);
                 record_error(msg);
                 return ALPHA_SPARSE_STATUS_INVALID_VALUE;

@@ -216,7 +216,8 @@ struct Operand {
 };
 
 // Checks operands in the order that they are given: there (NOT_INITIALIZED), leading dimension and alignment to the
-// element (INVALID_VALUE), no written operand in the place of another (INVALID_VALUE), memory of the current device
+// element (INVALID_VALUE), no written operand in the place of another (INVALID_VALUE; columns of one block of rows beside each
+// other are two places), memory of the current device
 // (INVALID_POINTER).  Operands without elements may be null.  An optional operand is left out by the caller.
 alphasparse_status_t check_operands(const char *call, std::initializer_list<Operand> operands);
 

@@ -206,7 +206,8 @@ alphasparse_status_t alphasparse_d_mv_exchange(const double alpha, const alphasp
  * may run at the same time, take two), so the calls can be captured.  Dense operands are row-major with a leading
  * dimension of at most 2^31 - 1 elements and any alignment that their elements allow; 16-byte aligned rows are fastest.
  * A missing operand is ALPHA_SPARSE_STATUS_NOT_INITIALIZED; sizes and enums out of range, leading dimensions below
- * the width and an output that lies in the place of another operand are ALPHA_SPARSE_STATUS_INVALID_VALUE.  Operands
+ * the width and an output that lies in the place of another operand (different columns of rows of one length are
+ * different places) are ALPHA_SPARSE_STATUS_INVALID_VALUE.  Operands
  * without elements may be NULL.  Row counts go to 2^31 - 4097, widths to 2^24.  Sums are formed in 32 bits in a
  * fixed order and rounded once: the same call gives the same bits.  Values that stand where nothing selects them are
  * not read, so a NaN there does not reach a result. */
@@ -272,7 +273,7 @@ alphasparse_status_t alphasparse_cuda_expert_plan(int64_t tokens, int64_t k, int
                                                   void *buffer, size_t buffer_bytes);
 
 /* xs[slot[t, j]] = x[t]; rows of xs that no slot names, those behind the last among them, are left as they were.  A slot
- * outside [0, rows) is empty.  The gradient of x is alphasparse_cuda_expert_combine of the gradient of xs with weight =
+ * outside [0, rows) is empty; no two slots are the same (a plan's are not), or either row may be the one that is written.  The gradient of x is alphasparse_cuda_expert_combine of the gradient of xs with weight =
  * NULL. */
 alphasparse_status_t alphasparse_cuda_expert_dispatch(alphasparse_cuda_type_t type, int64_t tokens, int64_t k,
                                                       int64_t width, const void *x, int64_t ldx, const int32_t *slot,

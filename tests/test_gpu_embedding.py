@@ -175,6 +175,13 @@ def test_offsets_beyond_32_bits():
     torch.cuda.empty_cache()
 
 
+def test_table_and_result_in_columns_of_one_block():
+    block = normal(gen(2), 9, 64)
+    want = block[[7, 0, 3], :32].clone()
+    ok(spblas.embedding(torch.tensor([7, 0, 3], device="cuda"), block[:, :32], 1.0, block[:3, 32:]))
+    assert torch.equal(block[:3, 32:], want)
+
+
 def test_refusals_on_the_device():
     t, table, y = torch.zeros(4, dtype=torch.int64, device="cuda"), torch.zeros(9, 8, device="cuda"), torch.zeros(4, 8, device="cuda")
     assert spblas.embedding(t, table, 1.0, table[:4]) == capi.INVALID_VALUE           # the output in the place of the table

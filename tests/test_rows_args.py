@@ -71,6 +71,17 @@ def test_route_grad_and_the_calls_on_rows():
     assert call("expert_combine_grad", 0, 0, 2, 8, 8, None, 8, None, 8, None, 2, None, 0, None, 8, None, 2) == capi.SUCCESS
 
 
+def test_columns_of_one_block_are_different_places():
+    passed = (capi.EXECUTION_FAILED, capi.INVALID_POINTER)  # on to the check of the memory, which this is not
+    lookup = lambda table, y, ldy=64, width=32: call("embedding", capi.INDEX_I64, capi.TYPE_F32, 4, 3 * A, 1, 9, width, 1.0, table, 64, y, ldy)  # noqa: E731
+    assert lookup(A, A + 128) in passed and lookup(A + 128, A) in passed
+    assert lookup(A, A + 128 + 256) in passed and lookup(A + 256, A + 128) in passed   # a row further down or up
+    assert lookup(A, A + 124) == capi.INVALID_VALUE and lookup(A + 128, A + 4) == capi.INVALID_VALUE
+    assert lookup(A, A + 132) == capi.INVALID_VALUE        # the last column is the first of the next row's
+    assert lookup(A, A + 128, ldy=65) == capi.INVALID_VALUE
+    assert lookup(A, A + 256) == capi.INVALID_VALUE and lookup(A, A) == capi.INVALID_VALUE
+
+
 def test_workspace_sizes():
     n = C.c_size_t()
     assert call("embedding_grad_buffer_size", 10, 10, 10, None) == capi.NOT_INITIALIZED
