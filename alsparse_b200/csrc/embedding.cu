@@ -66,7 +66,7 @@ alphasparse_status_t check_operands(const char *call, std::initializer_list<Oper
 
 // ANY: rows that begin on no 16-byte boundary.  A row of y is cut at the boundaries of its memory and read at whatever shift the
 // table's row has to it.  (16,000 rows of 3283 fp16: 2 bytes an access, 16 of
-// them in flight, 79 us, so 42 us.)
+// them in flight, 79 us; four vectors a thread 41 us, two 39 us, one 47 us.)
 template <typename T, typename I, int U, bool ANY>
 __global__ void __launch_bounds__(kRowThreads)
     embedding_kernel(int rows, const I *__restrict__ token, int64_t inctoken, int64_t vocab, int width, float scale,
@@ -444,14 +444,14 @@ extern "C" alphasparse_status_t alphasparse_cuda_embedding(alphasparse_cuda_inde
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     const int vb = vector_bytes(eb, {address(table), (uint64_t)ldt * eb, address(y), (uint64_t)ldy * eb, (uint64_t)width * eb});
     const bool any = vb < 16;
-    const RowShape shape = row_shape(tokens, any ? most_pieces(width, eb) : width * (int64_t)eb / 16, 4);
+    const RowShape shape = row_shape(tokens, any ? most_pieces(width, eb) : width * (int64_t)eb / 16, any ? 2 : 4);
     const Window all = window(table, vocab, width, ldt, eb);
     cudaStream_t st = current_stream();
     const auto run = [&](auto t) {
         using T = decltype(t);
         const auto with_index = [&](auto i) {
             using I = decltype(i);
-            const auto kernel = any ? (shape.unroll == 1 ? embedding_kernel<T, I, 1, true> : embedding_kernel<T, I, 4, true>)
+            const auto kernel = any ? (shape.unroll == 1 ? embedding_kernel<T, I, 1, true> : embedding_kernel<T, I, 2, true>)
                                     : (shape.unroll == 1 ? embedding_kernel<T, I, 1, false> : embedding_kernel<T, I, 4, false>);
             kernel<<<shape.grid, kRowThreads, 0, st>>>((int)tokens, (const I *)token, inctoken, vocab, (int)width, scale, (const T *)table, ldt, all,
                                                      (T *)y, ldy, shape.log);

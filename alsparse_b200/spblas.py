@@ -284,44 +284,53 @@ def _i32s(a):
     return _kind(a)[1] == capi.INDEX_I32
 
 
-def _layout(a):
-    """(shape, strides in elements, address) of a numpy array or a torch tensor."""
-    if isinstance(a, np.ndarray):
-        return a.shape, tuple(s // a.itemsize for s in a.strides), a.ctypes.data
-    return a.shape, a.stride(), a.data_ptr()
+def _np_strides(a):
+    return tuple(s // a.itemsize for s in a.strides)
 
 
 def _matrix(a):
-    """(rows, columns, leading dimension, address) of a row-major array whose rows are contiguous, None if it is not one (the
-    caller's view has to be copied first)."""
-    shape, s, at = _layout(a)
-    if len(s) != 2:
+    """(rows, columns, leading dimension, address) of a row-major numpy array or torch tensor whose rows are contiguous, None if it
+    is not one (the caller's view has to be copied first)."""
+    try:
+        rows, width = a.shape
+    except ValueError:
         return None
-    rows, width = shape
-    ld, step = s
+    if isinstance(a, np.ndarray):
+        (ld, step), at = _np_strides(a), a.ctypes.data
+    else:
+        (ld, step), at = a.stride(), a.data_ptr()
     if step != 1 and width > 1:
         return None
-    return rows, width, ld if rows > 1 else max(ld, width), at
+    return rows, width, ld if rows > 1 or ld > width else width, at
 
 
 def _vector(a):
     """(elements, distance, address) of an array of one dimension, None if it has another number of them."""
-    shape, s, at = _layout(a)
-    if len(s) != 1:
+    try:
+        n, = a.shape
+    except ValueError:
         return None
-    return shape[0], s[0] if shape[0] > 1 else 1, at
+    if isinstance(a, np.ndarray):
+        (step,), at = _np_strides(a), a.ctypes.data
+    else:
+        (step,), at = a.stride(), a.data_ptr()
+    return n, step if n > 1 else 1, at
 
 
 def _matrices(a):
     """(matrices, rows, columns, leading dimension, distance of the matrices, address) of an array of three dimensions."""
-    shape, s, at = _layout(a)
-    if len(s) != 3:
+    try:
+        n, rows, width = a.shape
+    except ValueError:
         return None
-    n, rows, width = shape
-    if s[2] != 1 and width > 1:
+    if isinstance(a, np.ndarray):
+        (apart, ld, step), at = _np_strides(a), a.ctypes.data
+    else:
+        (apart, ld, step), at = a.stride(), a.data_ptr()
+    if step != 1 and width > 1:
         return None
-    ld = s[1] if rows > 1 else max(s[1], width)
-    return n, rows, width, ld, s[0] if n > 1 else max(s[0], ld * rows), at
+    ld = ld if rows > 1 or ld > width else width
+    return n, rows, width, ld, apart if n > 1 or apart > ld * rows else ld * rows, at
 
 
 def _buffer(b):
