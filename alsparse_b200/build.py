@@ -52,7 +52,7 @@ def build_library(force=False, verbose_ptxas=False):
         nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3",
         "-std=c++17", "-shared", "-Xcompiler", "-fPIC,-fopenmp,-O2,-Wall",
         "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-ccbin", "/usr/bin/g++",
-        "-cudart", "static", "-o", LIB,
+        "-cudart", "static", "--threads", "0", "-o", LIB,  # sources side by side, a thread per core
     ]
     if verbose_ptxas:
         cmd += ["-Xptxas", "-v"]
