@@ -176,10 +176,11 @@ __device__ __forceinline__ unsigned long long now_ns() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-// Waits for the phase of the given parity; false when it ran out of time or another thread of the block did.  CLUSTER: what the
+// Waits for the phase of the given parity; false when it ran out of time or another thread of the block did.  `steps`: of a
+// product that has to be done first, a hundredth of a millisecond more for each.  CLUSTER: what the
 // pair's other block wrote before it arrived is seen (dear: about a microsecond).
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool barrier_wait(uint64_t *b, unsigned parity, volatile int *s_stop) {
+__device__ __forceinline__ bool barrier_wait(uint64_t *b, unsigned parity, volatile int *s_stop, int steps = 0) {
     unsigned long long begin = 0;
     for (unsigned i = 0;; i++) {
         unsigned done;
@@ -198,7 +199,7 @@ __device__ __forceinline__ bool barrier_wait(uint64_t *b, unsigned parity, volat
             if (*s_stop) return false;
             const unsigned long long t = now_ns();
             if (!begin) begin = t;
-            else if (t - begin > kMmLimitNs) {
+            else if (t - begin > kMmLimitNs + (unsigned long long)steps * 10000) {
                 *s_stop = 1;
                 return false;
             }
@@ -207,8 +208,8 @@ __device__ __forceinline__ bool barrier_wait(uint64_t *b, unsigned parity, volat
 }
 // ... by a whole warp, with one answer for all lanes
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool warp_wait(uint64_t *b, unsigned parity, volatile int *s_stop) {
-    return __all_sync(0xffffffffu, barrier_wait<CLUSTER>(b, parity, s_stop));
+__device__ __forceinline__ bool warp_wait(uint64_t *b, unsigned parity, volatile int *s_stop, int steps = 0) {
+    return __all_sync(0xffffffffu, barrier_wait<CLUSTER>(b, parity, s_stop, steps));
 }
 // PAIR: `barrier` is an address of the cluster's, the other block's too
 template <bool PAIR>
@@ -624,7 +625,7 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
             const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
             const int slot = count & 1, m = q.m0 + rank * kMmM + part * 32;
             if (q.steps > 0) {
-                if (!warp_wait(&s_acc_full[slot], (count >> 1) & 1, s_stop)) break;
+                if (!warp_wait(&s_acc_full[slot], (count >> 1) & 1, s_stop, q.steps)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 count++;
             }
@@ -703,7 +704,7 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
             if (q.steps > 0 && ragged(q, last)) {
                 const int at = (stage + last) % s.stages;
                 // both wait for every one: a phase that is not waited for would be taken for the one after the next
-                if (!(good = warp_wait(&s_own[at], own_phases >> at & 1, s_stop))) break;
+                if (!(good = warp_wait(&s_own[at], own_phases >> at & 1, s_stop, q.steps))) break;
                 own_phases ^= 1u << at;
                 turn ^= 1;
                 if (turn) {
