@@ -5,8 +5,8 @@
 // one per SM.  One warp issues copies, one the products, four empty the accumulators; two accumulators, so that a tile is
 // written while the next is multiplied.  The rows of an expert are the narrow side of the tile: its width is any multiple
 // of 16, so an expert's rows are cut into equal tiles of at most 256, and no more rows are fetched and written than there
-// are.  (A product of 128 x n x 16 takes some 128 cycles for every n up to 256: 306 ns for 64 of k at n = 32, 307 at 256, without
-// copies.  So a narrow tile of weights streams at most 61 GB/s through an SM.)  With many rows an expert two SMs work on one tile of
+// are.  (64 of k take 233 ns at n = 16, 304 at 256: the four products take 270 at 256, and
+// what there is to do around them is no less with narrow ones.  So a narrow tile of weights streams at most 70 GB/s through an SM.)  With many rows an expert two SMs work on one tile of
 // 256 (cta_group::2), which halves what each fetches of the narrow operand.  The offsets stay on the device: every block
 // forms the same table of row tiles.
 // Addresses or strides that TMA does not take (no multiple of 16 bytes) are brought by fourteen warps of their own instead.
@@ -167,7 +167,9 @@ __device__ __forceinline__ void barrier_expect(uint64_t *b, unsigned bytes) {
 }
 // True in one lane of a converged warp, always the same one.  The copies and products are issued under this and not under a
 // test of the lane's number: the compiler then keeps their operands in uniform registers (as it is, a product of
-// 128 x 32 x 16 was issued every 250 cycles under lane == 0).
+// 128 x 32 x 16 was issued every 250 cycles under lane == 0).  What the warp of the products does for 64 of k besides bounds
+// narrow tiles: 273 ns with an election each time, 233 ns with one lane for the whole loop and the four products written out.
+// The copying warp is better off with all lanes in the loop (one lane: 249 to 303 ns).
 __device__ __forceinline__ bool elect_one() {
     unsigned one;
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
@@ -582,43 +584,43 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
                 if (++stage == s.stages) stage = 0, phase ^= 1;
             }
         }
-    } else if (w == 1) {
+    } else if (w == 1 && rank == 0 && elect_one()) {
         int stage = 0, count = 0;
         unsigned full_phases = 0, ready_phases = 0;  // a bit for each stage: the phase that comes next
         bool good = true;
-        for (int t = worker; rank == 0 && good && t < tiles; t += workers) {
+        for (int t = worker; good && t < tiles; t += workers) {
             const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
             if (q.steps == 0) continue;
             const int slot = count & 1;
-            if (!(good = warp_wait(&s_acc_empty[slot], ((count >> 1) & 1) ^ 1, s_stop))) break;
+            if (!(good = barrier_wait(&s_acc_empty[slot], ((count >> 1) & 1) ^ 1, s_stop))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             count++;
             const int length = FORM == kGradient ? q.length : s.reduced;
             const unsigned instruction = s.instruction | (unsigned)(q.n >> 3) << 17;
+            const unsigned d = tmem + slot * s.acc_stride;
             for (int k = 0; k < q.steps; k++) {
                 char *a = ring + (size_t)stage * s.stage_bytes;
                 const int left = length - k * kMmK, parts = min(4, (left + 15) / 16);
                 if (!ANY && FORM == kGradient && ragged(q, k)) {
-                    if (!(good = warp_wait<true>(&s_ready[stage], ready_phases >> stage & 1, s_stop))) break;
+                    if (!(good = barrier_wait<true>(&s_ready[stage], ready_phases >> stage & 1, s_stop))) break;
                     ready_phases ^= 1u << stage;
                 } else {
-                    if (!(good = warp_wait(&s_full[stage], full_phases >> stage & 1, s_stop))) break;
+                    if (!(good = barrier_wait(&s_full[stage], full_phases >> stage & 1, s_stop))) break;
                     full_phases ^= 1u << stage;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (elect_one()) {
-                    const uint64_t da = operand_descriptor(smem_address(a), a_k), db = operand_descriptor(smem_address(a + a_bytes), b_k);
-                    for (int i = 0; i < parts; i++)
-                        multiply<PAIR>(tmem + slot * s.acc_stride, da + (uint64_t)(i * (a_k ? 32 : 2048) >> 4),
-                                       db + (uint64_t)(i * (b_k ? 32 : 2048) >> 4), instruction, k > 0 || i > 0);
-                    commit<PAIR>(&s_empty[stage]);
-                    if (k == q.steps - 1) commit<PAIR>(&s_acc_full[slot]);
-                }
-                __syncwarp();
+                const uint64_t da = operand_descriptor(smem_address(a), a_k), db = operand_descriptor(smem_address(a + a_bytes), b_k);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (i < parts)
+                        multiply<PAIR>(d, da + (uint64_t)(i * (a_k ? 32 : 2048) >> 4), db + (uint64_t)(i * (b_k ? 32 : 2048) >> 4), instruction,
+                                       k > 0 || i > 0);
+                commit<PAIR>(&s_empty[stage]);
+                if (k == q.steps - 1) commit<PAIR>(&s_acc_full[slot]);
                 if (++stage == s.stages) stage = 0;
             }
         }
-    } else if (w < 10) {
+    } else if (w >= 2 && w < 10) {
         // the quarter of the accumulators' lanes that this warp may read, and whether it takes the even or the odd blocks of 32
         // columns (four warps alone take longer for a tile than the products of a few hundred rows)
         const int part = w & 3, odd = (w - 2) >> 2;
@@ -663,7 +665,7 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
                 }
             }
         }
-    } else if (ANY) {
+    } else if (ANY && w >= 10) {
         const int thread = threadIdx.x - 320;
         int stage = 0;
         unsigned phase = 0;
@@ -692,7 +694,7 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
                 if (++stage == s.stages) stage = 0, phase ^= 1;
             }
         }
-    } else if (FORM == kGradient) {
+    } else if (FORM == kGradient && w >= 10) {
         // the ends of experts whose rows are no multiple of 16: rows of the next expert (or behind the last) came along with
         // the copy.  Zeros in both operands up to the next multiple, so that nothing that stands there, NaN included, gets
         // into the sum; then the first block's products may go on.  Two warps in turn: one alone takes 1.7 us a tile, of which its
