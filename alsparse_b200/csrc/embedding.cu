@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kRowThreads)
         const int v = v0 + (u << log);
         p[u] = zero_pack<T, E>();
         if (ANY) {
-            if (inside && cut.is_whole(v)) p[u] = load_any<T>(src + cut.begin(v), all);
+            if (inside && cut.count(v) > 0) p[u] = load_any<T>(src + cut.begin(v), cut.count(v), all);
         } else if (inside && v * E < width) {
             p[u] = load_pack<T, E>(src + v * E);
         }
@@ -102,10 +102,7 @@ __global__ void __launch_bounds__(kRowThreads)
             p[u] = pack<T, E>(f);
         }
         if (ANY) {
-            if (cut.is_whole(v)) store_pack<T, E>(dst + cut.begin(v), p[u]);
-            else
-                for (int i = cut.begin(v); i < cut.end(v); i++)
-                    dst[i] = !inside ? from_float<T>(0.f) : scale != 1.f ? from_float<T>(to_float(__ldg(src + i)) * scale) : __ldg(src + i);
+            store_any<T>(dst + cut.begin(v), cut.count(v), p[u]);
         } else if (v * E < width) {
             store_pack<T, E>(dst + v * E, p[u]);
         }
@@ -444,7 +441,7 @@ extern "C" alphasparse_status_t alphasparse_cuda_embedding(alphasparse_cuda_inde
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     const int vb = vector_bytes(eb, {address(table), (uint64_t)ldt * eb, address(y), (uint64_t)ldy * eb, (uint64_t)width * eb});
     const bool any = vb < 16;
-    const RowShape shape = row_shape(tokens, any ? most_pieces(width, eb) : width * (int64_t)eb / 16, any ? 2 : 4);
+    const RowShape shape = row_shape(tokens, any ? most_pieces(width, eb) : width * (int64_t)eb / 16, any ? 2 : 4, width * (int64_t)eb < 1024 ? 3 : 5);
     const Window all = window(table, vocab, width, ldt, eb);
     cudaStream_t st = current_stream();
     const auto run = [&](auto t) {

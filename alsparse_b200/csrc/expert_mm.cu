@@ -367,53 +367,6 @@ struct MmShape {
     Window all_a, all_b;
 };
 
-__device__ __forceinline__ uint4 load_if(const char *p, bool there) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    asm("{\n.reg .pred p;\nsetp.ne.b32 p, %5, 0;\n@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n}"
-        : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
-        : "l"(p), "r"((unsigned)there));
-    return v;
-}
-
-// load_any in two parts: the two aligned vectors are requested without a branch, so that several are on their way at once, and
-// shifted together when they are needed.  `there` false: zeros.  (32,768 x 1001 x 1439, 16 experts: 1346 us with load_any and eight warps, 876 us
-// so, 834 us with fourteen.  The kernels on rows, which have more blocks to hide latency, lose by the registers: lookup of odd rows 42 -> 61 us.)
-template <typename T>
-struct AnyPack {
-    static constexpr int E = 16 / sizeof(T);
-    uint4 x, y;
-    const T *p;
-    bool apart;
-    __device__ __forceinline__ AnyPack() {}
-    __device__ __forceinline__ AnyPack(const T *p_, const Window &w, bool there) : p(p_) {
-        const char *at = reinterpret_cast<const char *>(p);
-        const unsigned shift = (unsigned)(reinterpret_cast<uintptr_t>(at) & 15);
-        const char *a = at - shift;
-        const bool inside = shift == 0 || (a >= w.lo && a + 32 <= w.hi);
-        x = load_if(a, there && inside);
-        y = load_if(a + 16, there && inside && shift != 0);
-        apart = there && !inside;
-    }
-    __device__ __forceinline__ Pack<T, E> get() const {
-        Pack<T, E> r;
-        if (apart) {
-            float f[E];
-#pragma unroll
-            for (int i = 0; i < E; i++) f[i] = to_float(__ldg(p + i));
-            return pack<T, E>(f);
-        }
-        const unsigned shift = (unsigned)(reinterpret_cast<uintptr_t>(p) & 15);
-        unsigned c[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int i = 0; i < 6; i++) c[i] = shift & 8 ? c[i + 2] : c[i];
-#pragma unroll
-        for (int i = 0; i < 5; i++) c[i] = shift & 4 ? c[i + 1] : c[i];
-#pragma unroll
-        for (int i = 0; i < 4; i++) r.w[i] = sizeof(T) == 4 ? c[i] : __funnelshift_r(c[i], c[i + 1], (shift & 2) * 8);
-        return r;
-    }
-};
-
 // ANY: a thread's share of an operand's part of a stage, in the order that the copies of TMA leave it in (16 bytes c of a row of
 // 128 bytes at c ^ (row & 7)).  K_MAJOR: one box of `extent` rows; else boxes of 64 rows side by side, `extent` columns wide.  Only
 // `rows_there` rows and `cols_there` columns exist; the rest becomes zeros.

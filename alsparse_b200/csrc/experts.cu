@@ -170,7 +170,8 @@ struct PlanShape {
 
 // Threads along a token's row as row_shape lays them out: the row is read once and written to every place of the token.  ANY:
 // rows that begin on no 16-byte boundary; each place is cut at the boundaries of its memory, and the row read again at the
-// shift that it has to it, out of L1.
+// shift that it has to it, out of L1.  (12,001 tokens of 6 rows of 2047 fp16: 154 us in groups of a warp, 168 of a block.  Aligned,
+// 2880 wide bf16: 74 us in groups of a warp, so 70.)
 template <typename T, int U, bool ANY>
 __global__ void __launch_bounds__(kRowThreads)
     dispatch_kernel(int tokens, int k, int width, const T *__restrict__ x, int64_t ldx, Window all, const int *__restrict__ slot,
@@ -197,14 +198,12 @@ __global__ void __launch_bounds__(kRowThreads)
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int v = v0 + (u << log);
-                if (cut.is_whole(v)) p[u] = load_any<T>(src + cut.begin(v), all);
+                if (cut.count(v) > 0) p[u] = load_any<T>(src + cut.begin(v), cut.count(v), all);
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int v = v0 + (u << log);
-                if (cut.is_whole(v)) store_pack<T, E>(dst + cut.begin(v), p[u]);
-                else
-                    for (int i = cut.begin(v); i < cut.end(v); i++) dst[i] = __ldg(src + i);
+                const int v = v0 + (u << log), n = cut.count(v);
+                if (n > 0) store_any<T>(dst + cut.begin(v), n, p[u]);
             }
         } else {
 #pragma unroll
@@ -221,34 +220,24 @@ __global__ void __launch_bounds__(kRowThreads)
 // out[t] = sum over j of weight[t, j] y[slot[t, j]] + beta out[t], in 32 bits in the order of j, rounded once.  Eight rows of y
 // are requested at a time, 16 bytes of each by a thread: 128 bytes in flight at 64 registers.  (12,001 tokens of 6 rows of 2048
 // fp16: four rows of 64 bytes at 138 registers, one block per SM, 94 us; so 65 us.)  ANY, rows that begin on no 16-byte
-// boundary: four rows at a time, since each takes two loads.
-constexpr int kCombineAhead = 8, kCombineAheadAny = 4;
+// boundary: a row's two vectors are loaded where they are added, and blocks enough to fill the SM wait in turn instead: 32
+// registers, eight blocks.  (2047 wide: all rows requested first, with their shifts 127 us; 40 registers 94 us; so 82 us.)
+constexpr int kCombineAhead = 8;
 
 template <typename T, bool ANY>
-__global__ void __launch_bounds__(kRowThreads, 4)
+__global__ void __launch_bounds__(kRowThreads, ANY ? 8 : 4)
     combine_kernel(int tokens, int k, int width, const T *__restrict__ y, int64_t ldy, Window all, int64_t rows,
                    const int *__restrict__ slot, int64_t lds, const float *__restrict__ weight, int64_t ldw, float beta,
                    T *__restrict__ out, int64_t ldo, int log) {
-    constexpr int E = 16 / sizeof(T), A = ANY ? kCombineAheadAny : kCombineAhead;
+    constexpr int E = 16 / sizeof(T), A = ANY ? 2 : kCombineAhead;
     const int64_t t = (int64_t)blockIdx.x * (kRowThreads >> log) + (threadIdx.x >> log);
     if (t >= tokens) return;
     const int v = (int)((blockIdx.y << log) + (threadIdx.x & ((1 << log) - 1)));
     T *dst = out + t * ldo;
     const Cut<T> cut(dst, width);
     const int *places = slot + t * lds;
-    if (ANY && !cut.is_whole(v)) {
-        for (int i = cut.begin(v); i < cut.end(v); i++) {
-            float acc = 0.f;
-            for (int j = 0; j < k; j++) {
-                const int at = __ldg(places + j);
-                if (at >= 0 && at < rows) acc = fmaf(weight ? __ldg(weight + t * ldw + j) : 1.f, to_float(__ldg(y + at * ldy + i)), acc);
-            }
-            dst[i] = from_float<T>(beta != 0.f ? fmaf(beta, to_float(dst[i]), acc) : acc);
-        }
-        return;
-    }
-    const int from = ANY ? cut.begin(v) : v * E;
-    if (from >= width) return;
+    const int from = ANY ? cut.begin(v) : v * E, n = ANY ? cut.count(v) : E;
+    if (ANY ? n <= 0 : from >= width) return;
     float acc[E] = {};
     for (int j0 = 0; j0 < k; j0 += A) {
         Pack<T, E> p[A];
@@ -260,13 +249,13 @@ __global__ void __launch_bounds__(kRowThreads, 4)
         }
 #pragma unroll
         for (int j = 0; j < A; j++)
-            if (at[j] >= 0) p[j] = ANY ? load_any<T>(y + at[j] * ldy + from, all) : load_pack<T, E>(y + at[j] * ldy + from);
+            if (!ANY && at[j] >= 0) p[j] = load_pack<T, E>(y + at[j] * ldy + from);
 #pragma unroll
         for (int j = 0; j < A; j++) {
             if (at[j] < 0) continue;
             const float w = weight ? __ldg(weight + t * ldw + j0 + j) : 1.f;
             float f[E];
-            unpack<T, E>(p[j], f);
+            unpack<T, E>(ANY ? load_any<T>(y + at[j] * ldy + from, n, all) : p[j], f);
 #pragma unroll
             for (int i = 0; i < E; i++) acc[i] = fmaf(w, f[i], acc[i]);
         }
@@ -274,18 +263,24 @@ __global__ void __launch_bounds__(kRowThreads, 4)
     dst += from;
     if (beta != 0.f) {
         float f[E];
-        unpack<T, E>(load_pack<T, E, true>(dst), f);
+        if (n == E) {
+            unpack<T, E>(load_pack<T, E, true>(dst), f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; i++) f[i] = i < n ? to_float(dst[i]) : 0.f;
+        }
 #pragma unroll
         for (int i = 0; i < E; i++) acc[i] = fmaf(beta, f[i], acc[i]);
     }
-    store_pack<T, E>(dst, pack<T, E>(acc));
+    store_any<T>(dst, n, pack<T, E>(acc));
 }
 
 // dy[slot[t, j]] = weight[t, j] dout[t] and dweight[t, j] = <dout[t], y[slot[t, j]]>.  A group of threads of one block has the
 // whole row of a token, so that the inner products end in it: lanes, then warps, in a fixed order.  Eight rows at a time,
 // as above; their eight inner products are added up over a warp together, each step halving what a lane holds.  (12,001
-// tokens of 6 rows of 2048 fp16: four rows at a time 143 us, so 119 us; two blocks per SM instead of three 151 us.)  ANY: each
-// row of dy is cut at the boundaries of its memory, and the rows of dout and y read at the shifts that they have to it.
+// tokens of 6 rows of 2048 fp16: four rows at a time 143 us, so 119 us; two blocks per SM instead of three 151 us.)  Groups
+// of two warps or more for wide rows: 6000 tokens of 4100 elements 182 us, 217 in single warps.  ANY: each row of dy is cut at the
+// boundaries of its memory, and the rows of dout and y read at the shifts that they have to it.
 template <typename T, bool ANY>
 __global__ void __launch_bounds__(kRowThreads, 3)
     combine_grad_kernel(int tokens, int k, int width, const T *__restrict__ dout, int64_t ldo, Window all_dout,
@@ -311,28 +306,20 @@ __global__ void __launch_bounds__(kRowThreads, 3)
 #pragma unroll
                 for (int j = 0; j < kCombineAhead; j++) {
                     if (at[j] < 0) continue;
-                    const float w = weight ? __ldg(weight + t * ldw + j0 + j) : 1.f;
-                    const T *y_row = y + at[j] * ldy;
                     T *dst = dy + at[j] * lddy;
                     const Cut<T> cut(dst, width);
-                    const int from = cut.begin(v);
-                    if (cut.is_whole(v)) {
-                        float f[E], g[E];
-                        unpack<T, E>(load_any<T>(d_row + from, all_dout), f);
-                        unpack<T, E>(load_any<T>(y_row + from, all_y), g);
+                    const int from = cut.begin(v), n = cut.count(v);
+                    if (n <= 0) continue;
+                    const float w = weight ? __ldg(weight + t * ldw + j0 + j) : 1.f;
+                    float f[E], g[E];
+                    unpack<T, E>(load_any<T>(d_row + from, n, all_dout), f);
+                    unpack<T, E>(load_any<T>(y + at[j] * ldy + from, n, all_y), g);
 #pragma unroll
-                        for (int i = 0; i < E; i++) {
-                            dot[j] = fmaf(f[i], g[i], dot[j]);
-                            f[i] *= w;
-                        }
-                        store_pack<T, E>(dst + from, pack<T, E>(f));
-                    } else {
-                        for (int i = from; i < cut.end(v); i++) {
-                            const float f = to_float(__ldg(d_row + i));
-                            dot[j] = fmaf(f, to_float(__ldg(y_row + i)), dot[j]);
-                            dst[i] = from_float<T>(w * f);
-                        }
+                    for (int i = 0; i < E; i++) {
+                        if (i < n) dot[j] = fmaf(f[i], g[i], dot[j]);
+                        f[i] *= w;
                     }
+                    store_any<T>(dst + from, n, pack<T, E>(f));
                 }
             } else {
                 const int from = v * E;
@@ -461,7 +448,7 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_dispatch(alphasparse_cud
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     const int vb = vector_bytes(eb, {address(x), (uint64_t)ldx * eb, address(xs), (uint64_t)ldxs * eb, (uint64_t)width * eb});
     const bool any = vb < 16;
-    const RowShape shape = row_shape(tokens, any ? most_pieces(width, eb) : width * (int64_t)eb / 16, 4);
+    const RowShape shape = row_shape(tokens, any ? most_pieces(width, eb) : width * (int64_t)eb / 16, 4, any ? 5 : 8);
     const Window all = window(x, tokens, width, ldx, eb);
     cudaStream_t st = current_stream();
     const auto run = [&](auto t) {
@@ -490,7 +477,7 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_combine(alphasparse_cuda
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     const int vb = vector_bytes(eb, {address(y), (uint64_t)ldy * eb, address(out), (uint64_t)ldo * eb, (uint64_t)width * eb});
     const bool any = vb < 16;
-    const RowShape shape = row_shape(tokens, any ? most_pieces(width, eb) : width * (int64_t)eb / 16, 1);
+    const RowShape shape = row_shape(tokens, any ? most_pieces(width, eb) : width * (int64_t)eb / 16, 1, width * (int64_t)eb < 1024 ? 3 : 5);
     const Window all = window(y, rows, width, ldy, eb);
     cudaStream_t st = current_stream();
     const auto run = [&](auto t) {
@@ -525,8 +512,7 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_combine_grad(alphasparse
                                      (uint64_t)lddy * eb, (uint64_t)width * eb});
     const bool any = vb < 16;
     const int64_t pieces = any ? most_pieces(width, eb) : width * (int64_t)eb / 16;
-    int log = 0;
-    while ((1 << log) < kRowThreads && (int64_t)1 << log < pieces) log++;
+    const int log = row_group(tokens, pieces, 1, pieces < 128 ? 5 : 6);
     const unsigned blocks = (unsigned)((tokens + (kRowThreads >> log) - 1) / (kRowThreads >> log));
     const Window all_dout = window(dout, tokens, width, ldo, eb), all_y = window(y, rows, width, ldy, eb);
     cudaStream_t st = current_stream();

@@ -123,47 +123,104 @@ struct Window {
     const char *lo, *hi;
 };
 
-// 16 bytes of elements from an address that is only aligned to the element: the two aligned vectors that hold them, shifted
-// together; element by element where those reach out of the operand.
+// The 16 bytes that begin `shift` bytes into two aligned vectors
 template <typename T>
-__device__ __forceinline__ Pack<T, 16 / sizeof(T)> load_any(const T *p, const Window &w) {
-    constexpr int E = 16 / sizeof(T);
-    const char *at = reinterpret_cast<const char *>(p);
-    const unsigned shift = (unsigned)(reinterpret_cast<uintptr_t>(at) & 15);
-    const char *a = at - shift;
-    if (shift == 0) return load_pack<T, E>(p);
-    Pack<T, E> r;
-    if (a >= w.lo && a + 32 <= w.hi) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(a)), y = __ldg(reinterpret_cast<const uint4 *>(a) + 1);
-        unsigned c[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+__device__ __forceinline__ Pack<T, 16 / sizeof(T)> across(const uint4 &x, const uint4 &y, unsigned shift) {
+    Pack<T, 16 / sizeof(T)> r;
+    unsigned c[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int i = 0; i < 6; i++) c[i] = shift & 8 ? c[i + 2] : c[i];
+    for (int i = 0; i < 6; i++) c[i] = shift & 8 ? c[i + 2] : c[i];
 #pragma unroll
-        for (int i = 0; i < 5; i++) c[i] = shift & 4 ? c[i + 1] : c[i];
+    for (int i = 0; i < 5; i++) c[i] = shift & 4 ? c[i + 1] : c[i];
 #pragma unroll
-        for (int i = 0; i < 4; i++) r.w[i] = sizeof(T) == 4 ? c[i] : __funnelshift_r(c[i], c[i + 1], (shift & 2) * 8);
-    } else {
-        float f[E];
-#pragma unroll
-        for (int i = 0; i < E; i++) f[i] = to_float(__ldg(p + i));
-        r = pack<T, E>(f);
-    }
+    for (int i = 0; i < 4; i++) r.w[i] = sizeof(T) == 4 ? c[i] : __funnelshift_r(c[i], c[i + 1], (shift & 2) * 8);
     return r;
 }
 
-// A row of `width` elements cut at the 16-byte boundaries of memory: piece 0 up to the first, pieces 1 .. whole of 16 bytes,
-// piece whole + 1 behind the last.
+template <typename T>
+__device__ __forceinline__ Pack<T, 16 / sizeof(T)> one_by_one(const T *p, int n) {
+    constexpr int E = 16 / sizeof(T);
+    Pack<T, E> r = zero_pack<T, E>();
+#pragma unroll
+    for (int i = 0; i < E; i++)
+        if (i < n) {
+            if constexpr (sizeof(T) == 4) r.w[i] = __ldg(reinterpret_cast<const unsigned *>(p) + i);
+            else r.w[i / 2] |= (unsigned)__ldg(reinterpret_cast<const unsigned short *>(p) + i) << (i & 1) * 16;
+        }
+    return r;
+}
+
+// n elements, 16 bytes at most, from an address that is only aligned to the element: the two aligned vectors that hold them,
+// shifted together; element by element where those reach out of the operand.  What comes behind the n is nobody's.
+template <typename T>
+__device__ __forceinline__ Pack<T, 16 / sizeof(T)> load_any(const T *p, int n, const Window &w) {
+    constexpr int E = 16 / sizeof(T);
+    const unsigned shift = (unsigned)(reinterpret_cast<uintptr_t>(p) & 15);
+    const char *a = reinterpret_cast<const char *>(p) - shift;
+    if (shift == 0 && n == E) return load_pack<T, E>(p);
+    if (a < w.lo || a + 32 > w.hi) return one_by_one<T>(p, n);
+    return across<T>(__ldg(reinterpret_cast<const uint4 *>(a)), __ldg(reinterpret_cast<const uint4 *>(a) + 1), shift);
+}
+
+__device__ __forceinline__ uint4 load_if(const void *p, bool there) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    asm("{\n.reg .pred p;\nsetp.ne.b32 p, %5, 0;\n@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n}"
+        : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+        : "l"(p), "r"((unsigned)there));
+    return v;
+}
+
+// 16 bytes as load_any gives them, in two parts: the two aligned vectors are requested without a branch, so that several are on
+// their way at once, and shifted together when they are needed.  `there` false: zeros.  (Experts' products of 32,768 x 1001 x 1439,
+// 16 experts: 1346 us with load_any and eight warps, 876 us so, about 850 with fourteen.  The kernels on rows, which have more
+// blocks to hide latency, lose by the registers: combine of rows of 2047 94 -> 127 us.)
+template <typename T>
+struct AnyPack {
+    static constexpr int E = 16 / sizeof(T);
+    uint4 x, y;
+    const T *p;
+    bool apart;
+    __device__ __forceinline__ AnyPack() {}
+    __device__ __forceinline__ AnyPack(const T *p_, const Window &w, bool there) : p(p_) {
+        const unsigned shift = (unsigned)(reinterpret_cast<uintptr_t>(p) & 15);
+        const char *a = reinterpret_cast<const char *>(p) - shift;
+        const bool inside = shift == 0 || (a >= w.lo && a + 32 <= w.hi);
+        x = load_if(a, there && inside);
+        y = load_if(a + 16, there && inside && shift != 0);
+        apart = there && !inside;
+    }
+    __device__ __forceinline__ Pack<T, E> get() const {
+        return apart ? one_by_one<T>(p, E) : across<T>(x, y, (unsigned)(reinterpret_cast<uintptr_t>(p) & 15));
+    }
+};
+
+// The first n elements of a pack to where a row ends or begins; all of it, where n says so, to a 16-byte boundary
+template <typename T>
+__device__ __forceinline__ void store_any(T *p, int n, const Pack<T, 16 / sizeof(T)> &v) {
+    constexpr int E = 16 / sizeof(T);
+    if (n == E) {
+        store_pack<T, E>(p, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < E; i++)
+        if (i < n) {
+            if constexpr (sizeof(T) == 4) reinterpret_cast<unsigned *>(p)[i] = v.w[i];
+            else reinterpret_cast<unsigned short *>(p)[i] = (unsigned short)(v.w[i / 2] >> (i & 1) * 16);
+        }
+}
+
+// A row of `width` elements cut at the 16-byte boundaries of memory: piece 0 up to the first, then pieces of 16 bytes, the last
+// of what is left, and empty ones.
 template <typename T>
 struct Cut {
     static constexpr int E = 16 / sizeof(T);
-    int head, whole, width;
+    int head, width;
     __device__ __forceinline__ Cut(const T *row, int width_) : width(width_) {
         head = min(width, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T));
-        whole = (width - head) / E;
     }
-    __device__ __forceinline__ bool is_whole(int v) const { return v >= 1 && v <= whole; }
     __device__ __forceinline__ int begin(int v) const { return v == 0 ? 0 : min(width, head + (v - 1) * E); }
-    __device__ __forceinline__ int end(int v) const { return v == 0 ? head : min(width, head + v * E); }  // of pieces that are not whole
+    __device__ __forceinline__ int count(int v) const { return v == 0 ? head : min(width, head + v * E) - begin(v); }
 };
 // Pieces of a row, whichever way it is cut
 inline int64_t most_pieces(int64_t width, size_t elem) { return width * (int64_t)elem / 16 + 2; }
@@ -230,18 +287,36 @@ inline int vector_bytes(size_t elem, std::initializer_list<uint64_t> all) {
 
 inline uint64_t address(const void *p) { return (uint64_t)reinterpret_cast<uintptr_t>(p); }
 
-// A row of `nv` vectors by a group of 2^log threads, `unroll` vectors a thread and piece of the row.  Few vectors in all:
-// one a thread, so that the call is done in one round trip to memory; many: `many`, so that enough are in flight.
+constexpr int kRowThreads = 256;
+
+// log2 of the threads, at most a block, that share a row of `nv` vectors, `unroll` vectors a thread at a time.  Few vectors in
+// all: as many as the row has, so that it is done in one round trip to memory.  Many: the number from 2^least up that leaves the
+// fewest of them idle in the row's last piece, the largest of equals.  (Rows of 272 vectors, by a whole block twice: combine 55 us,
+// its gradient 104; by 32 and 64 threads 47 and 78.)  Wide rows in groups of a warp or more; rows of up to 1 KB in groups
+// from 8 threads on (33 vectors: 20 us, 27 by warps).
+inline int row_group(int64_t rows, int64_t nv, int unroll, int least) {
+    int best = 0;
+    while ((1 << best) < kRowThreads && (int64_t)unroll << best < nv) best++;
+    if (rows * nv <= 148 * 2048 || nv > 16 * (int64_t)unroll * kRowThreads) return best;  // of many pieces, one more or less
+    const auto slots = [&](int log) {
+        const int64_t piece = (int64_t)unroll << log;
+        return (nv + piece - 1) / piece * piece;
+    };
+    for (int log = best - 1; log >= least; log--)
+        if (slots(log) < slots(best)) best = log;
+    return best;
+}
+
+// A row by groups of 2^log threads, `unroll` vectors a thread and piece of the row: one where there are few in all; many: `many`,
+// so that enough are in flight.
 struct RowShape {
     int log, unroll;
     dim3 grid;
 };
-constexpr int kRowThreads = 256;
-inline RowShape row_shape(int64_t rows, int64_t nv, int many) {
+inline RowShape row_shape(int64_t rows, int64_t nv, int many, int least) {
     RowShape s;
     s.unroll = rows * nv <= 148 * 2048 ? 1 : many;
-    s.log = 0;
-    while ((1 << s.log) < kRowThreads && (int64_t)s.unroll << s.log < nv) s.log++;
+    s.log = row_group(rows, nv, s.unroll, least);
     const int64_t per_block = kRowThreads >> s.log, piece = (int64_t)s.unroll << s.log;
     s.grid = dim3((unsigned)((rows + per_block - 1) / per_block), (unsigned)((nv + piece - 1) / piece));
     return s;
