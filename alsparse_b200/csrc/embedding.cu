@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(kRowThreads)
 constexpr int kGradMostRows = 1024;  // table rows whose tokens one block of the sort collects, at most
 constexpr int kGradSortWarps = 32;
 constexpr int kGradAhead = 16;       // tokens a lane of the sort requests at a time
+constexpr int kGradGroups = 256;     // groups of kGradAhead steps whose steps a warp of the sort remembers
 constexpr int kGradPiece = 32;       // sorted positions one block of the sum walks
 constexpr int kGradThreads = 128;
 
@@ -121,44 +122,58 @@ constexpr int kGradThreads = 128;
 // takes one contiguous share of them, counts those of each of the block's rows, and after the prefix over warps and rows
 // goes through its share again and writes the positions to where they belong.  Tokens below the block's rows are
 // counted on the way, so that no block waits for another.  Bound by the latency of a few dependent steps up to some
-// 16,384 tokens, whose shares stay in registers between the two passes; beyond, by instructions.
+// 16,384 tokens, whose shares stay in registers between the two passes; beyond, by instructions (51 per step of 32 tokens: 35 us
+// for 65,536 tokens, 61 for 131,072), where the second pass leaves out the steps without a token of the block's rows, four of five
+// with 148 blocks (the call with 131,072 tokens 114 -> 97 us).
 template <typename I>
 __global__ void __launch_bounds__(kGradSortWarps * 32)
     tokens_by_row_kernel(int tokens, const I *__restrict__ token, int64_t inctoken, int vocab, int own, int *__restrict__ ptr,
                          int *__restrict__ pos, int *__restrict__ row, int *__restrict__ joins) {
     extern __shared__ int s_count[];  // [warp][row]
     __shared__ int s_sum[kGradSortWarps], s_below[kGradSortWarps];
+    __shared__ unsigned short s_hits[kGradSortWarps][kGradGroups];
     let_next_begin();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int base = blockIdx.x * own;
     const int mine = min(own, vocab - base);
     if (blockIdx.x == 0 && threadIdx.x == 0) *joins = 0;  // the list of the sum begins empty
     const int share = (int)(((int64_t)tokens + kGradSortWarps * 32 - 1) / (kGradSortWarps * 32)) * 32;
-    const int64_t begin = min((int64_t)tokens, (int64_t)w * share), end = min((int64_t)tokens, begin + share);
+    const int begin = (int)min((int64_t)tokens, (int64_t)w * share), end = (int)min((int64_t)tokens, (int64_t)begin + share);
     int *count = s_count + w * own;
     int below = 0;
-    // the block's row of each token of this lane, -1 for none
-    int r[kGradAhead];
-    const auto request = [&](int64_t i0) {
-        I t[kGradAhead];
+    // 16 steps' tokens of this lane, of those steps that `steps` names; what cannot be a row of the table is the highest number
+    unsigned t[kGradAhead];
+    const auto request = [&](int i0, unsigned steps) {
+        I v[kGradAhead];
+        const I *p = token + (i0 + lane) * inctoken;
 #pragma unroll
-        for (int u = 0; u < kGradAhead; u++) {
-            const int64_t i = i0 + u * 32 + lane;
-            t[u] = i < end ? token[i * inctoken] : (I)-1;
+        for (int u = 0; u < kGradAhead; u++, p += 32 * inctoken) {
+            v[u] = (I)-1;
+            if ((steps >> u & 1) && i0 + u * 32 + lane < end) v[u] = *p;
         }
 #pragma unroll
-        for (int u = 0; u < kGradAhead; u++) r[u] = t[u] >= 0 && t[u] < (I)vocab ? (int)t[u] - base : INT_MIN;
+        for (int u = 0; u < kGradAhead; u++) {
+            if constexpr (sizeof(I) == 8) t[u] = (unsigned long long)v[u] >> 32 ? ~0u : (unsigned)v[u];
+            else t[u] = (unsigned)v[u];
+        }
     };
-    request(begin);
+    request(begin, ~0u);
     for (int i = threadIdx.x; i < kGradSortWarps * own; i += blockDim.x) s_count[i] = 0;
     __syncthreads();
-    for (int64_t i0 = begin; i0 < end; i0 += kGradAhead * 32) {
-        if (i0 != begin) request(i0);
+    unsigned hits = 0;  // the steps of the last group that hold a token of the block's rows
+    int group = 0;
+    for (int i0 = begin; i0 < end; i0 += kGradAhead * 32, group++) {
+        if (i0 != begin) request(i0, ~0u);
+        hits = 0;
 #pragma unroll
         for (int u = 0; u < kGradAhead; u++) {
-            if (r[u] < 0) below += r[u] != INT_MIN;
-            else if (r[u] < mine) atomicAdd(&count[r[u]], 1);
+            below += t[u] < (unsigned)base;
+            const bool in = t[u] - (unsigned)base < (unsigned)mine;
+            if (!__any_sync(0xffffffffu, in)) continue;
+            hits |= 1u << u;
+            if (in) atomicAdd(&count[t[u] - base], 1);
         }
+        if (lane == 0 && group < kGradGroups) s_hits[w][group] = (unsigned short)hits;
     }
     below = __reduce_add_sync(0xffffffffu, below);
     if (lane == 0) s_below[w] = below;
@@ -192,20 +207,25 @@ __global__ void __launch_bounds__(kGradSortWarps * 32)
         if (base + (int)threadIdx.x == vocab - 1) ptr[vocab] = start + total;
     }
     __syncthreads();
-    for (int64_t i0 = begin; i0 < end; i0 += kGradAhead * 32) {
-        if (share > kGradAhead * 32) request(i0);
+    group = 0;
+    for (int i0 = begin; i0 < end; i0 += kGradAhead * 32, group++) {
+        if (share > kGradAhead * 32) {
+            hits = group < kGradGroups ? s_hits[w][group] : ~0u;
+            request(i0, hits);
+        }
 #pragma unroll
         for (int u = 0; u < kGradAhead; u++) {
-            const bool in = r[u] >= 0 && r[u] < mine;
-            if (!__any_sync(0xffffffffu, in)) continue;
-            const unsigned same = __match_any_sync(0xffffffffu, in ? r[u] : -1);
+            if (!(hits >> u & 1)) continue;
+            const int r = (int)(t[u] - base);
+            const bool in = t[u] - (unsigned)base < (unsigned)mine;
+            const unsigned same = __match_any_sync(0xffffffffu, in ? r : -1);
             const int lower = __popc(same & ((1u << lane) - 1u));
-            const int at = in ? count[r[u]] + lower : 0;
+            const int at = in ? count[r] + lower : 0;
             __syncwarp();
             if (in) {
-                pos[at] = (int)(i0 + u * 32 + lane);
-                row[at] = base + r[u];
-                if (lower == 0) count[r[u]] += __popc(same);
+                pos[at] = i0 + u * 32 + lane;
+                row[at] = (int)t[u];
+                if (lower == 0) count[r] += __popc(same);
             }
             __syncwarp();
         }
@@ -495,8 +515,9 @@ extern "C" alphasparse_status_t alphasparse_cuda_embedding_grad(alphasparse_cuda
     char *space = static_cast<char *>(buffer);
     int *ptr = reinterpret_cast<int *>(space + sp.ptr), *pos = reinterpret_cast<int *>(space + sp.pos),
         *row = reinterpret_cast<int *>(space + sp.row);
-    // as many blocks as there are SMs, while their counts fit shared memory
-    const int own = (int)std::min<int64_t>(kGradMostRows, ((vocab + 147) / 148 + 31) / 32 * 32);
+    // as many blocks as there are SMs, while their counts fit shared memory, however few rows that leaves each: the fewer it has,
+    // the more steps its second pass leaves out (300 rows, 131,072 tokens: 10 blocks of 32 rows 118 us, 100 of 3 97)
+    const int own = (int)std::min<int64_t>(kGradMostRows, (vocab + 147) / 148);
     const unsigned blocks = (unsigned)((vocab + own - 1) / own);
     const size_t smem = sizeof(int) * kGradSortWarps * (size_t)own;
     const auto sort = [&](auto i) {

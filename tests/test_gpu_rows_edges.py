@@ -4,8 +4,7 @@ import pytest
 import torch
 
 from alsparse_b200 import spblas
-
-from tests.rows_util import TYPES, U, assert_within, floor_of, gen, half_step, normal, ok, strided, untouched
+from rows_util import TYPES, U, assert_within, buffer_of, floor_of, gen, half_step, normal, ok, strided, untouched
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +99,25 @@ def test_the_widest_rows(width):
     ok(spblas.expert_combine_grad(x, x, slot, weight, y, dweight))
     assert torch.equal(x * 0.5, y)
     assert_within(dweight, (x.double() ** 2).sum()[None, None], U * (width / 256 + 32) * (x.double() ** 2).sum())  # 256 threads' sums
+
+
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("count,vocab", [(16_385, 90_000), (20_000, 700), (100_003, 151), (100_003, 160_000), (4_300_001, 700)])
+def test_gradient_of_many_tokens(index, count, vocab):
+    g = gen(count)
+    tokens = torch.randint(-vocab // 10, vocab + vocab // 10, (2 * count,), generator=g, device="cuda")
+    tokens[: count // 2] = tokens[: count // 2] % 7 * (vocab // 8)  # a few rows of many tokens
+    tokens[-4:] = torch.tensor([vocab, -1, 2**31 - 1, -2**31], device="cuda")
+    if index is torch.int64:
+        tokens[:8] = torch.tensor([2**32, -2**32, 2**32 + 5, -2**63, 2**63 - 1, 2**40, vocab - 1, 0], device="cuda")
+    tokens = tokens.to(index)[::2]
+    inside = (tokens >= 0) & (tokens < vocab)
+    dy, dtable = normal(g, count, 3), torch.full((vocab, 3), float("nan"), device="cuda")
+    buffer = buffer_of(spblas.embedding_grad_buffer_size(count, vocab, 3))
+    ok(spblas.embedding_grad(tokens, dy, 1.0, 0.0, dtable, buffer))
+    exact, size, terms = (torch.zeros(vocab, 3, dtype=torch.float64, device="cuda") for _ in range(3))
+    at = tokens[inside].long()
+    exact.index_add_(0, at, dy[inside].double())
+    size.index_add_(0, at, dy[inside].double().abs())
+    terms.index_add_(0, at, torch.ones_like(dy[inside], dtype=torch.float64))
+    assert_within(dtable, exact, U * (terms + 2) * size)  # any order of a row's terms
