@@ -172,7 +172,7 @@ __device__ __forceinline__ uint4 load_if(const void *p, bool there) {
 
 // 16 bytes as load_any gives them, in two parts: the two aligned vectors are requested without a branch, so that several are on
 // their way at once, and shifted together when they are needed.  `there` false: zeros.  (Experts' products of 32,768 x 1001 x 1439,
-// 16 experts: 1346 us with load_any and eight warps, 876 us so, about 850 with fourteen.  The kernels on rows, which have more
+// 16 experts: 1346 us with load_any and eight warps, 876 us so, about 870 with fourteen.  The kernels on rows, which have more
 // blocks to hide latency, lose by the registers: combine of rows of 2047 94 -> 127 us.)
 template <typename T>
 struct AnyPack {
