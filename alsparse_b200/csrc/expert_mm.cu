@@ -16,6 +16,7 @@
 
 #include <algorithm>
 
+#include "expert_tiles.h"
 #include "rows.h"
 
 namespace asb {
@@ -424,7 +425,7 @@ __device__ __forceinline__ MmTile mm_tile(const MmShape &s, const int *s_first, 
         q.expert = expert_of(s_first, s.experts, r);
         q.lo = s_begin[q.expert], hi = max(q.lo, s_begin[q.expert + 1]);
         // equal shares of the expert's rows
-        const int tiles = s_first[q.expert + 1] - s_first[q.expert], share = ((hi - q.lo + tiles - 1) / tiles + unit - 1) / unit * unit;
+        const int share = equal_share(hi - q.lo, s_first[q.expert + 1] - s_first[q.expert], unit);
         q.n0 = q.lo + (r - s_first[q.expert]) * share;
         q.length = min(share, hi - q.n0);
         q.n = (q.length + unit - 1) / unit * unit;
