@@ -153,7 +153,6 @@ constexpr int kMmThreads = 384;  // copies, products, eight warps for the accumu
 constexpr int kMmCopyWarps = 14;  // ANY: after the others, instead of the two for ragged ends
 constexpr int kMmThreadsAny = 320 + 32 * kMmCopyWarps;
 constexpr int kMmM = 128, kMmK = 64;
-constexpr int kMmMostStages = 8;
 constexpr unsigned long long kMmLimitNs = 2000000000ull;
 
 __device__ __forceinline__ unsigned smem_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -452,7 +451,7 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
     constexpr unsigned a_bytes = kMmM * kMmK * sizeof(T);
     extern __shared__ __align__(16) char s_raw[];
     __shared__ int s_first[kMostExperts + 1], s_begin[kMostExperts + 1];  // row tiles before an expert; the offsets, clamped
-    __shared__ uint64_t s_full[kMmMostStages], s_empty[kMmMostStages], s_own[kMmMostStages], s_ready[kMmMostStages], s_acc_full[2], s_acc_empty[2];
+    __shared__ uint64_t s_full[kMmMostStages], s_empty[kMmMostStages], s_own[2 * kMmMostStages], s_ready[kMmMostStages], s_acc_full[2], s_acc_empty[2];
     __shared__ unsigned s_tmem;
     __shared__ int s_stop_word;
     volatile int *s_stop = &s_stop_word;
@@ -470,7 +469,8 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
                 asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
                 if (b_k) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_c) : "memory");
             }
-            for (int i = 0; i < s.stages; i++) barrier_init(&s_full[i], ANY ? kMmCopyWarps : 1), barrier_init(&s_empty[i], 1), barrier_init(&s_own[i], 1), barrier_init(&s_ready[i], PAIR ? 2 : 1);
+            for (int i = 0; i < s.stages; i++) barrier_init(&s_full[i], ANY ? kMmCopyWarps : 1), barrier_init(&s_empty[i], 1), barrier_init(&s_ready[i], PAIR ? 2 : 1);
+            for (int i = 0; i < 2 * kMmMostStages; i++) barrier_init(&s_own[i], 1);
             for (int i = 0; i < 2; i++) barrier_init(&s_acc_full[i], 1), barrier_init(&s_acc_empty[i], PAIR ? 16 : 8);
             s_stop_word = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -499,6 +499,7 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
     if (w == 0) {
         int stage = 0;
         unsigned phase = 0;
+        EndTurn turn;
         bool good = !ANY;
         for (int t = worker; good && t < tiles; t += workers) {
             const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
@@ -522,10 +523,12 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
                     }
                     for (int g = 0; g < narrow; g++) copy_tile<B>(b + wide * 8192 + g * 2048, &map_c, k0, n0 + wide * 64 + g * 16, 0, barrier);
                 };
+                const bool end = !ANY && FORM == kGradient && ragged(q, k);
+                uint64_t *own = &s_own[end ? end_barrier(turn.take(), stage) : 0];
                 if (elect_one()) {
-                    if (!ANY && FORM == kGradient && ragged(q, k)) {
-                        barrier_expect(&s_own[stage], bytes);
-                        copy(std::false_type{}, smem_address(&s_own[stage]));
+                    if (end) {
+                        barrier_expect(own, bytes);
+                        copy(std::false_type{}, smem_address(own));
                     } else if (PAIR) {
                         if (rank == 0) barrier_expect(&s_full[stage], 2 * bytes);
                         copy(std::true_type{}, address_in_first(&s_full[stage]));
@@ -653,19 +656,18 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
         // the copy.  Zeros in both operands up to the next multiple, so that nothing that stands there, NaN included, gets
         // into the sum; then the first block's products may go on.  Two warps in turn: one alone takes 1.7 us a tile, of which its
         // fence and arrival are most, and the rest of a short tile 1.0.
-        int stage = 0, turn = w & 1;
+        int stage = 0;
         unsigned own_phases = 0;  // a bit for each stage: the phase that comes next
+        EndTurn turn;
         bool good = true;
         for (int t = worker; good && t < tiles; t += workers) {
             const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
             const int last = q.steps - 1, left = q.length - last * kMmK;
             if (q.steps > 0 && ragged(q, last)) {
                 const int at = (stage + last) % s.stages;
-                // both wait for every one: a phase that is not waited for would be taken for the one after the next
-                if (!(good = warp_wait(&s_own[at], own_phases >> at & 1, s_stop, q.steps))) break;
-                own_phases ^= 1u << at;
-                turn ^= 1;
-                if (turn) {
+                if (turn.take() == (w & 1)) {
+                    if (!(good = warp_wait(&s_own[end_barrier(w & 1, at)], own_phases >> at & 1, s_stop, q.steps))) break;
+                    own_phases ^= 1u << at;
                     char *a = ring + (size_t)at * s.stage_bytes;
                     const int end = ((left + 15) / 16 * 16 - left) * 8, boxes = 2 + (((PAIR ? q.n >> 1 : q.n) + 63) >> 6);
                     for (int box = 0; box < boxes; box++)
