@@ -153,7 +153,6 @@ constexpr int kMmThreads = 384;  // copies, products, eight warps for the accumu
 constexpr int kMmCopyWarps = 14;  // ANY: after the others, instead of the two for ragged ends
 constexpr int kMmThreadsAny = 320 + 32 * kMmCopyWarps;
 constexpr int kMmM = 128, kMmK = 64;
-constexpr unsigned long long kMmLimitNs = 2000000000ull;
 
 __device__ __forceinline__ unsigned smem_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void barrier_init(uint64_t *b, unsigned count) {
@@ -180,11 +179,11 @@ __device__ __forceinline__ unsigned long long now_ns() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-// Waits for the phase of the given parity; false when it ran out of time or another thread of the block did.  `steps`: of a
-// product that has to be done first, a hundredth of a millisecond more for each.  CLUSTER: what the
-// pair's other block wrote before it arrived is seen (dear: about a microsecond).
+// Waits for the phase of the given parity; false when it ran out of time or another thread of the block did.  `work`: what the
+// block may have to do first (tile_work).  CLUSTER: what the pair's other block wrote before it arrived is seen (dear: about a
+// microsecond).
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool barrier_wait(uint64_t *b, unsigned parity, volatile int *s_stop, int steps = 0) {
+__device__ __forceinline__ bool barrier_wait(uint64_t *b, unsigned parity, volatile int *s_stop, long long work) {
     unsigned long long begin = 0;
     for (unsigned i = 0;; i++) {
         unsigned done;
@@ -203,7 +202,7 @@ __device__ __forceinline__ bool barrier_wait(uint64_t *b, unsigned parity, volat
             if (*s_stop) return false;
             const unsigned long long t = now_ns();
             if (!begin) begin = t;
-            else if (t - begin > kMmLimitNs + (unsigned long long)steps * 10000) {
+            else if (t - begin > wait_limit_ns(work)) {
                 *s_stop = 1;
                 return false;
             }
@@ -212,8 +211,8 @@ __device__ __forceinline__ bool barrier_wait(uint64_t *b, unsigned parity, volat
 }
 // ... by a whole warp, with one answer for all lanes
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool warp_wait(uint64_t *b, unsigned parity, volatile int *s_stop, int steps = 0) {
-    return __all_sync(0xffffffffu, barrier_wait<CLUSTER>(b, parity, s_stop, steps));
+__device__ __forceinline__ bool warp_wait(uint64_t *b, unsigned parity, volatile int *s_stop, long long work) {
+    return __all_sync(0xffffffffu, barrier_wait<CLUSTER>(b, parity, s_stop, work));
 }
 // PAIR: `barrier` is an address of the cluster's, the other block's too
 template <bool PAIR>
@@ -495,6 +494,7 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = s_tmem;
     const int tiles = FORM == kGradient ? s.experts * s.m_tiles * s.n_tiles : s_first[s.experts] * s.m_tiles;
+    long long work = 0;  // of this warp's tiles so far, for the limits of its waits
 
     if (w == 0) {
         int stage = 0;
@@ -503,12 +503,13 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
         bool good = !ANY;
         for (int t = worker; good && t < tiles; t += workers) {
             const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
+            work += tile_work(q.steps);
             const int half = PAIR ? q.n >> 1 : q.n, m0 = q.m0 + rank * kMmM, n0 = q.n0 + rank * half;
             // kRows: boxes of 64 rows, then of 16; kGradient: boxes of 64 columns
             const int wide = b_k ? half >> 6 : (half + 63) >> 6, narrow = b_k ? (half & 63) >> 4 : 0;
             const unsigned bytes = a_bytes + (unsigned)wide * 8192u + (unsigned)narrow * 2048u;
             for (int k = 0; k < q.steps; k++) {
-                if (!(good = warp_wait(&s_empty[stage], phase ^ 1, s_stop))) break;
+                if (!(good = warp_wait(&s_empty[stage], phase ^ 1, s_stop, work))) break;
                 char *a = ring + (size_t)stage * s.stage_bytes, *b = a + a_bytes;
                 const int k0 = k * kMmK;
                 const auto copy = [&](auto both, unsigned barrier) {
@@ -547,9 +548,10 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
         bool good = true;
         for (int t = worker; good && t < tiles; t += workers) {
             const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
+            work += tile_work(q.steps);
             if (q.steps == 0) continue;
             const int slot = count & 1;
-            if (!(good = barrier_wait(&s_acc_empty[slot], ((count >> 1) & 1) ^ 1, s_stop))) break;
+            if (!(good = barrier_wait(&s_acc_empty[slot], ((count >> 1) & 1) ^ 1, s_stop, work))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             count++;
             const int length = FORM == kGradient ? q.length : s.reduced;
@@ -559,10 +561,10 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
                 char *a = ring + (size_t)stage * s.stage_bytes;
                 const int left = length - k * kMmK, parts = min(4, (left + 15) / 16);
                 if (!ANY && FORM == kGradient && ragged(q, k)) {
-                    if (!(good = barrier_wait<true>(&s_ready[stage], ready_phases >> stage & 1, s_stop))) break;
+                    if (!(good = barrier_wait<true>(&s_ready[stage], ready_phases >> stage & 1, s_stop, work))) break;
                     ready_phases ^= 1u << stage;
                 } else {
-                    if (!(good = barrier_wait(&s_full[stage], full_phases >> stage & 1, s_stop))) break;
+                    if (!(good = barrier_wait(&s_full[stage], full_phases >> stage & 1, s_stop, work))) break;
                     full_phases ^= 1u << stage;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -584,9 +586,10 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
         int count = 0;
         for (int t = worker; t < tiles; t += workers) {
             const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
+            work += tile_work(q.steps);
             const int slot = count & 1, m = q.m0 + rank * kMmM + part * 32;
             if (q.steps > 0) {
-                if (!warp_wait(&s_acc_full[slot], (count >> 1) & 1, s_stop, q.steps)) break;
+                if (!warp_wait(&s_acc_full[slot], (count >> 1) & 1, s_stop, work)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 count++;
             }
@@ -629,8 +632,9 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
         bool good = true;
         for (int t = worker; good && t < tiles; t += workers) {
             const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
+            work += tile_work(q.steps);
             for (int k = 0; k < q.steps; k++) {
-                if (!(good = warp_wait(&s_empty[stage], phase ^ 1, s_stop))) break;
+                if (!(good = warp_wait(&s_empty[stage], phase ^ 1, s_stop, work))) break;
                 char *a = ring + (size_t)stage * s.stage_bytes, *b = a + a_bytes;
                 const int k0 = k * kMmK, m_there = s.m_size - q.m0;
                 const T *pa = static_cast<const T *>(s.a), *pb = static_cast<const T *>(s.b);
@@ -662,11 +666,12 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
         bool good = true;
         for (int t = worker; good && t < tiles; t += workers) {
             const MmTile q = mm_tile<FORM, PAIR>(s, s_first, s_begin, t);
+            work += tile_work(q.steps);
             const int last = q.steps - 1, left = q.length - last * kMmK;
             if (q.steps > 0 && ragged(q, last)) {
                 const int at = (stage + last) % s.stages;
                 if (turn.take() == (w & 1)) {
-                    if (!(good = warp_wait(&s_own[end_barrier(w & 1, at)], own_phases >> at & 1, s_stop, q.steps))) break;
+                    if (!(good = warp_wait(&s_own[end_barrier(w & 1, at)], own_phases >> at & 1, s_stop, work))) break;
                     own_phases ^= 1u << at;
                     char *a = ring + (size_t)at * s.stage_bytes;
                     const int end = ((left + 15) / 16 * 16 - left) * 8, boxes = 2 + (((PAIR ? q.n >> 1 : q.n) + 63) >> 6);

@@ -312,8 +312,8 @@ alphasparse_status_t alphasparse_cuda_expert_mm_grad(alphasparse_cuda_type_t typ
                                                      int64_t in, const void *dy, int64_t lddy, const void *x,
                                                      int64_t ldx, float beta, void *dw, int64_t ldw, int64_t stride_w);
 
-/* The kernels of the two calls above wait for their copies, each wait for two seconds at most (and 10 us for each 64
- * terms of a sum that has to be done first).  Waits for the library stream
+/* The kernels of the two calls above wait for their copies, each wait for two seconds at most, and 10 us for each 64 terms
+ * and 320 us for each tile of the output that may have to be done first.  Waits for the library stream
  * and stores 1 if such a wait has run out on the current device (the outputs of that call are not complete), else 0;
  * clear != 0 resets it. */
 alphasparse_status_t alphasparse_cuda_expert_mm_status(int *status, int clear);

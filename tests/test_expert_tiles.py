@@ -1,6 +1,7 @@
 """What the experts' products compute about their tiles (csrc/expert_tiles.h), compiled for the host: the sizes at the limits are
 too large to be run."""
 import os
+import re
 import subprocess
 
 from alsparse_b200 import build
@@ -116,3 +117,43 @@ def test_a_warp_that_is_held_back_misses_no_end(tmp_path):
     run_on_host(tmp_path, TURNS)
     kernel = open(os.path.join(build.CSRC, "expert_mm.cu")).read()
     assert kernel.count("turn.take()") == 2 and kernel.count("end_barrier(") == 2  # the copies and the clearing warps
+
+
+LIMITS = r"""
+#include <stdio.h>
+#include <stdlib.h>
+#include "expert_tiles.h"
+using namespace asb;
+// Tiles of a block one after the other, some with long sums that no end is cleared in, some of experts without rows: whoever waits
+// for something of a tile waits longer than all that stands before it takes, at five times the time measured for a step and a tile.
+int main() {
+    long long wrong = 0;
+    const int steps[] = {0, 0, 0, 1, 8, 300, 8192, 33554432};  // the last: an expert of 2^31 rows
+    for (int i = 0; i < 100000; i++) {
+        long long work = 0;
+        double before_us = 0;
+        for (int t = 0; t < 30; t++) {
+            const int n = steps[rand() % 8];
+            work += tile_work(n);
+            before_us += 5 * (0.3 * n + 32);
+            wrong += wait_limit_ns(work) < before_us * 1000.0 || wait_limit_ns(work) < 2000000000ull;
+        }
+    }
+    // 524,288 rows of an expert, 221 tiles of 65,536 x 65,536 a pair, then one short expert with an end: 8192 steps each
+    long long work = 0;
+    for (int t = 0; t < 221 * 4; t++) work += tile_work(8192);
+    wrong += wait_limit_ns(work + tile_work(1)) < 3000000000ull;
+    printf("%lld\n", wrong);
+    return wrong != 0;
+}
+"""
+
+
+def test_a_wait_lasts_as_long_as_what_comes_before_it(tmp_path):
+    run_on_host(tmp_path, LIMITS)
+    kernel = open(os.path.join(build.CSRC, "expert_mm.cu")).read()
+    body = kernel[kernel.index("    expert_mm_kernel("):kernel.index("typedef CUresult")]
+    waits = re.findall(r"(?:warp|barrier)_wait(?:<true>)?\((.*)\)", body)
+    assert len(waits) == 7 and all("s_stop, work)" in w for w in waits), waits
+    roles = re.findall(r"mm_tile<FORM, PAIR>\(s, s_first, s_begin, t\);\n(.*)", body)
+    assert len(roles) == 5 and all(r.strip() == "work += tile_work(q.steps);" for r in roles), roles
