@@ -23,6 +23,11 @@ namespace asb {
 
 // Set by a kernel whose bounded wait ran out (alphasparse_cuda_expert_mm_status).
 static __device__ int g_expert_mm_status;
+// What a call to it reads.  Read and cleared in one step, so that no failure falls between the two.
+static __device__ int g_expert_mm_told;
+static __global__ void tell_status_kernel(int clear) {
+    g_expert_mm_told = clear ? atomicExch(&g_expert_mm_status, 0) : atomicAdd(&g_expert_mm_status, 0);
+}
 
 // D[m, n] = sum over k of A[m, k] B[n, k].  What the three dimensions are:
 enum MmForm {
@@ -946,10 +951,20 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_mm_grad(alphasparse_cuda
 extern "C" alphasparse_status_t alphasparse_cuda_expert_mm_status(int *status, int clear) {
     if (!status) return ALPHA_SPARSE_STATUS_NOT_INITIALIZED;
     cudaStream_t st = current_stream();
+    if (being_captured(st)) {  // it waits; and refused here, the capture goes on
+        record_error("alphasparse_cuda_expert_mm_status: the library stream is being captured");
+        return ALPHA_SPARSE_STATUS_EXECUTION_FAILED;
+    }
+    static std::mutex one_at_a_time;  // the word for the host is one per device
+    std::lock_guard<std::mutex> lock(one_at_a_time);
     void *word = nullptr;
-    ASB_CUDA_OR(cudaGetSymbolAddress(&word, g_expert_mm_status), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
-    ASB_CUDA_OR(cudaMemcpyAsync(status, word, sizeof(int), cudaMemcpyDeviceToHost, st), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    ASB_CUDA_OR(cudaGetSymbolAddress(&word, g_expert_mm_told), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    tell_status_kernel<<<1, 1, 0, st>>>(clear);
+    ASB_CUDA_OR(cudaGetLastError(), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    count_launch();
+    int told = 0;
+    ASB_CUDA_OR(cudaMemcpyAsync(&told, word, sizeof(int), cudaMemcpyDeviceToHost, st), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
     ASB_CUDA_OR(cudaStreamSynchronize(st), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
-    if (clear) ASB_CUDA_OR(cudaMemsetAsync(word, 0, sizeof(int), st), ALPHA_SPARSE_STATUS_EXECUTION_FAILED);
+    *status = told;
     return ALPHA_SPARSE_STATUS_SUCCESS;
 }

@@ -473,7 +473,7 @@ def expert_mm_grad(offsets, dy, x, beta, dw):
 
 
 def expert_mm_status(clear=False):
-    """alphasparse_cuda_expert_mm_status: (status, 1 if a wait of a product ran out)."""
+    """alphasparse_cuda_expert_mm_status: (status, 1 if a wait of any product on the current device ran out since it was last cleared)."""
     v = C.c_int()
     st = capi.load().alphasparse_cuda_expert_mm_status(C.byref(v), 1 if clear else 0)
     return st, v.value

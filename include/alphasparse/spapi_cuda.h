@@ -202,7 +202,7 @@ alphasparse_status_t alphasparse_d_mv_exchange(const double alpha, const alphasp
  *
  * All of them: every pointer is memory of the current device (or managed), else ALPHA_SPARSE_STATUS_INVALID_POINTER;
  * work is enqueued on the library stream and the call returns without waiting; nothing is allocated, kept from call to
- * call or shared between calls (workspaces are the caller's: two calls that may overlap, and two captured graphs that
+ * call or shared between calls but the word of alphasparse_cuda_expert_mm_status (workspaces are the caller's: two calls that may overlap, and two captured graphs that
  * may run at the same time, take two), so the calls can be captured.  Dense operands are row-major with a leading
  * dimension of at most 2^31 - 1 elements and any alignment that their elements allow; 16-byte aligned rows are fastest.
  * A missing operand is ALPHA_SPARSE_STATUS_NOT_INITIALIZED; sizes and enums out of range, leading dimensions below
@@ -314,8 +314,10 @@ alphasparse_status_t alphasparse_cuda_expert_mm_grad(alphasparse_cuda_type_t typ
 
 /* The kernels of the two calls above wait for their copies, each wait for two seconds at most, and 10 us for each 64 terms
  * and 320 us for each tile of the output that may have to be done first.  Waits for the library stream
- * and stores 1 if such a wait has run out on the current device (the outputs of that call are not complete), else 0;
- * clear != 0 resets it. */
+ * and stores 1 if such a wait has run out on the current device since the last call with clear != 0 (the outputs of that
+ * product are not complete), else 0; clear != 0 resets it in the same step.  There is one such word per device, for the
+ * products of all streams, threads and replayed graphs of the process: it names no call, and of several callers that clear it one
+ * is told.  Refused (EXECUTION_FAILED) while the library stream is being captured. */
 alphasparse_status_t alphasparse_cuda_expert_mm_status(int *status, int clear);
 
 /* Error word of a handle's kernels.  Kernels that wait (the row-tile kernel waits for its bulk copies) give up
