@@ -716,15 +716,15 @@ typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, 
                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 static EncodeTiled encode_tiled() {
-    static const EncodeTiled f = [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
-            found != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<EncodeTiled>(p);
-    }();
-    return f;
+    static std::atomic<void *> known{nullptr};  // once it was found
+    void *p = known.load();
+    if (p) return reinterpret_cast<EncodeTiled>(p);
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+        return nullptr;
+    known.store(p);
+    return reinterpret_cast<EncodeTiled>(p);
 }
 
 // `width` x `rows` x `count` elements of 16 bits, boxes of 64 x box_rows
@@ -736,9 +736,16 @@ static bool make_map(CUtensorMap *map, alphasparse_cuda_type_t type, const void 
     // distances of dimensions of one element are never used, but have to be legal
     const cuuint64_t strides[2] = {(cuuint64_t)(rows > 1 ? ld * 2 : (width * 2 + 15) / 16 * 16), (cuuint64_t)(count > 1 ? stride * 2 : 16)};
     const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
-    return f(map, type == ALPHA_SPARSE_CUDA_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-             const_cast<void *>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const auto encode = [&] {
+        return f(map, type == ALPHA_SPARSE_CUDA_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                 const_cast<void *>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    if (encode()) return true;
+    // In a thread whose first call this is nothing has made the device's context current yet, which the runtime does by itself
+    // and this function of the driver does not.
+    int dev = -1;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encode();
 }
 
 static bool takes_tma(const void *p, int64_t ld, int64_t rows, int64_t stride, int64_t count) {

@@ -52,3 +52,23 @@ def test_status_from_several_threads():
     for t in threads:
         t.join()
     assert seen == [(capi.SUCCESS, 0)] * 800
+
+
+@pytest.mark.parametrize("which", ["product", "gradient", "status"])
+def test_first_call_of_a_thread(which):
+    """Nothing else of CUDA has been called in it."""
+    offsets, x, w, y = _product(gen(2), 64)
+    dw = torch.zeros(4, 64, 64, device="cuda")
+    call = {"product": lambda: spblas.expert_mm(capi.TRANSPOSE, offsets, x, w, y), "gradient": lambda: spblas.expert_mm_grad(offsets, y, x, 0.0, dw),
+            "status": lambda: spblas.expert_mm_status()[0]}[which]
+    torch.cuda.synchronize()
+    seen = []
+    thread = threading.Thread(target=lambda: seen.append((call(), spblas.last_error())))
+    thread.start()
+    thread.join()
+    assert seen[0][0] == capi.SUCCESS, seen
+    torch.cuda.synchronize()
+    if which == "product":
+        here = torch.zeros_like(y)
+        ok(spblas.expert_mm(capi.TRANSPOSE, offsets, x, w, here))
+        assert torch.equal(here, y)
