@@ -777,7 +777,8 @@ static cudaError_t launch_mm(alphasparse_cuda_type_t type, MmShape s, int64_t mo
     const int smem = 1024 + s.stages * (int)s.stage_bytes;
     int sms = 0;
     cudaError_t e = multiprocessors(&sms);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // the most that any call takes, the same from every thread: a call with small stages must not lower it under another's launch
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute cluster[1];
     cluster[0].id = cudaLaunchAttributeClusterDimension;

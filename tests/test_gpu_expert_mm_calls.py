@@ -72,3 +72,66 @@ def test_first_call_of_a_thread(which):
         here = torch.zeros_like(y)
         ok(spblas.expert_mm(capi.TRANSPOSE, offsets, x, w, here))
         assert torch.equal(here, y)
+
+
+@pytest.mark.parametrize("op", [capi.TRANSPOSE, capi.NON_TRANSPOSE])
+def test_threads_with_different_sizes(op):
+    """Few rows an expert and more of them take tiles, and shared memory, of different sizes."""
+    calls = [_product(gen(rows), rows) for rows in (32, 128, 240, 32)]
+    want = []
+    for c in calls:
+        ok(spblas.expert_mm(op, *c))
+        want.append(c[3].clone())
+        c[3].zero_()
+    torch.cuda.synchronize()
+    refused = []
+
+    def work(c):
+        for _ in range(4000):
+            status = spblas.expert_mm(op, *c)
+            if status != capi.SUCCESS:
+                refused.append((status, spblas.last_error()))
+
+    threads = [threading.Thread(target=work, args=(c,)) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not refused, (len(refused), refused[0])
+    for c, y in zip(calls, want):
+        assert torch.equal(c[3], y)
+
+
+@pytest.mark.parametrize("out_type", [torch.bfloat16, torch.float32])
+def test_threads_with_different_gradients(out_type):
+    """Narrow and wide columns of dy: stages of different sizes."""
+    calls = []
+    for out in (32, 96, 256):
+        g = gen(out)
+        offsets = torch.tensor([0, 20, 20, 70], dtype=torch.int32, device="cuda")
+        calls.append((offsets, normal(g, 70, out, dtype=torch.bfloat16), normal(g, 70, 64, dtype=torch.bfloat16), 0.0,
+                      torch.zeros(3, out, 64, dtype=out_type, device="cuda")))
+    want = []
+    for c in calls:
+        ok(spblas.expert_mm_grad(*c))
+        want.append(c[4].clone())
+        c[4].zero_()
+    torch.cuda.synchronize()
+    refused = []
+
+    def work(c):
+        for _ in range(4000):
+            status = spblas.expert_mm_grad(*c)
+            if status != capi.SUCCESS:
+                refused.append((status, spblas.last_error()))
+
+    threads = [threading.Thread(target=work, args=(c,)) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not refused, (len(refused), refused[0])
+    for c, d in zip(calls, want):
+        assert torch.equal(c[4], d)
