@@ -258,10 +258,9 @@ constexpr int kJoinTile = 128;
 // what is there else.
 template <typename T, typename TO, int N, bool BETA>
 __global__ void __launch_bounds__(kGradThreads)
-    embedding_grad_kernel(int pieces, int tiles, int nv, int vocab, const int *__restrict__ ptr, const int *__restrict__ pos,
-                          const int *__restrict__ row, const T *__restrict__ dy, int64_t lddy, float alpha, float beta,
-                          TO *__restrict__ dtable, int64_t ldt, float *__restrict__ partial, int64_t ldp, int *__restrict__ joins,
-                          Join *__restrict__ join) {
+    embedding_grad_kernel(int pieces, int tiles, int nv, int vocab, const int *ptr, const int *pos, const int *row,
+                          const T *__restrict__ dy, int64_t lddy, float alpha, float beta, TO *__restrict__ dtable, int64_t ldt,
+                          float *partial, int64_t ldp, int *joins, Join *join) {
     after_previous();
     let_next_begin();
     const int64_t sums = (int64_t)pieces * tiles;
@@ -345,7 +344,7 @@ __global__ void __launch_bounds__(kGradThreads)
 template <typename TO>
 __global__ void __launch_bounds__(kJoinWarps * 32)
     embedding_grad_join_kernel(float alpha, float beta, TO *__restrict__ dtable, int64_t ldt,
-                               const float *__restrict__ partial, int64_t ldp, const int *__restrict__ joins, const Join *__restrict__ join) {
+                               const float *partial, int64_t ldp, const int *joins, const Join *join) {
     __shared__ float4 s_sum[kJoinWarps][32];
     after_previous();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, count = *joins;

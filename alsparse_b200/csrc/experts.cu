@@ -43,7 +43,7 @@ __device__ __forceinline__ int plan_scan(int v, int *s_sum) {
 template <bool PLACE>
 __global__ void __launch_bounds__(kPlanThreads)
     plan_kernel(int64_t pairs, int64_t share, int experts, int k, const int *__restrict__ index, int64_t ldi,
-                int *__restrict__ counts, int *__restrict__ offsets, int *__restrict__ slot, int64_t lds) {
+                int *counts, int *__restrict__ offsets, int *__restrict__ slot, int64_t lds) {
     extern __shared__ int s_count[];  // [warp][expert]
     __shared__ int s_sum[kPlanWarps];
     __shared__ int s_total[kPlanThreads], s_before[kPlanThreads];

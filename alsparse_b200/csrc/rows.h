@@ -229,7 +229,9 @@ inline int64_t most_pieces(int64_t width, size_t elem) { return width * (int64_t
 
 // A kernel that begins with after_previous(): its blocks may be made resident while the kernel before it on the stream ends
 // (as soon as that one has called let_next_begin or its blocks are done), and wait there until its writes are complete.
-// Saves about two microseconds between the kernels of one call.
+// Saves about two microseconds between the kernels of one call.  What the kernel before it writes is taken by plain pointers:
+// behind `const ... __restrict__` the compiler may use loads that demand memory which nobody writes while the kernel lives, and
+// may move them before the wait.
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 template <typename... P, typename... A>

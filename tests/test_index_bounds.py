@@ -50,3 +50,18 @@ def test_kernels_request_ahead_through_the_bounds(kernel):
     for name in ("from", "k0", "kg", "r"):
         sums = re.findall(r"\b%s \+ [^;?]*(?:<=?) *(?:k_end|r_end|min\()" % name, body)
         assert not sums, sums
+
+
+def test_what_the_kernel_before_writes_is_not_promised_to_stand_still():
+    """A kernel that is made resident before its predecessor is done takes that one's results by pointers without __restrict__."""
+    source = "".join(open(os.path.join(build.CSRC, f)).read() for f in build.CUDA_SOURCES)
+    written = {"embedding_grad_kernel": ("ptr", "pos", "row", "partial", "joins", "join"), "embedding_grad_join_kernel": ("partial", "joins", "join"),
+               "plan_kernel": ("counts",)}
+    kernels = re.findall(r"\b(\w+)\(([^{;()]*)\) \{\n(.*?)\n\}\n", source, re.S)
+    behind = {name: args for name, args, body in kernels if "after_previous()" in body}
+    assert set(behind) == set(written)
+    for name, args in behind.items():
+        args = [" ".join(a.split()) for a in args.split(",")]
+        for pointer in written[name]:
+            found = [a for a in args if re.search(r"\b%s$" % pointer, a)]
+            assert len(found) == 1 and "__restrict__" not in found[0], (name, pointer, found)
