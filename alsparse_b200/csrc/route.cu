@@ -119,7 +119,8 @@ __device__ __forceinline__ unsigned best_groups(const RouteShape &sh, const F *s
             if (o > first) second = first, v2 = v1, first = o, v1 = v;
             else if (o > second) second = o, v2 = v;
         }
-        *value = BIAS && second != 0 ? v1 + v2 : v1;
+        // half the sum of two keys, which no finite ones take out of range
+        *value = BIAS ? F(.5) * v1 + (second != 0 ? F(.5) * v2 : F(0)) : v1;
         worth = first == 0 ? 0 : order_of(*value);
     }
     int ahead = 0;
@@ -174,7 +175,7 @@ __device__ __forceinline__ bool choose(const RouteShape &sh, const float (&x)[I]
             // the last group that is in and the first that is not
             const unsigned in = __ballot_sync(kAll, rank == sh.top_groups - 1), out = __ballot_sync(kAll, rank == sh.top_groups);
             const float a = (float)__shfl_sync(kAll, value, __ffs(in) - 1), b = (float)__shfl_sync(kAll, value, __ffs(out) - 1);
-            if (!apart(.5f * a, .5f * b) && b != -INFINITY) return false;  // sums of two keys: twice as far off
+            if (!apart(a, b) && b != -INFINITY) return false;
         }
         group = group0, within = within0;
 #pragma unroll
@@ -288,7 +289,7 @@ __device__ __forceinline__ bool choose_sorted(const RouteShape &sh, const float 
         if (BIAS) {
             const unsigned in = __ballot_sync(kAll, rank == sh.top_groups - 1), out = __ballot_sync(kAll, rank == sh.top_groups);
             const float a = __shfl_sync(kAll, value, __ffs(in) - 1), b = __shfl_sync(kAll, value, __ffs(out) - 1);
-            if (!apart(.5f * a, .5f * b) && b != -INFINITY) return false;  // sums of two keys: twice as far off
+            if (!apart(a, b) && b != -INFINITY) return false;
         }
         group = group0, within = within0;
 #pragma unroll
@@ -312,7 +313,7 @@ __device__ __forceinline__ bool choose_sorted(const RouteShape &sh, const float 
         }
         unsigned worth = first;
         if (BIAS) {
-            worth = order_of(key_of(first) + (second != 0 ? key_of(second) : 0.f));
+            worth = order_of(.5f * key_of(first) + (second != 0 ? .5f * key_of(second) : 0.f));  // halves, as in best_groups
             if (first == 0) worth = 0;
         }
         const int mine = lane / sh.group_lanes;
@@ -324,7 +325,7 @@ __device__ __forceinline__ bool choose_sorted(const RouteShape &sh, const float 
         const bool there = mine < sh.groups, kept = there && ahead < sh.top_groups;
         if (BIAS) {
             const unsigned last = __reduce_min_sync(kAll, kept ? worth : 0xffffffffu), next = __reduce_max_sync(kAll, there && !kept ? worth : 0u);
-            if (next != 0 && !apart(.5f * key_of(last), .5f * key_of(next))) return false;
+            if (next != 0 && !apart(key_of(last), key_of(next))) return false;
         }
         if (!kept) key[0] = 0;  // never taken, so none behind it is either
     }
