@@ -98,11 +98,13 @@ __global__ void __launch_bounds__(256)
     __shared__ int s_first[kMostExperts + 1], s_begin[kMostExperts + 1];
     __shared__ __align__(16) float s_a[kPlainStep][kPlainTile + 4], s_b[kPlainStep][kPlainTile + 4];  // read four at a time
     int e, lo, hi, m0, m_end, k_end;
-    const int n0 = blockIdx.x * kPlainTile;
-    if (GRAD) {
+    int n0 = blockIdx.x * kPlainTile;
+    if (GRAD) {  // the tiles of an expert along x, both ways
         e = blockIdx.z;
         rows_of(offsets, e, rows, &lo, &hi);
-        m0 = blockIdx.y * kPlainTile, m_end = m_size, k_end = hi - lo;
+        const unsigned across = ((unsigned)n_size + kPlainTile - 1) / kPlainTile, down = blockIdx.x / across;
+        n0 = (int)(blockIdx.x - down * across) * kPlainTile;
+        m0 = (int)down * kPlainTile, m_end = m_size, k_end = hi - lo;
     } else {
         load_offsets(offsets, experts, rows, s_begin);
         __syncthreads();
@@ -937,8 +939,9 @@ extern "C" alphasparse_status_t alphasparse_cuda_expert_mm_grad(alphasparse_cuda
         if (type == ALPHA_SPARSE_CUDA_TYPE_F16) go(__half());
         else go(__nv_bfloat16());
     } else {
-        if ((out + kPlainTile - 1) / kPlainTile > 65535) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
-        const dim3 grid((unsigned)((in + kPlainTile - 1) / kPlainTile), (unsigned)((out + kPlainTile - 1) / kPlainTile), (unsigned)experts);
+        const int64_t tiles = (in + kPlainTile - 1) / kPlainTile * ((out + kPlainTile - 1) / kPlainTile);
+        if (tiles > 0x7fffffff) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+        const dim3 grid((unsigned)tiles, 1, (unsigned)experts);
         const auto go = [&](auto t) {
             using T = decltype(t);
             if (weight_type == ALPHA_SPARSE_CUDA_TYPE_F32)
