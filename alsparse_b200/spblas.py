@@ -334,9 +334,11 @@ def _matrices(a):
 
 
 def _buffer(b):
-    """Address and bytes of a workspace: a contiguous array, or None."""
+    """Address and bytes of a workspace: a contiguous array, or None; (None, -1) if its elements are apart."""
     if b is None:
         return None, 0
+    if not (b.flags.c_contiguous if isinstance(b, np.ndarray) else b.is_contiguous()):
+        return None, -1
     return _ptr(b), b.nbytes
 
 
@@ -363,6 +365,8 @@ def embedding_grad(tokens, dy, alpha, beta, dtable, buffer):
     if t is None or d is None or o is None or d[0] != t[0] or d[1] != o[1]:
         return capi.INVALID_VALUE
     at, size = _buffer(buffer)
+    if size < 0:
+        return capi.INVALID_VALUE
     return capi.load().alphasparse_cuda_embedding_grad(_kind(tokens)[1], _kind(dy)[0], _kind(dtable)[0], t[0], t[2], t[1], o[0], o[1], alpha,
                                                        d[3], d[2], beta, o[3], o[2], at, size)
 
@@ -407,6 +411,8 @@ def expert_plan(index, offsets, slot, buffer):
     if i is None or s is None or o is None or i[:2] != s[:2] or o[1] != 1 or not _i32s(index) or not _i32s(offsets) or not _i32s(slot):
         return capi.INVALID_VALUE
     at, size = _buffer(buffer)
+    if size < 0:
+        return capi.INVALID_VALUE
     return capi.load().alphasparse_cuda_expert_plan(i[0], i[1], o[0] - 1, i[3], i[2], o[2], s[3], s[2], at, size)
 
 

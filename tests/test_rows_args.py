@@ -148,3 +148,17 @@ def test_shapes_and_types_of_the_experts_products():
     assert spblas.expert_mm_grad(o, y, x, 0.0, f((2, 8, 4), np.float16)) == capi.INVALID_VALUE
     assert spblas.expert_mm_grad(o, y, x[:5], 0.0, w) == capi.INVALID_VALUE
     assert call("expert_mm_status", None, 0) == capi.NOT_INITIALIZED
+
+
+def test_workspaces_whose_elements_are_apart():
+    """What lies between them is not the call's to write."""
+    f = np.zeros
+    t, dy, d = f(4, np.int64), f((4, 8), np.float32), f((9, 8), np.float32)
+    size = spblas.embedding_grad_buffer_size(4, 9, 8)[1]
+    apart = f(2 * size + 64, np.uint8)[::2]
+    assert apart.nbytes >= size and spblas.embedding_grad(t, dy, 1.0, 0.0, d, apart) == capi.INVALID_VALUE
+    index, size = f((9000, 2), np.int32), spblas.expert_plan_buffer_size(9000, 2, 8)[1]
+    apart = f((size, 2), np.uint8)[:, 0]
+    assert apart.nbytes >= size and spblas.expert_plan(index, f(9, np.int32), index.copy(), apart) == capi.INVALID_VALUE
+    whole = spblas.expert_plan(index, f(9, np.int32), index.copy(), f(size, np.uint8))
+    assert whole in (capi.EXECUTION_FAILED, capi.INVALID_POINTER)  # on to the check of the memory, which is the host's
