@@ -427,7 +427,8 @@ static cudaError_t launch_grad_sums(const GradSpace &sp, char *buffer, int64_t t
     };
     cudaError_t e;
     constexpr int full = 16 / sizeof(T);
-    // a pack of the input becomes one of as many elements of the output: both have to allow it
+    // A pack of the input becomes one of as many elements of the output: both have to allow it.  Rows on no 16-byte boundary go by
+    // one or two elements (16,384 x 2047 bf16 into 65,536 rows of fp32 198 us, 2048 wide 117; beta = 1: 79 and 53).
     if (vb == 16 && vo == 16) e = go(std::integral_constant<int, full>{});
     else if (sizeof(T) == 2 && vb >= 4 && vo >= 2 * (int)sizeof(TO)) e = go(std::integral_constant<int, 2>{});
     else e = go(std::integral_constant<int, 1>{});
@@ -515,7 +516,9 @@ extern "C" alphasparse_status_t alphasparse_cuda_embedding_grad(alphasparse_cuda
     int *ptr = reinterpret_cast<int *>(space + sp.ptr), *pos = reinterpret_cast<int *>(space + sp.pos),
         *row = reinterpret_cast<int *>(space + sp.row);
     // as many blocks as there are SMs, while their counts fit shared memory, however few rows that leaves each: the fewer it has,
-    // the more steps its second pass leaves out (300 rows, 131,072 tokens: 10 blocks of 32 rows 118 us, 100 of 3 97)
+    // the more steps its second pass leaves out (300 rows, 131,072 tokens: 10 blocks of 32 rows 118 us, 100 of 3 97).  Above
+    // 148 * 1024 rows there are more blocks than SMs, whose second wave reads all tokens again (64 wide, beta = 1, 16,384 /
+    // 131,072 tokens: 151,552 rows 27 / 95 us, 151,553 rows 31 / 100, 303,105 rows 38 / 130)
     const int own = (int)std::min<int64_t>(kGradMostRows, (vocab + 147) / 148);
     const unsigned blocks = (unsigned)((vocab + own - 1) / own);
     const size_t smem = sizeof(int) * kGradSortWarps * (size_t)own;

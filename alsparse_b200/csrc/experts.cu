@@ -170,8 +170,8 @@ struct PlanShape {
 
 // Threads along a token's row as row_shape lays them out: the row is read once and written to every place of the token.  ANY:
 // rows that begin on no 16-byte boundary; each place is cut at the boundaries of its memory, and the row read again at the
-// shift that it has to it, out of L1.  (12,001 tokens of 6 rows of 2047 fp16: 154 us in groups of a warp, 168 of a block.  Aligned,
-// 2880 wide bf16: 74 us in groups of a warp, so 70.)
+// shift that it has to it, out of L1.  (12,001 tokens of 6 rows of 2047 fp16: 90 us.  Groups of a warp against those of a block,
+// before the ends of rows were loaded as vectors: 154 and 168 us.  Aligned, 2880 wide bf16: 74 us in groups of a warp, so 70.)
 template <typename T, int U, bool ANY>
 __global__ void __launch_bounds__(kRowThreads)
     dispatch_kernel(int tokens, int k, int width, const T *__restrict__ x, int64_t ldx, Window all, const int *__restrict__ slot,

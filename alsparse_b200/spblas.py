@@ -343,7 +343,7 @@ def _buffer(b):
 
 
 def embedding(tokens, table, scale, y):
-    """alphasparse_cuda_embedding: y[i] = scale * table[tokens[i]].  tokens: one dimension of int32 or int64, any stride;
+    """alphasparse_cuda_embedding: y[i] = scale * table[tokens[i]].  tokens: one dimension of int32 or int64, at any distance above 0;
     table (vocab, width) and y (tokens, width) of one type, rows contiguous.  Returns the status."""
     t, e, o = _vector(tokens), _matrix(table), _matrix(y)
     if t is None or e is None or o is None or y.dtype != table.dtype or o[0] != t[0] or o[1] != e[1]:

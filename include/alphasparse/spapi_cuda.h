@@ -202,8 +202,8 @@ alphasparse_status_t alphasparse_d_mv_exchange(const double alpha, const alphasp
  *
  * All of them: every pointer is memory of the current device (or managed), else ALPHA_SPARSE_STATUS_INVALID_POINTER;
  * work is enqueued on the library stream and the call returns without waiting; nothing is allocated, kept from call to
- * call or shared between calls but the word of alphasparse_cuda_expert_mm_status (workspaces are the caller's: two calls that may overlap, and two captured graphs that
- * may run at the same time, take two), so the calls can be captured.  Dense operands are row-major with a leading
+ * call or shared between calls but the word of alphasparse_cuda_expert_mm_status (workspaces are the caller's: two calls
+ * that may overlap, and two captured graphs that may run at the same time, take two), so the calls can be captured.  Dense operands are row-major with a leading
  * dimension of at most 2^31 - 1 elements and any alignment that their elements allow; 16-byte aligned rows are fastest.
  * A missing operand is ALPHA_SPARSE_STATUS_NOT_INITIALIZED; sizes and enums out of range, leading dimensions below
  * the width and an output that lies in the place of another operand (different columns of rows of one length are
@@ -219,7 +219,7 @@ typedef enum {
 typedef enum { ALPHA_SPARSE_CUDA_INDEX_I32 = 0, ALPHA_SPARSE_CUDA_INDEX_I64 = 1 } alphasparse_cuda_index_t;
 typedef enum { ALPHA_SPARSE_CUDA_SCORE_SOFTMAX = 0, ALPHA_SPARSE_CUDA_SCORE_SIGMOID = 1 } alphasparse_cuda_score_t;
 
-/* Embedding lookup: y[i] = scale * table[token[i * inctoken]], i < tokens; y and table hold elements of `type`.  A
+/* Embedding lookup: y[i] = scale * table[token[i * inctoken]], i < tokens, inctoken at least 1; y and table hold elements of `type`.  A
  * token outside [0, vocab) selects nothing: its row of y is zero (padding; tokens of another part of a table that
  * is divided over GPUs). */
 alphasparse_status_t alphasparse_cuda_embedding(alphasparse_cuda_index_t index_type, alphasparse_cuda_type_t type,
@@ -273,8 +273,8 @@ alphasparse_status_t alphasparse_cuda_expert_plan(int64_t tokens, int64_t k, int
                                                   void *buffer, size_t buffer_bytes);
 
 /* xs[slot[t, j]] = x[t]; rows of xs that no slot names, those behind the last among them, are left as they were.  A slot
- * outside [0, rows) is empty; no two slots are the same (a plan's are not), or either row may be the one that is written.  The gradient of x is alphasparse_cuda_expert_combine of the gradient of xs with weight =
- * NULL. */
+ * outside [0, rows) is empty; no two slots are the same (a plan's are not), or either row may be the one that is
+ * written.  The gradient of x is alphasparse_cuda_expert_combine of the gradient of xs with weight = NULL. */
 alphasparse_status_t alphasparse_cuda_expert_dispatch(alphasparse_cuda_type_t type, int64_t tokens, int64_t k,
                                                       int64_t width, const void *x, int64_t ldx, const int32_t *slot,
                                                       int64_t lds, int64_t rows, void *xs, int64_t ldxs);
@@ -286,7 +286,7 @@ alphasparse_status_t alphasparse_cuda_expert_combine(alphasparse_cuda_type_t typ
                                                      float beta, void *out, int64_t ldo);
 
 /* Its gradients: dy[slot[t, j]] = weight[t, j] * dout[t] (other rows of dy are left as they were) and dweight[t, j] =
- * <dout[t], y[slot[t, j]]>, 0 for an empty slot. */
+ * <dout[t], y[slot[t, j]]>, 0 for an empty slot.  As for dispatch, no two slots are the same. */
 alphasparse_status_t alphasparse_cuda_expert_combine_grad(alphasparse_cuda_type_t type, int64_t tokens, int64_t k,
                                                           int64_t width, int64_t rows, const void *dout, int64_t ldo,
                                                           const void *y, int64_t ldy, const int32_t *slot, int64_t lds,
@@ -297,15 +297,16 @@ alphasparse_status_t alphasparse_cuda_expert_combine_grad(alphasparse_cuda_type_
  * row-major, out x in, at w + e * stride_w.  ALPHA_SPARSE_OPERATION_TRANSPOSE: x has `in` columns and y `out` (weights
  * stored an output feature a row); NON_TRANSPOSE: x has `out` columns and y `in` (weights stored the other way
  * round, and the gradient of x from that of y).  offsets (experts + 1 ints on the device) ascend within [0, rows]; rows of y
- * outside them are left as they were.  The matrices of two experts do not overlap.  F16 and BF16 whose rows begin on 16-byte
- * boundaries run on the tensor cores; F32 and others on the ordinary units, for completeness.  Up to 1024 experts. */
+ * outside them are left as they were.  The matrices of two experts stand one behind the other: stride_w is at least
+ * (out - 1) * ldw + in.  F16 and BF16 run on the tensor cores, at about a tenth of the rate where x or w has rows on no
+ * 16-byte boundary; F32 runs on the ordinary units, in full 32-bit products.  Up to 1024 experts. */
 alphasparse_status_t alphasparse_cuda_expert_mm(alphasparse_operation_t operation, alphasparse_cuda_type_t type,
                                                 int64_t experts, int64_t rows, const int32_t *offsets, int64_t out,
                                                 int64_t in, const void *x, int64_t ldx, const void *w, int64_t ldw,
                                                 int64_t stride_w, void *y, int64_t ldy);
 
 /* Gradient of the weights (operation TRANSPOSE): dw[e] = (sum over the rows r of e of dy[r]^T x[r]) + beta * dw[e], elements
- * of weight_type (that of dy and x, or F32); an expert without rows gets beta * dw[e].  For weights stored the other
+ * of weight_type (that of dy and x, or F32), stride_w as above; an expert without rows gets beta * dw[e].  For weights stored the other
  * way round exchange dy with x and out with in. */
 alphasparse_status_t alphasparse_cuda_expert_mm_grad(alphasparse_cuda_type_t type, alphasparse_cuda_type_t weight_type,
                                                      int64_t experts, int64_t rows, const int32_t *offsets, int64_t out,
