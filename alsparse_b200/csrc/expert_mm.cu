@@ -223,6 +223,14 @@ template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_wait(uint64_t *b, unsigned parity, volatile int *s_stop, long long work) {
     return __all_sync(0xffffffffu, barrier_wait<CLUSTER>(b, parity, s_stop, work));
 }
+// After the last copy: waits until every stage has been used for the last time, so that no arrival of a product comes to a block
+// that has ended (the products' arrivals on two barriers need not come in their order).  A stage that was never filled is free.
+__device__ __forceinline__ void last_uses(uint64_t *empty, int stage, unsigned phase, int stages, volatile int *s_stop, long long work) {
+    for (int i = 0; i < stages; i++) {
+        if (!warp_wait(&empty[stage], phase ^ 1, s_stop, work)) return;
+        if (++stage == stages) stage = 0, phase ^= 1;
+    }
+}
 // PAIR: `barrier` is an address of the cluster's, the other block's too
 template <bool PAIR>
 __device__ __forceinline__ void copy_tile(void *dst, const CUtensorMap *map, int x, int y, int z, unsigned barrier) {
@@ -551,6 +559,7 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
                 if (++stage == s.stages) stage = 0, phase ^= 1;
             }
         }
+        if (good) last_uses(s_empty, stage, phase, s.stages, s_stop, work);
     } else if (w == 1 && rank == 0 && elect_one()) {
         int stage = 0, count = 0;
         unsigned full_phases = 0, ready_phases = 0;  // a bit for each stage: the phase that comes next
@@ -664,6 +673,7 @@ __global__ void __launch_bounds__(ANY ? kMmThreadsAny : kMmThreads, 1)
                 if (++stage == s.stages) stage = 0, phase ^= 1;
             }
         }
+        if (good) last_uses(s_empty, stage, phase, s.stages, s_stop, work);
     } else if (FORM == kGradient && w >= 10) {
         // the ends of experts whose rows are no multiple of 16: rows of the next expert (or behind the last) came along with
         // the copy.  Zeros in both operands up to the next multiple, so that nothing that stands there, NaN included, gets

@@ -157,3 +157,37 @@ def test_a_wait_lasts_as_long_as_what_comes_before_it(tmp_path):
     assert len(waits) == 7 and all("s_stop, work)" in w for w in waits), waits
     roles = re.findall(r"mm_tile<FORM, PAIR>\(s, s_first, s_begin, t\);\n(.*)", body)
     assert len(roles) == 5 and all(r.strip() == "work += tile_work(q.steps);" for r in roles), roles
+
+
+STAGES = r"""
+#include <stdio.h>
+// A ring as the copies walk it: what they wait for after their last step is the last use of every stage, and nothing else.
+int main() {
+    long long wrong = 0;
+    for (int stages = 1; stages <= 8; stages++)
+        for (int steps = 0; steps < 60; steps++) {
+            int stage = 0, uses[8] = {};
+            unsigned phase = 0;
+            for (int k = 0; k < steps; k++) {
+                uses[stage]++;
+                if (++stage == stages) stage = 0, phase ^= 1;
+            }
+            for (int i = 0; i < stages; i++) {
+                // done once the phase that `uses` products complete is over: phases 0 .. uses - 1; none was ever begun for 0 uses
+                const unsigned parity = phase ^ 1;
+                wrong += parity != ((unsigned)(uses[stage] - 1) & 1u);
+                if (++stage == stages) stage = 0, phase ^= 1;
+            }
+        }
+    printf("%lld\n", wrong);
+    return wrong != 0;
+}
+"""
+
+
+def test_a_block_waits_for_the_last_use_of_every_stage(tmp_path):
+    run_on_host(tmp_path, STAGES)
+    kernel = open(os.path.join(build.CSRC, "expert_mm.cu")).read()
+    loops = re.findall(r"warp_wait\(&s_empty\[stage\], phase \^ 1, s_stop, work\)", kernel)
+    ends = re.findall(r"if \(good\) last_uses\(s_empty, stage, phase, s.stages, s_stop, work\);\n    \} else if", kernel)
+    assert len(loops) == len(ends) == 2  # copies by TMA, copies by warps
