@@ -34,7 +34,7 @@ ASB_HD int end_barrier(int warp, int stage) {
 
 // The limit of a wait.  What a wait may have to sit through is at most what its block has to do from its start to the end of the
 // tile at hand: `work`, the sum of tile_work over those tiles.  Two seconds, and 10 us for each unit (a step of 64 terms takes
-// 0.3 us, 2.5 us unaligned; a tile of the output 100 us at most, where old values are read element by element).
+// 0.3 us, 2.5 us unaligned; a tile of the output 64 us at most, where old values are read element by element).
 ASB_HD long long tile_work(int steps) {
     return (long long)steps + 32;
 }

@@ -203,8 +203,9 @@ alphasparse_status_t alphasparse_d_mv_exchange(const double alpha, const alphasp
  * All of them: every pointer is memory of the current device (or managed), else ALPHA_SPARSE_STATUS_INVALID_POINTER;
  * work is enqueued on the library stream and the call returns without waiting; nothing is allocated, kept from call to
  * call or shared between calls but the word of alphasparse_cuda_expert_mm_status (workspaces are the caller's: two calls
- * that may overlap, and two captured graphs that may run at the same time, take two), so the calls can be captured.  Dense operands are row-major with a leading
- * dimension of at most 2^31 - 1 elements and any alignment that their elements allow; 16-byte aligned rows are fastest.
+ * that may overlap, and two captured graphs that may run at the same time, take two), so the calls can be captured.
+ * Dense operands are row-major with a leading dimension of at most 2^31 - 1 elements and any alignment that their
+ * elements allow; 16-byte aligned rows are fastest.
  * A missing operand is ALPHA_SPARSE_STATUS_NOT_INITIALIZED; sizes and enums out of range, leading dimensions below
  * the width and an output that lies in the place of another operand (different columns of rows of one length are
  * different places) are ALPHA_SPARSE_STATUS_INVALID_VALUE.  Operands
@@ -219,8 +220,8 @@ typedef enum {
 typedef enum { ALPHA_SPARSE_CUDA_INDEX_I32 = 0, ALPHA_SPARSE_CUDA_INDEX_I64 = 1 } alphasparse_cuda_index_t;
 typedef enum { ALPHA_SPARSE_CUDA_SCORE_SOFTMAX = 0, ALPHA_SPARSE_CUDA_SCORE_SIGMOID = 1 } alphasparse_cuda_score_t;
 
-/* Embedding lookup: y[i] = scale * table[token[i * inctoken]], i < tokens, inctoken at least 1; y and table hold elements of `type`.  A
- * token outside [0, vocab) selects nothing: its row of y is zero (padding; tokens of another part of a table that
+/* Embedding lookup: y[i] = scale * table[token[i * inctoken]], i < tokens, inctoken at least 1; y and table hold
+ * elements of `type`.  A token outside [0, vocab) selects nothing: its row of y is zero (padding; tokens of another part of a table that
  * is divided over GPUs). */
 alphasparse_status_t alphasparse_cuda_embedding(alphasparse_cuda_index_t index_type, alphasparse_cuda_type_t type,
                                                 int64_t tokens, const void *token, int64_t inctoken, int64_t vocab,
@@ -306,8 +307,8 @@ alphasparse_status_t alphasparse_cuda_expert_mm(alphasparse_operation_t operatio
                                                 int64_t stride_w, void *y, int64_t ldy);
 
 /* Gradient of the weights (operation TRANSPOSE): dw[e] = (sum over the rows r of e of dy[r]^T x[r]) + beta * dw[e], elements
- * of weight_type (that of dy and x, or F32), stride_w as above; an expert without rows gets beta * dw[e].  For weights stored the other
- * way round exchange dy with x and out with in. */
+ * of weight_type (that of dy and x, or F32), stride_w as above; an expert without rows gets beta * dw[e].  For
+ * weights stored the other way round exchange dy with x and out with in. */
 alphasparse_status_t alphasparse_cuda_expert_mm_grad(alphasparse_cuda_type_t type, alphasparse_cuda_type_t weight_type,
                                                      int64_t experts, int64_t rows, const int32_t *offsets, int64_t out,
                                                      int64_t in, const void *dy, int64_t lddy, const void *x,
